@@ -25,6 +25,8 @@ LP_BWD_DW_BF16 = 2
 LP_BWD_NO_DW = 4
 LP_BWD_NO_DH = 8
 LP_HEAD_LOGPROBS = 1
+LP_DIST_MAX_TOKENS = 256
+LP_TOP_MAX = 128
 
 # Every symbol include/lp_logprob.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
@@ -71,6 +73,28 @@ _SIG = {
     "lp_head": (
         ctypes.c_int,
         [_P, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, _P, _I64, ctypes.c_int, _P, _P, _P, _P, ctypes.c_size_t],
+    ),
+    "lp_dist_fwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "lp_dist_fwd": (
+        ctypes.c_int,
+        [_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, ctypes.c_float, _P, _P, _P, _P, _P, _P, ctypes.c_size_t],
+    ),
+    "lp_dist_combine": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
+    "lp_dist_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, ctypes.c_int]),
+    "lp_dist_bwd": (
+        ctypes.c_int,
+        [_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, _P, _P, _P, _P, _P, _P, _I64, _P,
+         ctypes.c_int, _I64, _P, ctypes.c_size_t],
+    ),
+    "lp_top_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "lp_top": (
+        ctypes.c_int,
+        [_P, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, ctypes.c_int, _P, _P, _P, _P, _P, _P, ctypes.c_size_t],
+    ),
+    "lp_sample_top_k": (
+        ctypes.c_int,
+        [_P, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, ctypes.c_int, _P, ctypes.c_float, ctypes.c_float, _P, _P, _P,
+         ctypes.c_size_t],
     ),
     "lp_compact_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
     "lp_compact": (

@@ -14,6 +14,7 @@
 
 #include "../../include/lp_logprob.h"
 #include "lp_gemm.cuh"
+#include "lp_dist_kernels.cuh"
 #include "lp_plan.cuh"
 #include "lp_small_kernels.cuh"
 
@@ -385,7 +386,10 @@ int launch_gemm_cg(cudaStream_t st, const CUtensorMap& a, const CUtensorMap& b, 
   const int grid = CG * std::max(1, std::min(p.s.num_units, workers(di, CG)));
   GemmParams pp = p;
   pp.dbg = dbg_ptr(tag);
-  if (int rc = sched_slot(st, &pp.sched)) return rc;
+  // callers that keep a zeroed counter of their own (in their workspace) pass it in
+  if (pp.sched == nullptr) {
+    if (int rc = sched_slot(st, &pp.sched)) return rc;
+  }
   ProfScope prof(st, tag);
   if constexpr (CG == 1) {
     kern<<<grid, NUM_THREADS, smem, st>>>(a, b, o, pp);
@@ -825,9 +829,32 @@ struct MeshSum {
   unsigned long long limit_ns;
 };
 
+// The backward of given tokens' log-probabilities and the entropy (lp_dist_bwd): K tokens per row
+// and two row constants take the place of one target and its gradient.
+struct DistGrad {
+  int K;
+  int64_t V;  // the whole vocabulary
+  const float *zt, *lse, *entropy, *g, *ge;
+};
+
+// Scratch of lp_dist_bwd before the layout of lp_bwd: the work counters of every GEMM launch
+// (three per chunk), then the row constants. In the workspace, not in the library's rotating
+// slots, a counter belongs to the call (or to the captured graph) that zeroes it.
+struct DistBwdLayout {
+  size_t counters_bytes, row_off, base;
+};
+DistBwdLayout dist_bwd_layout(int64_t T, int64_t chunks) {
+  DistBwdLayout L;
+  L.counters_bytes = align_up((size_t)std::max<int64_t>(chunks, 1) * 3 * sizeof(unsigned), 1024);
+  L.row_off = L.counters_bytes;
+  L.base = L.row_off + align_up((size_t)T * 3 * sizeof(float), 1024);
+  return L;
+}
+
 int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs, int64_t v_off,
              const int32_t* y, float softcap, const float* norm, const float* g, void* dH, int64_t ld_dh, void* dW,
-             int flags, int64_t token_chunk, void* workspace, size_t workspace_bytes, const MeshSum* ms) {
+             int flags, int64_t token_chunk, void* workspace, size_t workspace_bytes, const MeshSum* ms,
+             const DistGrad* dist = nullptr) {
   int rc = check_common(H, T, d, ldh, W, Vs, y);
   if (rc) return rc;
   const bool want_dh = !(flags & LP_BWD_NO_DH), want_dw = !(flags & LP_BWD_NO_DW);
@@ -835,7 +862,7 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
   if (want_dh && (dH == nullptr || ld_dh < d || ld_dh % 8 != 0))
     return fail(LP_EINVAL, "dH must be non-null with ld_dh >= d and ld_dh %% 8 == 0");
   if (want_dw && dW == nullptr) return fail(LP_EINVAL, "null dW");
-  if (T > 0 && (norm == nullptr || g == nullptr)) return fail(LP_EINVAL, "null norm or g");
+  if (T > 0 && dist == nullptr && (norm == nullptr || g == nullptr)) return fail(LP_EINVAL, "null norm or g");
   DeviceInfo* di = nullptr;
   if ((rc = current_device_info(&di))) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -851,10 +878,24 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
     if (token_chunk < T) token_chunk = std::max<int64_t>(256, token_chunk / 256 * 256);
   }
   const BwdLayout L = bwd_layout(T, d, Vs, token_chunk, flags, workers(di, cg_dh), 128 * cg_dh);
-  if (workspace == nullptr || workspace_bytes < L.total)
-    return fail(LP_EWORKSPACE, "lp_bwd needs %zu workspace bytes, got %zu", L.total, workspace_bytes);
+  DistBwdLayout DL{};
+  if (dist != nullptr) DL = dist_bwd_layout(T, L.chunks);
+  if (workspace == nullptr || workspace_bytes < DL.base + L.total)
+    return fail(LP_EWORKSPACE, "%s needs %zu workspace bytes, got %zu", dist != nullptr ? "lp_dist_bwd" : "lp_bwd",
+                DL.base + L.total, workspace_bytes);
   if ((reinterpret_cast<uintptr_t>(workspace) & 1023) != 0) return fail(LP_EINVAL, "workspace must be 1024-byte aligned");
-  char* ws = reinterpret_cast<char*>(workspace);
+  unsigned* counters = nullptr;  // the next launch's work counter (dist only)
+  float* row_const = nullptr;
+  if (dist != nullptr) {
+    counters = reinterpret_cast<unsigned*>(workspace);
+    row_const = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + DL.row_off);
+    LP_CUDA_TRY(cudaMemsetAsync(counters, 0, DL.counters_bytes, st));
+    ProfScope prof(st, "dist_row_const");
+    dist_row_const_kernel<<<(unsigned)cdiv(T, 256), 256, 0, st>>>(dist->lse, dist->entropy, y, dist->g, dist->ge,
+                                                                  (int)T, dist->K, dist->V, row_const);
+    LP_LAUNCH_CHECK("dist_row_const_kernel");
+  }
+  char* ws = reinterpret_cast<char*>(workspace) + DL.base;
   __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>(ws + L.dz_off);
   float* part = reinterpret_cast<float*>(ws + L.part_off);
   float* dw_acc = (want_dw && dw_bf16 && L.chunks > 1) ? reinterpret_cast<float*>(ws + L.dwacc_off)
@@ -875,14 +916,29 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
       if ((rc = map_store_bf16(&to, dz, Vs, tcur, L.ldz, "dZ store"))) return rc;
       GemmParams p{};
       p.s = plan_dz(tcur, Vs, d, workers(di, cg_dz), 128 * cg_dz);
-      p.e.y = y + t0;
-      p.e.v_off = v_off;
       p.e.softcap = softcap;
-      p.e.g = g + t0;
-      p.e.stats = norm + t0;
-      p.e.stats_ld = T;
       set_hints(p, G_DZ);
-      if ((rc = launch_gemm_cap<EPI_BWD_DZ, false, false>(cap, st, ta, tb, to, p, di, "bwd_dz_gemm"))) return rc;
+      if (dist != nullptr) {
+        p.e.row_const = row_const + t0;
+        p.e.row_ld = T;
+        p.sched = counters++;
+        if ((rc = launch_gemm_cap<EPI_DIST_DZ, false, false>(cap, st, ta, tb, to, p, di, "dist_dz_gemm"))) return rc;
+        const int64_t slots = tcur * dist->K;
+        if (slots > 0) {
+          ProfScope prof(st, "dist_dz_targets");
+          dist_dz_targets_kernel<<<(unsigned)cdiv(slots, 256), 256, 0, st>>>(
+              y + t0 * dist->K, dist->zt + t0 * dist->K, dist->g != nullptr ? dist->g + t0 * dist->K : nullptr,
+              row_const + t0, T, (int)tcur, dist->K, v_off, Vs, softcap, dz, L.ldz);
+          LP_LAUNCH_CHECK("dist_dz_targets_kernel");
+        }
+      } else {
+        p.e.y = y + t0;
+        p.e.v_off = v_off;
+        p.e.g = g + t0;
+        p.e.stats = norm + t0;
+        p.e.stats_ld = T;
+        if ((rc = launch_gemm_cap<EPI_BWD_DZ, false, false>(cap, st, ta, tb, to, p, di, "bwd_dz_gemm"))) return rc;
+      }
     }
     // 2) dH[t0:t0+tcur] = dZ . W
     if (want_dh) {
@@ -930,6 +986,7 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
         p.e.split_rows = (int)L.mpad;
       }
       set_hints(p, G_DH);
+      if (counters != nullptr) p.sched = counters++;
       if ((rc = launch_gemm<EPI_STORE, false, true, false>(st, ta, tb, to, p, di, "bwd_dh_gemm"))) return rc;
       if (p.s.k_splits > 1) {
         const int64_t total = tcur * (d / 4);
@@ -962,6 +1019,7 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
         p.e.store_mode = c == 0 ? STORE_F32 : STORE_F32_ADD;
       }
       set_hints(p, G_DW);
+      if (counters != nullptr) p.sched = counters++;
       if ((rc = launch_gemm<EPI_STORE, true, true, false>(st, ta, tb, to, p, di, "bwd_dw_gemm"))) return rc;
     }
   }
@@ -1147,6 +1205,268 @@ int lp_peer_barrier(void* stream, const unsigned long long* signal_pads, int ran
                                              (unsigned long long)timeout_ms * 1000000ull);
   LP_LAUNCH_CHECK("peer_barrier_kernel");
   return LP_OK;
+}
+
+}  // extern "C"
+
+// ============================================================================= distribution operators
+namespace {
+
+// A pair's 256-row tile is half empty for at most 128 rows: those run as single CTAs.
+int cta_group_dist(int64_t T) {
+  const int f = forced_cta_group();
+  return f ? f : (T <= 128 ? 1 : cta_group_for(CG_FWD));
+}
+
+struct DistFwdLayout {
+  GemmSched s;
+  int cg;
+  size_t part_off, part_a_off, logits_off, total;
+};
+
+// Scratch of one launch over T rows: its work counter, the (max, S) and A partials, and (top) the
+// f32 logits.
+DistFwdLayout dist_fwd_layout(int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di, int sms, int64_t ld_logits) {
+  DistFwdLayout L{};
+  L.cg = cta_group_dist(T);
+  L.s = plan_fwd(T, Vs, d, di != nullptr ? workers(di, L.cg) : sms / L.cg, 128 * L.cg);
+  L.part_off = 256;
+  L.part_a_off = L.part_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float2), 256);
+  L.logits_off = L.part_a_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float), 256);
+  L.total = L.logits_off + align_up((size_t)T * ld_logits * sizeof(float), 256);
+  return L;
+}
+
+int check_dist(const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs, const int32_t* y,
+               int64_t K) {
+  if (K < 0 || K > LP_DIST_MAX_TOKENS) return fail(LP_EINVAL, "K=%lld tokens per row, at most %d", (long long)K,
+                                                    LP_DIST_MAX_TOKENS);
+  if (K > 0 && T > 0 && y == nullptr) return fail(LP_EINVAL, "null tokens");
+  static const int32_t none = 0;
+  return check_common(H, T, d, ldh, W, Vs, K > 0 ? y : &none);
+}
+
+// Rows per launch of the selection: their f32 logits stay within 1 GiB.
+int64_t top_rows(int64_t T, int64_t V) {
+  const int64_t ld = (V + 3) / 4 * 4;
+  return std::max<int64_t>(1, std::min<int64_t>(T, ((int64_t)1 << 30) / (ld * 4)));
+}
+
+size_t top_workspace(int64_t T, int64_t V, const DeviceInfo* di, int sms) {
+  const int64_t ld = (V + 3) / 4 * 4, rows = top_rows(T, V);
+  size_t need = dist_fwd_layout(rows, V, 64, di, sms, ld).total;
+  if (T % rows != 0) need = std::max(need, dist_fwd_layout(T % rows, V, 64, di, sms, ld).total);
+  return need;
+}
+
+// The selection of lp_top and lp_sample_top_k over all rows; `P` holds the outputs and options.
+int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t V, float softcap,
+             bool sample, TopParams P, void* workspace, size_t workspace_bytes) {
+  DeviceInfo* di = nullptr;
+  int rc = current_device_info(&di);
+  if (rc) return rc;
+  const size_t need = top_workspace(T, V, di, di->sms);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(LP_EWORKSPACE, "%zu workspace bytes needed, got %zu", need, workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return fail(LP_EINVAL, "workspace must be 256-byte aligned");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t ld = (V + 3) / 4 * 4, rows = top_rows(T, V);
+  char* ws = reinterpret_cast<char*>(workspace);
+  P.W = reinterpret_cast<const __nv_bfloat16*>(W);
+  P.ldh = ldh;
+  P.d = d;
+  P.V = V;
+  P.cap = softcap;
+  P.ld_logits = ld;
+  const TopParams all = P;
+  for (int64_t t0 = 0; t0 < T; t0 += rows) {
+    const int64_t n = std::min<int64_t>(rows, T - t0);
+    const DistFwdLayout L = dist_fwd_layout(n, V, d, di, di->sms, ld);
+    const __nv_bfloat16* Hc = reinterpret_cast<const __nv_bfloat16*>(H) + t0 * ldh;
+    alignas(64) CUtensorMap ta, tb, to;
+    if ((rc = map_bf16(&ta, Hc, d, n, ldh, BK, 128, "hidden"))) return rc;
+    if ((rc = map_bf16(&tb, W, d, V, d, BK, b_box_rows(L.cg), "embedding"))) return rc;
+    if ((rc = map_store_f32(&to, ws + L.logits_off, V, n, ld, "logits store"))) return rc;
+    LP_CUDA_TRY(cudaMemsetAsync(ws, 0, sizeof(unsigned), st));
+    GemmParams p{};
+    p.s = L.s;
+    p.sched = reinterpret_cast<unsigned*>(ws);
+    p.e.softcap = softcap;
+    p.e.part = reinterpret_cast<float2*>(ws + L.part_off);
+    p.e.part_a = reinterpret_cast<float*>(ws + L.part_a_off);
+    set_hints(p, G_FWD);
+    if ((rc = launch_gemm_cap<EPI_DIST_LOGITS, false, false>(softcap > 0.f, st, ta, tb, to, p, di, "top_gemm")))
+      return rc;
+    P = all;
+    P.part = p.e.part;
+    P.part_a = p.e.part_a;
+    P.n_parts = 2 * L.s.n_groups;
+    P.T = (int)n;
+    P.H = Hc;
+    P.logits = reinterpret_cast<const float*>(ws + L.logits_off);
+    ProfScope prof(st, "top_select");
+    if (sample) {
+      P.uniform = all.uniform + t0;
+      P.sampled = all.sampled + t0;
+      P.logps = all.logps + t0;
+      top_select_kernel<true><<<(unsigned)n, kTopThreads, 0, st>>>(P);
+    } else {
+      P.tokens = all.tokens != nullptr ? all.tokens + t0 : nullptr;
+      P.ids = all.ids + t0 * all.k;
+      P.logps = all.logps + t0 * all.k;
+      P.entropy = all.entropy + t0;
+      P.token_logps = all.token_logps != nullptr ? all.token_logps + t0 : nullptr;
+      top_select_kernel<false><<<(unsigned)n, kTopThreads, 0, st>>>(P);
+    }
+    LP_LAUNCH_CHECK("top_select_kernel");
+  }
+  return LP_OK;
+}
+
+int check_top(const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t V, int k) {
+  if (int rc = check_dist(H, T, d, ldh, W, V, nullptr, 0)) return rc;
+  if (k < 1 || k > LP_TOP_MAX || k > V)
+    return fail(LP_EINVAL, "k=%d must be between 1 and min(%d, V=%lld)", k, LP_TOP_MAX, (long long)V);
+  return LP_OK;
+}
+
+}  // namespace
+
+static_assert(kTopMax == LP_TOP_MAX, "LP_TOP_MAX");
+
+extern "C" {
+
+size_t lp_dist_fwd_workspace_bytes(int64_t T, int64_t Vs) {
+  DeviceInfo* di = nullptr;
+  const bool have = current_device_info(&di) == LP_OK;
+  if (T <= 0 || Vs <= 0) return 256;
+  return dist_fwd_layout(T, Vs, 64, have ? di : nullptr, 148, 0).total;
+}
+
+int lp_dist_fwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs,
+                int64_t v_off, const int32_t* y, int64_t K, float softcap, float* stats, float* zt, float* lse,
+                float* entropy, float* logp, void* workspace, size_t workspace_bytes) {
+  int rc = check_dist(H, T, d, ldh, W, Vs, y, K);
+  if (rc) return rc;
+  if (T == 0) return LP_OK;
+  DeviceInfo* di = nullptr;
+  if ((rc = current_device_info(&di))) return rc;
+  const DistFwdLayout L = dist_fwd_layout(T, Vs, d, di, di->sms, 0);
+  if (workspace == nullptr || workspace_bytes < L.total)
+    return fail(LP_EWORKSPACE, "lp_dist_fwd needs %zu workspace bytes, got %zu", L.total, workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return fail(LP_EINVAL, "workspace must be 256-byte aligned");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  char* ws = reinterpret_cast<char*>(workspace);
+  alignas(64) CUtensorMap ta, tb;
+  if ((rc = map_bf16(&ta, H, d, T, ldh, BK, 128, "hidden"))) return rc;
+  if ((rc = map_bf16(&tb, W, d, Vs, d, BK, b_box_rows(L.cg), "embedding"))) return rc;
+  LP_CUDA_TRY(cudaMemsetAsync(ws, 0, sizeof(unsigned), st));
+  GemmParams p{};
+  p.s = L.s;
+  p.sched = reinterpret_cast<unsigned*>(ws);
+  p.e.softcap = softcap;
+  p.e.part = reinterpret_cast<float2*>(ws + L.part_off);
+  p.e.part_a = reinterpret_cast<float*>(ws + L.part_a_off);
+  set_hints(p, G_FWD);
+  if ((rc = launch_gemm_cap<EPI_DIST, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "dist_fwd_gemm"))) return rc;
+  ProfScope prof(st, "dist_finalize");
+  const __nv_bfloat16* Hb = reinterpret_cast<const __nv_bfloat16*>(H);
+  const __nv_bfloat16* Wb = reinterpret_cast<const __nv_bfloat16*>(W);
+  const int n_parts = 2 * L.s.n_groups;
+  // eight rows per block share the 32-byte sectors of the partials; few rows get a block each
+  if (T < (int64_t)8 * di->sms)
+    dist_finalize_kernel<1><<<(unsigned)T, kDistThreads, 0, st>>>(p.e.part, p.e.part_a, n_parts, (int)T, Hb, ldh, Wb, d,
+                                                                  Vs, v_off, y, (int)K, softcap, stats, zt, lse, entropy,
+                                                                  logp);
+  else
+    dist_finalize_kernel<8><<<(unsigned)cdiv(T, 8), kDistThreads, 0, st>>>(p.e.part, p.e.part_a, n_parts, (int)T, Hb, ldh,
+                                                                           Wb, d, Vs, v_off, y, (int)K, softcap, stats,
+                                                                           zt, lse, entropy, logp);
+  LP_LAUNCH_CHECK("dist_finalize_kernel");
+  return LP_OK;
+}
+
+int lp_dist_combine(void* stream, const float* shard_stats, const float* shard_zt, int P, int64_t T, int64_t K,
+                    int64_t V, const int32_t* y, float* lse, float* entropy, float* zt, float* logp) {
+  if (P <= 0 || T < 0 || T > (int64_t)1 << 30) return fail(LP_EINVAL, "bad P=%d or T=%lld", P, (long long)T);
+  if (K < 0 || K > LP_DIST_MAX_TOKENS) return fail(LP_EINVAL, "K=%lld tokens per row, at most %d", (long long)K,
+                                                    LP_DIST_MAX_TOKENS);
+  if (T == 0) return LP_OK;
+  if (shard_stats == nullptr || lse == nullptr || entropy == nullptr)
+    return fail(LP_EINVAL, "null shard_stats, lse or entropy");
+  if (K > 0 && (shard_zt == nullptr || y == nullptr || zt == nullptr || logp == nullptr))
+    return fail(LP_EINVAL, "null shard_zt, tokens, zt or logp");
+  DeviceInfo* di = nullptr;
+  if (int rc = current_device_info(&di)) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  ProfScope prof(st, "dist_combine");
+  dist_combine_kernel<<<(unsigned)cdiv(T, 128), 128, 0, st>>>(shard_stats, shard_zt, P, (int)T, (int)K, V, y, lse,
+                                                              entropy, zt, logp);
+  LP_LAUNCH_CHECK("dist_combine_kernel");
+  return LP_OK;
+}
+
+size_t lp_dist_bwd_workspace_bytes(int64_t T, int64_t d, int64_t Vs, int64_t token_chunk, int flags) {
+  if (T <= 0 || Vs <= 0 || d <= 0) return 256;
+  const int64_t tc = token_chunk > 0 ? std::min<int64_t>(token_chunk, T) : default_token_chunk(T, Vs, d);
+  return dist_bwd_layout(T, cdiv(T, tc)).base + lp_bwd_workspace_bytes(T, d, Vs, token_chunk, flags);
+}
+
+int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs,
+                int64_t v_off, int64_t V, const int32_t* y, int64_t K, float softcap, const float* zt, const float* lse,
+                const float* entropy, const float* g_logp, const float* g_entropy, void* dH, int64_t ld_dh, void* dW,
+                int flags, int64_t token_chunk, void* workspace, size_t workspace_bytes) {
+  if (int rc = check_dist(H, T, d, ldh, W, Vs, y, K)) return rc;
+  if (v_off < 0 || v_off + Vs > V) return fail(LP_EINVAL, "shard [%lld, %lld) outside the vocabulary of %lld",
+                                               (long long)v_off, (long long)(v_off + Vs), (long long)V);
+  if (T > 0 && (lse == nullptr || entropy == nullptr || (K > 0 && zt == nullptr)))
+    return fail(LP_EINVAL, "null lse, entropy or zt");
+  static const int32_t none = 0;
+  const DistGrad dg{(int)K, V, zt, lse, entropy, K > 0 ? g_logp : nullptr, g_entropy};
+  return bwd_impl(stream, H, T, d, ldh, W, Vs, v_off, K > 0 ? y : &none, softcap, nullptr, nullptr, dH, ld_dh, dW, flags,
+                  token_chunk, workspace, workspace_bytes, nullptr, &dg);
+}
+
+size_t lp_top_workspace_bytes(int64_t T, int64_t V) {
+  DeviceInfo* di = nullptr;
+  const bool have = current_device_info(&di) == LP_OK;
+  if (T <= 0 || V <= 0) return 256;
+  return top_workspace(T, V, have ? di : nullptr, 148);
+}
+
+int lp_top(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t V, float softcap,
+           int k, const int32_t* tokens, int32_t* ids, float* logps, float* entropy, float* token_logps,
+           void* workspace, size_t workspace_bytes) {
+  if (int rc = check_top(H, T, d, ldh, W, V, k)) return rc;
+  if (T == 0) return LP_OK;
+  if (ids == nullptr || logps == nullptr || entropy == nullptr) return fail(LP_EINVAL, "null ids, logps or entropy");
+  if (tokens != nullptr && token_logps == nullptr) return fail(LP_EINVAL, "tokens need token_logps");
+  TopParams P{};
+  P.k = k;
+  P.tokens = tokens;
+  P.ids = ids;
+  P.logps = logps;
+  P.entropy = entropy;
+  P.token_logps = token_logps;
+  return top_impl(stream, H, T, d, ldh, W, V, softcap, false, P, workspace, workspace_bytes);
+}
+
+int lp_sample_top_k(void* stream, const void* H, int64_t B, int64_t d, int64_t ldh, const void* W, int64_t V,
+                    float softcap, int k, const float* uniform, float temperature, float top_p, int32_t* token,
+                    float* logp, void* workspace, size_t workspace_bytes) {
+  if (int rc = check_top(H, B, d, ldh, W, V, k)) return rc;
+  if (!(temperature > 0.f) || temperature > 3.4e38f) return fail(LP_EINVAL, "temperature must be finite and positive");
+  if (!(top_p > 0.f && top_p <= 1.f)) return fail(LP_EINVAL, "top_p must be in (0, 1]");
+  if (B == 0) return LP_OK;
+  if (uniform == nullptr || token == nullptr || logp == nullptr) return fail(LP_EINVAL, "null uniform, token or logp");
+  TopParams P{};
+  P.k = k;
+  P.uniform = uniform;
+  P.temperature = temperature;
+  P.top_p = top_p;
+  P.sampled = token;
+  P.logps = logp;
+  return top_impl(stream, H, B, d, ldh, W, V, softcap, true, P, workspace, workspace_bytes);
 }
 
 }  // extern "C"

@@ -32,6 +32,12 @@
 //   EPI_HEAD    : sampler head: softcapped logits stored as f32 (optional), running
 //                 (max, sum-exp) per row in base 2 and the first column of the row maximum;
 //                 one partial of each per row per unit and column half.
+//   EPI_DIST    : softcap + running (max m, S = sum 2^(z-m), A = sum 2^(z-m) (z-m)) per row in
+//                 base 2, from which the log-normaliser and the entropy follow.
+//   EPI_DIST_LOGITS : EPI_DIST, with the softcapped logits stored as f32.
+//   EPI_DIST_DZ : recompute path of log-probabilities and entropy; every column of
+//                 dZ = -p * (a + b * log2 p) * softcap' (two row constants), written as bf16 as
+//                 EPI_BWD_DZ does.
 //
 // Synchronisation (all waits bounded, see lp_ptx.cuh):
 //   full[s]   : TMA -> MMA. CG=2: lives in the leader, counts both CTAs' bytes.
@@ -80,7 +86,22 @@ constexpr int A_STAGE_BYTES = 128 * BK * 2;                // 16 KB: 128 rows of
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-enum : int { EPI_FWD_LSE = 0, EPI_BWD_DZ = 1, EPI_STORE = 2, EPI_HEAD = 3 };
+enum : int {
+  EPI_FWD_LSE = 0,
+  EPI_BWD_DZ = 1,
+  EPI_STORE = 2,
+  EPI_HEAD = 3,
+  EPI_DIST = 4,
+  EPI_DIST_LOGITS = 5,
+  EPI_DIST_DZ = 6
+};
+
+// Epilogues that only read the accumulator: no store staging, the deepest operand ring.
+template <int EPI>
+__host__ __device__ constexpr bool epi_stages_output() {
+  return EPI != EPI_FWD_LSE && EPI != EPI_DIST;
+}
+
 enum : int { STORE_BF16 = 0, STORE_F32 = 1, STORE_F32_ADD = 2 };
 
 template <int CG>
@@ -108,7 +129,7 @@ __host__ __device__ constexpr int staging_buf_bytes() {
 template <int CG, int EPI>
 __host__ __device__ constexpr int num_stages() {
   return CG == 1 ? LP_STAGES_CG1
-                 : (EPI == EPI_STORE ? LP_STAGES_CG2_STORE : (EPI == EPI_FWD_LSE ? LP_STAGES_CG2_FWD : LP_STAGES_CG2));
+                 : (EPI == EPI_STORE ? LP_STAGES_CG2_STORE : (epi_stages_output<EPI>() ? LP_STAGES_CG2 : LP_STAGES_CG2_FWD));
 }
 
 struct GemmSched {
@@ -136,6 +157,9 @@ struct EpiParams {
   float* tgt;            // FWD: [M] target logit (natural units), written by the owning tile
   float2* best;          // HEAD: [n_groups][M] (largest logit, its column as int bits)
   int store_logits;      // HEAD: store the logits through tmO (else only the row statistics)
+  float* part_a;         // DIST: [n_groups][M] running A (part holds the running max and S)
+  const float* row_const;  // DIST_DZ: [3][row_ld] per row: a, b, log2 of the normaliser
+  long long row_ld;        // DIST_DZ: row stride of row_const
   const float* g;        // DZ : [M] upstream d logp
   const float* stats;    // DZ : [2][stats_ld] global (max, sum) in natural units
   long long stats_ld;    // DZ : row stride of stats
@@ -260,7 +284,7 @@ __host__ __device__ __forceinline__ Unit get_unit(const GemmSched& s, int u) {
 template <int CG, int EPI>
 __host__ __device__ constexpr int staging_bytes() {
   // double-buffered box per epilogue warp
-  return EPI == EPI_FWD_LSE ? 0 : EPI_WARPS * 2 * staging_buf_bytes<CG, EPI>();
+  return epi_stages_output<EPI>() ? EPI_WARPS * 2 * staging_buf_bytes<CG, EPI>() : 0;
 }
 
 template <int CG, int EPI>
@@ -273,7 +297,10 @@ __host__ __device__ constexpr int gemm_smem_bytes() {
 static_assert(gemm_smem_bytes<1, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<1, EPI_BWD_DZ>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_STORE>() <= 232448 && gemm_smem_bytes<1, EPI_HEAD>() <= 232448 &&
                   gemm_smem_bytes<2, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<2, EPI_BWD_DZ>() <= 232448 &&
-                  gemm_smem_bytes<2, EPI_STORE>() <= 232448 && gemm_smem_bytes<2, EPI_HEAD>() <= 232448,
+                  gemm_smem_bytes<2, EPI_STORE>() <= 232448 && gemm_smem_bytes<2, EPI_HEAD>() <= 232448 &&
+                  gemm_smem_bytes<1, EPI_DIST>() <= 232448 && gemm_smem_bytes<2, EPI_DIST>() <= 232448 &&
+                  gemm_smem_bytes<1, EPI_DIST_LOGITS>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_LOGITS>() <= 232448 &&
+                  gemm_smem_bytes<1, EPI_DIST_DZ>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_DZ>() <= 232448,
               "GEMM shared memory above 227 KB");
 
 // Byte offset of 16-byte chunk c (0..3) of row r in a 64-byte-swizzled box of 64-byte rows
@@ -289,6 +316,19 @@ template <int RB>
 __device__ __forceinline__ uint32_t staging_offset(int r, int c) {
   if constexpr (RB == 128) return sw128_offset(r, c);
   else return sw64_offset(r, c);
+}
+
+// Moves the running (m, S, A) of a row to the maximum of m and `mx` (base 2). Nothing has been
+// summed while m is -inf, so the old sums count only from a finite m on.
+__device__ __forceinline__ void dist_rescale(float& m, float& s, float& a, float mx) {
+  const float nm = fmaxf(m, mx);
+  if (nm != m) {
+    const float dm = m - nm;
+    const float scale = m == -INFINITY ? 0.f : fast_ex2(dm);
+    a = m == -INFINITY ? 0.f : fmaf(s, dm, a) * scale;
+    s *= scale;
+    m = nm;
+  }
 }
 
 // ----------------------------------------------------------------------------- kernel
@@ -345,7 +385,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
-    if (EPI != EPI_FWD_LSE) prefetch_tmap(&tmO);
+    if (epi_stages_output<EPI>()) prefetch_tmap(&tmO);
   }
   if (warp == 1) {
     if (CG == 2) {
@@ -633,6 +673,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       float best_z = -INFINITY;  // HEAD: largest logit so far (natural units) and its column
       int best_i = -1;
       float gv = 0.f, l2 = 0.f;
+      float run_a = 0.f;               // DIST: sum of 2^(z - run_m) (z - run_m)
+      float row_a = 0.f, row_b = 0.f;  // DIST_DZ: the row's constants
+      if (EPI == EPI_DIST_DZ) {
+        if (row_ok) {
+          row_a = E.row_const[row];
+          row_b = E.row_const[E.row_ld + row];
+          l2 = E.row_const[2 * E.row_ld + row];
+        }
+      }
       if (EPI == EPI_FWD_LSE) {
         if (row_ok) {
           const long long t = (long long)E.y[row] - E.v_off;
@@ -826,6 +875,143 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               sb ^= 1;
             }
           }
+        } else if constexpr (EPI == EPI_DIST) {
+#pragma unroll 1
+          for (int c = 0; c < BN / 64; ++c) {
+            uint32_t r[32];
+            __syncwarp();
+            tmem_ld32(taddr + c * 32, r);
+            tmem_wait_ld(r);
+            const int nvalid = S.N - (colh + c * 32);  // columns >= nvalid are vocabulary padding (warp-uniform)
+            if (nvalid <= 0) continue;
+            float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float x = __uint_as_float(r[j]);
+              const float z = HAS_CAP ? fmaf(-2.f * c2, fast_rcp(1.f + fast_ex2(x * k1)), c2) : x * kLog2e;
+              r[j] = __float_as_uint(z);
+              if (j < nvalid) {
+                if (j & 1) mx1 = fmaxf(mx1, z); else mx0 = fmaxf(mx0, z);
+              }
+            }
+            dist_rescale(run_m, run_s, run_a, fmaxf(mx0, mx1));
+            // A's terms are all of one sign, so it keeps full relative accuracy however flat or
+            // peaked the row is; -(sum p z) + log-normaliser would cancel
+            float s0 = 0.f, s1 = 0.f, a0 = 0.f, a1 = 0.f;
+            if (nvalid >= 32) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                const float d0 = __uint_as_float(r[j]) - run_m, d1 = __uint_as_float(r[j + 1]) - run_m;
+                const float e0 = fast_ex2(d0), e1 = fast_ex2(d1);
+                s0 += e0;
+                s1 += e1;
+                a0 = fmaf(e0, d0, a0);
+                a1 = fmaf(e1, d1, a1);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (j < nvalid) {
+                  const float d0 = __uint_as_float(r[j]) - run_m;
+                  const float e0 = fast_ex2(d0);
+                  s0 += e0;
+                  a0 = fmaf(e0, d0, a0);
+                }
+              }
+            }
+            run_s += s0 + s1;
+            run_a += a0 + a1;
+          }
+        } else if constexpr (EPI == EPI_DIST_LOGITS) {
+          // the same over 16-column pieces, each also stored as natural-unit f32 logits
+#pragma unroll 1
+          for (int pc = 0; pc < BN / 32; ++pc) {
+            uint32_t r[16];
+            __syncwarp();
+            tmem_ld16(taddr + pc * 16, r);
+            tmem_wait_ld16(r);
+            const int col0 = colh + pc * 16;
+            const int nvalid = S.N - col0;
+            if (nvalid <= 0) continue;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float x = __uint_as_float(r[j]);
+              const float z = HAS_CAP ? fmaf(-2.f * cap, fast_rcp(1.f + fast_ex2(x * k1)), cap) : x;
+              r[j] = __float_as_uint(z);
+              if (j < nvalid) mx = fmaxf(mx, z);
+            }
+            dist_rescale(run_m, run_s, run_a, mx * kLog2e);
+            float s0 = 0.f, a0 = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              if (j < nvalid) {
+                const float d0 = fmaf(__uint_as_float(r[j]), kLog2e, -run_m);
+                const float e0 = fast_ex2(d0);
+                s0 += e0;
+                a0 = fmaf(e0, d0, a0);
+              }
+            }
+            run_s += s0;
+            run_a += a0;
+            if (lane == 0) bulk_wait_read<1>();
+            __syncwarp();
+            uint8_t* buf_s = my_staging + sb * SBUF;
+            const uint32_t sbase = smem_u32(buf_s);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              st_shared_v4(sbase + sw64_offset(lane, c), r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmO, buf_s, col0, row_base);
+              bulk_commit();
+            }
+            sb ^= 1;
+          }
+        } else if constexpr (EPI == EPI_DIST_DZ) {
+#pragma unroll 1
+          for (int pc = 0; pc < BN / 64; ++pc) {
+            uint32_t r[32];
+            __syncwarp();
+            tmem_ld32(taddr + pc * 32, r);
+            tmem_wait_ld(r);
+            const int col0 = colh + pc * 32;
+            // log2 p = z2 - l2, p = 2^(log2 p), dZ = -p * (a + b log2 p) * softcap'; the given
+            // tokens' own terms are written over these afterwards (dist_dz_targets_kernel)
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float v[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float x = __uint_as_float(r[2 * j + i]);
+                if (HAS_CAP) {
+                  const float rr = fast_rcp(1.f + fast_ex2(x * k1));
+                  const float lp = fmaf(-2.f * c2, rr, c2 - l2);
+                  v[i] = (-4.f * rr) * (1.f - rr) * (fast_ex2(lp) * fmaf(row_b, lp, row_a));
+                } else {
+                  const float lp = fmaf(x, kLog2e, -l2);
+                  v[i] = -fast_ex2(lp) * fmaf(row_b, lp, row_a);
+                }
+              }
+              pk[j] = pack_bf16x2(v[0], v[1]);
+            }
+            if (lane == 0) bulk_wait_read<1>();
+            __syncwarp();
+            uint8_t* buf_s = my_staging + sb * SBUF;
+            const uint32_t sbase = smem_u32(buf_s);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              st_shared_v4(sbase + sw64_offset(lane, c), pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmO, buf_s, col0, row_base);
+              bulk_commit();
+            }
+            sb ^= 1;
+          }
         } else {  // EPI_STORE
           const int row0 = un.split * E.split_rows + row_base;
           if (E.store_mode == STORE_BF16) {
@@ -960,11 +1146,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // one (max, sum) partial per unit and column half
         if (row_ok) E.part[(size_t)(un.group * 2 + h) * S.M + row] = make_float2(run_m, run_s);
       }
+      if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_LOGITS) {
+        if (row_ok) {
+          const size_t at = (size_t)(un.group * 2 + h) * S.M + row;
+          E.part[at] = make_float2(run_m, run_s);
+          E.part_a[at] = run_a;
+        }
+      }
       if constexpr (EPI == EPI_HEAD) {
         if (row_ok) E.best[(size_t)(un.group * 2 + h) * S.M + row] = make_float2(best_z, __int_as_float(best_i));
       }
     }
-    if (EPI != EPI_FWD_LSE) {
+    if (epi_stages_output<EPI>()) {
       if (lane == 0) bulk_wait<0>();  // all TMA stores of this warp complete before exit
       // the multicast stores are performed at system scope before the kernel ends, so a
       // peer barrier after this launch publishes them

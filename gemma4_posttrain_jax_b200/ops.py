@@ -176,6 +176,188 @@ def head(
     return logits, norm, top, top_logp
 
 
+def _dense_rows(h: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``h`` [T, d] as the distribution kernels read it: unit column stride, 16-byte aligned rows
+    that do not overlap (an expanded or oddly sliced ``h`` is copied); (view, row stride)."""
+    T, d = h.shape
+    ok = h.stride(1) == 1 and h.data_ptr() % 16 == 0 and (T == 1 or (h.stride(0) % 8 == 0 and h.stride(0) >= d))
+    if not ok:
+        h = h.clone(memory_format=torch.contiguous_format)
+    return h, int(h.stride(0)) if T > 1 else d
+
+
+def _dense_embed(w: torch.Tensor) -> torch.Tensor:
+    if w.is_contiguous() and w.data_ptr() % 16 == 0:
+        return w
+    return w.clone(memory_format=torch.contiguous_format)
+
+
+def _check_head(embed: torch.Tensor, hidden: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
+    dev = _require_cuda(embed, hidden, *others)
+    _check_bf16("embedding", embed)
+    _check_bf16("hidden", hidden)
+    return dev
+
+
+def dist_forward(
+    embed: torch.Tensor,
+    hidden: torch.Tensor,
+    tokens: torch.Tensor,
+    softcap: float | None,
+    *,
+    vocab_offset: int = 0,
+    shard: bool = False,
+) -> tuple[torch.Tensor, ...]:
+    """``lp_dist_fwd`` for int32 ``tokens`` [T, K]: (logp [T, K], entropy [T], zt [T, K], lse [T]),
+    or for one ``shard`` of the vocabulary (stats [3, T], zt [T, K])."""
+    dev = _check_head(embed, hidden, tokens)
+    lib = _lib.load()
+    T, K = tokens.shape
+    zt = torch.empty((T, K), dtype=torch.float32, device=dev)
+    stats = logp = row = None
+    if shard:
+        stats = torch.empty((3, T), dtype=torch.float32, device=dev)
+    else:
+        logp = torch.empty((T, K), dtype=torch.float32, device=dev)
+        row = torch.empty((2, T), dtype=torch.float32, device=dev)
+    if T > 0:
+        h, ldh = _dense_rows(hidden)
+        w = _dense_embed(embed)
+        with torch.cuda.device(dev):
+            ws, wsp, wsn = _workspace(lib.lp_dist_fwd_workspace_bytes(T, w.shape[0]), dev)
+            rc = lib.lp_dist_fwd(
+                _stream(dev), _ptr(h), T, h.shape[1], ldh, _ptr(w), w.shape[0], int(vocab_offset), _ptr(tokens), K,
+                float(softcap or 0.0), _ptr(stats), _ptr(zt), _ptr(row) if row is None else _ptr(row[0]),
+                None if row is None else _ptr(row[1]), _ptr(logp), wsp, wsn,
+            )
+        _lib.check(rc, "lp_dist_fwd")
+    return (stats, zt) if shard else (logp, row[1], zt, row[0])
+
+
+def dist_combine(
+    shard_stats: torch.Tensor, shard_zt: torch.Tensor, tokens: torch.Tensor, vocab: int
+) -> tuple[torch.Tensor, ...]:
+    """``lp_dist_combine``: [P, 3, T] and [P, T, K] -> (logp [T, K], entropy [T], zt [T, K], lse [T])."""
+    dev = _require_cuda(shard_stats, shard_zt, tokens)
+    lib = _lib.load()
+    T, K = tokens.shape
+    P = shard_stats.shape[0]
+    logp = torch.empty((T, K), dtype=torch.float32, device=dev)
+    zt = torch.empty((T, K), dtype=torch.float32, device=dev)
+    row = torch.empty((2, T), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.lp_dist_combine(
+            _stream(dev), _ptr(shard_stats.contiguous()), _ptr(shard_zt.contiguous()), P, T, K, int(vocab), _ptr(tokens),
+            _ptr(row[0]), _ptr(row[1]), _ptr(zt), _ptr(logp),
+        )
+    _lib.check(rc, "lp_dist_combine")
+    return logp, row[1], zt, row[0]
+
+
+def dist_backward(
+    embed: torch.Tensor,
+    hidden: torch.Tensor,
+    tokens: torch.Tensor,
+    softcap: float | None,
+    zt: torch.Tensor,
+    lse: torch.Tensor,
+    entropy: torch.Tensor,
+    grad_logp: torch.Tensor | None,
+    grad_entropy: torch.Tensor | None,
+    *,
+    vocab_offset: int = 0,
+    vocab: int | None = None,
+    need_dh: bool = True,
+    need_dw: bool = True,
+    dh_dtype: torch.dtype = torch.bfloat16,
+    dw_dtype: torch.dtype = torch.bfloat16,
+    token_chunk: int | None = None,
+) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """``lp_dist_bwd``: (dH [T, d], partial over this shard; dW [Vs, d]) of f32 ``grad_logp`` [T, K]
+    and ``grad_entropy`` [T] (either may be None). ``vocab`` is the whole vocabulary's size."""
+    dev = _check_head(embed, hidden, tokens, zt, lse, entropy, grad_logp, grad_entropy)
+    lib = _lib.load()
+    T, K = tokens.shape
+    Vs, d = embed.shape
+    flags = 0
+    dH = dW = None
+    if need_dh:
+        dH = torch.empty((T, d), dtype=dh_dtype, device=dev)
+        flags |= _lib.LP_BWD_DH_F32 if dh_dtype == torch.float32 else 0
+    else:
+        flags |= _lib.LP_BWD_NO_DH
+    if need_dw:
+        dW = torch.empty((Vs, d), dtype=dw_dtype, device=dev)
+        flags |= _lib.LP_BWD_DW_BF16 if dw_dtype == torch.bfloat16 else 0
+    else:
+        flags |= _lib.LP_BWD_NO_DW
+    h, ldh = _dense_rows(hidden) if T > 0 else (hidden, d)
+    w = _dense_embed(embed)
+    chunk = int(token_chunk) if token_chunk else 0
+    with torch.cuda.device(dev):
+        ws, wsp, wsn = _workspace(lib.lp_dist_bwd_workspace_bytes(T, d, Vs, chunk, flags), dev)
+        rc = lib.lp_dist_bwd(
+            _stream(dev), _ptr(h), T, d, ldh, _ptr(w), Vs, int(vocab_offset), int(vocab) if vocab else Vs, _ptr(tokens), K,
+            float(softcap or 0.0), _ptr(zt), _ptr(lse), _ptr(entropy), _ptr(grad_logp), _ptr(grad_entropy), _ptr(dH), d,
+            _ptr(dW), flags, chunk, wsp, wsn,
+        )
+    _lib.check(rc, "lp_dist_bwd")
+    return dH, dW
+
+
+def top(
+    embed: torch.Tensor, hidden: torch.Tensor, softcap: float | None, k: int, tokens: torch.Tensor | None = None
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """``lp_top``: (ids int32 [T, k], logps [T, k], entropy [T], logps of int32 ``tokens`` [T] or None)."""
+    dev = _check_head(embed, hidden, tokens)
+    lib = _lib.load()
+    T, V = hidden.shape[0], embed.shape[0]
+    ids = torch.empty((T, k), dtype=torch.int32, device=dev)
+    logps = torch.empty((T, k), dtype=torch.float32, device=dev)
+    entropy = torch.empty((T,), dtype=torch.float32, device=dev)
+    token_logps = torch.empty((T,), dtype=torch.float32, device=dev) if tokens is not None else None
+    if T > 0:
+        h, ldh = _dense_rows(hidden)
+        w = _dense_embed(embed)
+        with torch.cuda.device(dev):
+            ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(T, V), dev)
+            rc = lib.lp_top(
+                _stream(dev), _ptr(h), T, h.shape[1], ldh, _ptr(w), V, float(softcap or 0.0), int(k), _ptr(tokens),
+                _ptr(ids), _ptr(logps), _ptr(entropy), _ptr(token_logps), wsp, wsn,
+            )
+        _lib.check(rc, "lp_top")
+    return ids, logps, entropy, token_logps
+
+
+def sample_top_k(
+    embed: torch.Tensor,
+    hidden: torch.Tensor,
+    softcap: float | None,
+    uniform: torch.Tensor,
+    *,
+    temperature: float,
+    top_k: int,
+    top_p: float,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``lp_sample_top_k``: (token int32 [B], logp [B]) for f32 ``uniform`` [B]."""
+    dev = _check_head(embed, hidden, uniform)
+    lib = _lib.load()
+    B, V = hidden.shape[0], embed.shape[0]
+    token = torch.empty((B,), dtype=torch.int32, device=dev)
+    logp = torch.empty((B,), dtype=torch.float32, device=dev)
+    if B > 0:
+        h, ldh = _dense_rows(hidden)
+        w = _dense_embed(embed)
+        with torch.cuda.device(dev):
+            ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(B, V), dev)
+            rc = lib.lp_sample_top_k(
+                _stream(dev), _ptr(h), B, h.shape[1], ldh, _ptr(w), V, float(softcap or 0.0), int(top_k), _ptr(uniform),
+                float(temperature), float(top_p), _ptr(token), _ptr(logp), wsp, wsn,
+            )
+        _lib.check(rc, "lp_sample_top_k")
+    return token, logp
+
+
 def combine(shard_stats: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``lp_combine``: [P, 3, T] per-shard triples -> (logp [T], normalization [2, T])."""
     dev = _require_cuda(shard_stats)

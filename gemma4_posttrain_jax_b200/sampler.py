@@ -14,9 +14,12 @@ same).
 
 from __future__ import annotations
 
+import math
+
 import torch
 
-from . import ops
+from . import _lib, ops
+from .losses import _validate_softcap
 
 
 def _rows_of(hidden: torch.Tensor) -> torch.Tensor:
@@ -87,3 +90,42 @@ def sample_token(
     lse = norm[0] + torch.log(norm[1])
     logp = torch.gather(logits, 1, token[:, None])[:, 0] - lse
     return token.to(torch.int32), logp
+
+
+def sample_top_k(
+    embed_tokens: torch.Tensor,
+    hidden: torch.Tensor,
+    softcap: float | None,
+    uniform: torch.Tensor,
+    *,
+    temperature: float,
+    top_k: int,
+    top_p: float = 1.0,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``sample_token``'s temperature / top-k / top-p draw for 1 <= top_k <= min(128, V), by given
+    random numbers: (token int32 [B], logp f32 [B]) of hidden [B, d].
+
+    ``uniform`` f32 [B] in [0, 1) picks each row's token by inverting the cumulative distribution of
+    the filtered tokens in descending order (the lowest id first among equals), so equal inputs draw
+    equal tokens. The distribution is ``sample_token``'s; the logits are neither sorted nor
+    returned, nothing waits on the host, and the call can be captured into a CUDA graph that is
+    replayed with new hidden states and random numbers. logp is the token's log-probability under
+    the full, untempered policy.
+    """
+    if hidden.ndim != 2:
+        raise ValueError(f"hidden must be [B, d], got {tuple(hidden.shape)}")
+    if embed_tokens.ndim != 2 or hidden.shape[-1] != embed_tokens.shape[-1]:
+        raise ValueError(f"incompatible embedding {tuple(embed_tokens.shape)} and hidden {tuple(hidden.shape)}")
+    _validate_softcap(softcap)
+    if not (math.isfinite(temperature) and temperature > 0):
+        raise ValueError("temperature must be finite and positive (sample_token decodes greedily)")
+    if not 1 <= top_k <= min(_lib.LP_TOP_MAX, embed_tokens.shape[0]):
+        raise ValueError(f"top_k must be between 1 and min({_lib.LP_TOP_MAX}, {embed_tokens.shape[0]}), got {top_k}")
+    if not 0.0 < top_p <= 1.0:
+        raise ValueError("top_p must be in (0, 1]")
+    if tuple(uniform.shape) != (hidden.shape[0],) or uniform.dtype != torch.float32:
+        raise ValueError(f"uniform must be float32 [{hidden.shape[0]}], got {uniform.dtype} {tuple(uniform.shape)}")
+    return ops.sample_top_k(
+        embed_tokens.detach(), hidden.detach(), softcap, uniform.contiguous(), temperature=float(temperature),
+        top_k=int(top_k), top_p=float(top_p),
+    )

@@ -263,6 +263,90 @@ LP_API int lp_head(void* stream, const void* H, int64_t B, int64_t d, int64_t ld
                    float softcap, float* logits, int64_t ld_logits, int flags, float* norm, int32_t* argmax,
                    float* argmax_logp, void* workspace, size_t workspace_bytes);
 
+/* ---- distribution operators: several given tokens, entropy, the most likely tokens ----
+ *
+ * With log p[t, v] = z[t, v] - lse[t], lse[t] = log sum_v exp(z[t, v]):
+ *     entropy[t] = -sum_v p log p
+ * They have no counterpart in the reference. Their work counters live in the caller's
+ * workspace (256-byte aligned; 1024-byte aligned for lp_dist_bwd), so calls with workspaces of
+ * their own never share state: calls on several streams and replays of several captured graphs
+ * may overlap.
+ */
+
+/* Most given tokens per row, and most tokens lp_top / lp_sample_top_k select. */
+#define LP_DIST_MAX_TOKENS 256
+#define LP_TOP_MAX 128
+
+/* Scratch bytes lp_dist_fwd needs for T rows against a shard of Vs rows. */
+LP_API size_t lp_dist_fwd_workspace_bytes(int64_t T, int64_t Vs);
+
+/*
+ * Log-probabilities of K given tokens per row and the row's entropy, over one vocabulary shard.
+ *   y        int32 [T, K] global ids, K <= LP_DIST_MAX_TOKENS (NULL with K == 0); ids outside
+ *            [v_off, v_off + Vs) are not owned
+ *   stats    f32 [3, T] or NULL: shard max m, sum exp(z - m), sum exp(z - m) (z - m)
+ *   zt       f32 [T, K] or NULL: the tokens' logits, 0 where not owned
+ *   lse, entropy  f32 [T] or NULL, logp  f32 [T, K] or NULL: meaningful when the shard is the
+ *            whole vocabulary; logp is 0 for an id outside it
+ */
+LP_API int lp_dist_fwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs,
+                       int64_t v_off, const int32_t* y, int64_t K, float softcap, float* stats, float* zt, float* lse,
+                       float* entropy, float* logp, void* workspace, size_t workspace_bytes);
+
+/*
+ * Merge of P shards: shard_stats f32 [P, 3, T] and shard_zt f32 [P, T, K] (lp_dist_fwd's stats
+ * and zt of every shard) into the lse, entropy, zt and logp of the whole vocabulary of V rows.
+ */
+LP_API int lp_dist_combine(void* stream, const float* shard_stats, const float* shard_zt, int P, int64_t T, int64_t K,
+                           int64_t V, const int32_t* y, float* lse, float* entropy, float* zt, float* logp);
+
+/* Scratch bytes lp_dist_bwd needs; token_chunk <= 0 selects the default chunk. */
+LP_API size_t lp_dist_bwd_workspace_bytes(int64_t T, int64_t d, int64_t Vs, int64_t token_chunk, int flags);
+
+/*
+ * Backward of lp_dist_fwd over one shard of a vocabulary of V rows:
+ *   dZ[t, v] = softcap'(z) * (sum_k g_logp[t, k] [y[t, k] = v]
+ *                             - p * (sum_k g_logp[t, k] + g_entropy[t] * (log p + entropy[t])))
+ *   dH = dZ . W (partial over this shard), dW = dZ^T . H
+ * (the first sum inside the brackets runs over the ids of [0, V) only; dZ is rounded to bf16).
+ *   zt, lse, entropy   the forward's (merged over the shards)
+ *   g_logp   f32 [T, K] or NULL (no gradient)      g_entropy  f32 [T] or NULL
+ * dH, dW, flags, token_chunk as lp_bwd.
+ */
+LP_API int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs,
+                       int64_t v_off, int64_t V, const int32_t* y, int64_t K, float softcap, const float* zt,
+                       const float* lse, const float* entropy, const float* g_logp, const float* g_entropy, void* dH,
+                       int64_t ld_dh, void* dW, int flags, int64_t token_chunk, void* workspace,
+                       size_t workspace_bytes);
+
+/* Scratch bytes lp_top and lp_sample_top_k need for T rows against V vocabulary rows. */
+LP_API size_t lp_top_workspace_bytes(int64_t T, int64_t V);
+
+/*
+ * The k most likely tokens of each row, 1 <= k <= min(LP_TOP_MAX, V), over the whole vocabulary.
+ * They are ranked by their dot products H[t] . W[v] in f64, the lowest id first among equals.
+ *   tokens       int32 [T] or NULL: one given token per row
+ *   ids          int32 [T, k]; logps f32 [T, k]: their log-probabilities, most likely first
+ *   entropy      f32 [T]
+ *   token_logps  f32 [T] (with tokens): log-probability of the given token, 0 for an id outside
+ *                [0, V)
+ */
+LP_API int lp_top(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t V,
+                  float softcap, int k, const int32_t* tokens, int32_t* ids, float* logps, float* entropy,
+                  float* token_logps, void* workspace, size_t workspace_bytes);
+
+/*
+ * One token per row from the temperature / top-k / top-p filtered distribution, by inversion of
+ * its cumulative distribution in descending order: with w_j = exp((z_j - z_0) / temperature) over
+ * lp_top's k tokens, token j is kept while w_0 + .. + w_(j-1) < top_p * sum w (the first always),
+ * and the drawn one is the first whose kept cumulative weight exceeds uniform * kept weight.
+ *   uniform  f32 [B] in [0, 1)          temperature > 0, 0 < top_p <= 1
+ *   token    int32 [B]; logp f32 [B]: its log-probability under the unfiltered, untempered policy
+ */
+LP_API int lp_sample_top_k(void* stream, const void* H, int64_t B, int64_t d, int64_t ldh, const void* W, int64_t V,
+                           float softcap, int k, const float* uniform, float temperature, float top_p, int32_t* token,
+                           float* logp, void* workspace, size_t workspace_bytes);
+
 /* Scratch bytes lp_compact needs for B * N response slots. */
 LP_API size_t lp_compact_workspace_bytes(int64_t B, int64_t N);
 

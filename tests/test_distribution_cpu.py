@@ -1,0 +1,124 @@
+"""Refusals of the distribution operators, none of which reaches a GPU."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from gemma4_posttrain_jax_b200 import _lib, build, sample_top_k, token_logps_and_entropy, top_token_logps
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _lib.LIB_PATH.exists():
+        build.build()
+    return _lib.load()
+
+
+W = torch.zeros((10, 16), dtype=torch.bfloat16)
+H = torch.zeros((2, 3, 16), dtype=torch.bfloat16)
+Y = torch.zeros((2, 3), dtype=torch.int64)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"tokens": Y[:1]}, "does not match"),
+    ({"tokens": Y.reshape(3, 2)}, "does not match"),
+    ({"tokens": Y.reshape(2, 3, 1, 1)}, "does not match"),
+    ({"tokens": Y.float()}, "integers"),
+    ({"tokens": Y.bool()}, "integers"),
+    ({"tokens": torch.zeros((2, 3, 257), dtype=torch.int32)}, "at most 256"),
+    ({"hidden": H[..., :8]}, "incompatible"),
+    ({"embed_tokens": W[0]}, "incompatible"),
+    ({"embed_tokens": W[:0]}, "no rows"),
+    ({"softcap": 0.0}, "softcap"),
+    ({"softcap": float("nan")}, "softcap"),
+    ({"backend": "pallas"}, "entropy"),
+    ({"backend": "triton"}, "unknown logprob backend"),
+    ({}, "CUDA tensors"),
+])  # fmt: skip
+def test_logps_refusals(change, message):
+    args = {"embed_tokens": W, "hidden": H, "tokens": Y, "softcap": 30.0} | change
+    embed, hidden, tokens = (args.pop(name) for name in ("embed_tokens", "hidden", "tokens"))
+    with pytest.raises(ValueError, match=message):
+        token_logps_and_entropy(embed, hidden, tokens, **args)
+
+
+@pytest.mark.parametrize("args,tokens,message", [
+    ((W, H, 30.0, 0), None, "k must be"),
+    ((W, H, 30.0, 11), None, "k must be"),
+    ((torch.zeros((500, 16)), H, 30.0, 129), None, "k must be"),
+    ((W, H, -1.0, 2), None, "softcap"),
+    ((W, H[..., :8], None, 2), None, "incompatible"),
+    ((W, H, None, 2), Y[:1], "does not match"),
+    ((W, H, None, 2), Y.float(), "integers"),
+    ((W, H, None, 2), None, "CUDA tensors"),
+])  # fmt: skip
+def test_top_refusals(args, tokens, message):
+    with pytest.raises(ValueError, match=message):
+        top_token_logps(*args, tokens=tokens)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"hidden": H}, r"\[B, d\]"),
+    ({"embed_tokens": W[:, :8]}, "incompatible"),
+    ({"softcap": 0.0}, "softcap"),
+    ({"temperature": 0.0}, "temperature"),
+    ({"temperature": float("inf")}, "temperature"),
+    ({"top_k": 0}, "top_k"),
+    ({"top_k": 11}, "top_k"),
+    ({"top_p": 0.0}, "top_p"),
+    ({"top_p": 1.5}, "top_p"),
+    ({"top_p": float("nan")}, "top_p"),
+    ({"uniform": torch.zeros(5)}, "uniform"),
+    ({"uniform": torch.zeros(6, dtype=torch.float64)}, "uniform"),
+    ({}, "CUDA tensors"),
+])  # fmt: skip
+def test_sample_refusals(change, message):
+    args = {"embed_tokens": W, "hidden": H.reshape(6, 16), "softcap": 30.0, "uniform": torch.zeros(6), "temperature": 1.0,
+            "top_k": 4} | change
+    first = [args.pop(name) for name in ("embed_tokens", "hidden", "softcap", "uniform")]
+    with pytest.raises(ValueError, match=message):
+        sample_top_k(*first, **args)
+
+
+def test_c_entries_refuse_before_the_device(lib):
+    P = ctypes.c_void_p
+    fake = P(4096)
+
+    def refused(rc, fragment):
+        assert rc == _lib.LP_EINVAL and fragment in lib.lp_last_error().decode()
+
+    def fwd(T=4, d=8, ldh=8, K=2, y=fake):
+        return lib.lp_dist_fwd(None, fake, T, d, ldh, fake, 10, 0, y, K, 0.0, None, fake, fake, fake, fake, fake, 1 << 20)
+
+    refused(fwd(d=12), "multiple of 8")
+    refused(fwd(ldh=4), "ldh")
+    refused(fwd(T=-1), "bad sizes")
+    refused(fwd(K=257), "at most 256")
+    refused(fwd(K=-1), "at most 256")
+    refused(fwd(y=None), "null tokens")
+    refused(lib.lp_dist_combine(None, fake, fake, 0, 4, 1, 10, fake, fake, fake, fake, fake), "bad P")
+    refused(lib.lp_dist_combine(None, fake, None, 2, 4, 1, 10, fake, fake, fake, fake, fake), "null shard_zt")
+
+    def bwd(v_off=0, V=10, zt=fake, dH=fake, dW=fake):
+        return lib.lp_dist_bwd(None, fake, 4, 8, 8, fake, 10, v_off, V, fake, 2, 0.0, zt, fake, fake, fake, fake, dH, 8, dW, 0,
+                               0, fake, 1 << 20)
+
+    refused(bwd(v_off=5), "outside the vocabulary")
+    refused(bwd(zt=None), "null lse")
+    refused(bwd(dH=None), "dH")
+    refused(bwd(dW=None), "dW")
+    for k in (0, 11, 129):
+        refused(lib.lp_top(None, fake, 4, 8, 8, fake, 10, 0.0, k, None, fake, fake, fake, None, fake, 1 << 20), "k=")
+    refused(lib.lp_top(None, fake, 4, 8, 8, fake, 10, 0.0, 2, fake, fake, fake, fake, None, fake, 1 << 20), "token_logps")
+
+    def draw(temperature=1.0, top_p=1.0, uniform=fake):
+        return lib.lp_sample_top_k(None, fake, 4, 8, 8, fake, 10, 0.0, 2, uniform, temperature, top_p, fake, fake, fake, 1 << 20)
+
+    refused(draw(temperature=0.0), "temperature")
+    refused(draw(temperature=float("nan")), "temperature")
+    refused(draw(top_p=0.0), "top_p")
+    refused(draw(top_p=1.5), "top_p")
+    refused(draw(uniform=None), "null uniform")
