@@ -1221,19 +1221,19 @@ int cta_group_dist(int64_t T) {
 struct DistFwdLayout {
   GemmSched s;
   int cg;
-  size_t part_off, part_a_off, logits_off, total;
+  size_t part_off, part_a_off, keys_off, total;
 };
 
 // Scratch of one launch over T rows: its work counter, the (max, S) and A partials, and (top) the
-// f32 logits.
-DistFwdLayout dist_fwd_layout(int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di, int sms, int64_t ld_logits) {
+// rows' selection keys.
+DistFwdLayout dist_fwd_layout(int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di, int sms, size_t key_row_bytes) {
   DistFwdLayout L{};
   L.cg = cta_group_dist(T);
   L.s = plan_fwd(T, Vs, d, di != nullptr ? workers(di, L.cg) : sms / L.cg, 128 * L.cg);
   L.part_off = 256;
   L.part_a_off = L.part_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float2), 256);
-  L.logits_off = L.part_a_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float), 256);
-  L.total = L.logits_off + align_up((size_t)T * ld_logits * sizeof(float), 256);
+  L.keys_off = L.part_a_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float), 256);
+  L.total = L.keys_off + align_up((size_t)T * key_row_bytes, 256);
   return L;
 }
 
@@ -1246,47 +1246,74 @@ int check_dist(const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, 
   return check_common(H, T, d, ldh, W, Vs, K > 0 ? y : &none);
 }
 
-// Rows per launch of the selection: their f32 logits stay within 1 GiB.
-int64_t top_rows(int64_t T, int64_t V) {
-  const int64_t ld = (V + 3) / 4 * 4;
-  return std::max<int64_t>(1, std::min<int64_t>(T, ((int64_t)1 << 30) / (ld * 4)));
+// Selection keys of a row. From kTopGroupRatio groups of 32 columns per selected token on, two
+// values per group: an eighth of the bytes of the f32 logits to write and to search, and few groups
+// that hold two of the most likely tokens, whose 32 columns have to be scored again. Fewer groups
+// and the logits themselves are the keys.
+constexpr int kTopGroupRatio = 8;
+struct TopKeys {
+  bool groups;
+  int64_t ld;  // keys per row in memory
+  int n;       // keys per row
+  size_t row_bytes;
+  int64_t rows;  // rows per launch: their keys stay within 1 GiB
+};
+TopKeys top_keys(int64_t T, int64_t V, int k) {
+  TopKeys K;
+  K.groups = cdiv(V, kTopGroup) >= (int64_t)kTopGroupRatio * k;
+  K.n = (int)(K.groups ? cdiv(V, kTopGroup) : V);
+  K.ld = K.groups ? cdiv(V, BN) * (BN / kTopGroup) : (V + 3) / 4 * 4;
+  K.row_bytes = (size_t)K.ld * (K.groups ? sizeof(float2) : sizeof(float));
+  K.rows = std::max<int64_t>(1, std::min<int64_t>(T, (int64_t)(((size_t)1 << 30) / K.row_bytes)));
+  return K;
 }
 
-size_t top_workspace(int64_t T, int64_t V, const DeviceInfo* di, int sms) {
-  const int64_t ld = (V + 3) / 4 * 4, rows = top_rows(T, V);
-  size_t need = dist_fwd_layout(rows, V, 64, di, sms, ld).total;
-  if (T % rows != 0) need = std::max(need, dist_fwd_layout(T % rows, V, 64, di, sms, ld).total);
+size_t top_workspace(int64_t T, int64_t V, int k, const DeviceInfo* di, int sms) {
+  const TopKeys K = top_keys(T, V, k);
+  size_t need = dist_fwd_layout(K.rows, V, 64, di, sms, K.row_bytes).total;
+  if (T % K.rows != 0) need = std::max(need, dist_fwd_layout(T % K.rows, V, 64, di, sms, K.row_bytes).total);
   return need;
 }
 
-// The selection of lp_top and lp_sample_top_k over all rows; `P` holds the outputs and options.
+template <bool SAMPLE, bool GROUPS>
+int launch_top_select(cudaStream_t st, TopParams& P, int64_t rows) {
+  const size_t key_bytes = (size_t)P.n_keys * sizeof(uint32_t);
+  P.keys_in_smem = key_bytes <= (size_t)kTopKeyBytes;
+  const size_t smem = std::max<size_t>(P.keys_in_smem ? key_bytes : 0, kTopCandBytes);
+  auto kern = top_select_kernel<SAMPLE, GROUPS>;
+  static bool configured[kMaxDevices] = {};
+  int dev = 0;
+  LP_CUDA_TRY(cudaGetDevice(&dev));
+  if (!configured[dev]) {
+    LP_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTopKeyBytes));
+    configured[dev] = true;
+  }
+  ProfScope prof(st, "top_select");
+  kern<<<(unsigned)rows, kTopThreads, smem, st>>>(P);
+  LP_LAUNCH_CHECK("top_select_kernel");
+  return LP_OK;
+}
+
+// The selection of lp_top and lp_sample_top_k over all rows; `all` holds the outputs and options.
 int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t V, float softcap,
-             bool sample, TopParams P, void* workspace, size_t workspace_bytes) {
+             bool sample, const TopParams& all, void* workspace, size_t workspace_bytes) {
   DeviceInfo* di = nullptr;
   int rc = current_device_info(&di);
   if (rc) return rc;
-  const size_t need = top_workspace(T, V, di, di->sms);
+  const TopKeys K = top_keys(T, V, all.k);
+  const size_t need = top_workspace(T, V, all.k, di, di->sms);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(LP_EWORKSPACE, "%zu workspace bytes needed, got %zu", need, workspace_bytes);
   if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return fail(LP_EINVAL, "workspace must be 256-byte aligned");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int64_t ld = (V + 3) / 4 * 4, rows = top_rows(T, V);
   char* ws = reinterpret_cast<char*>(workspace);
-  P.W = reinterpret_cast<const __nv_bfloat16*>(W);
-  P.ldh = ldh;
-  P.d = d;
-  P.V = V;
-  P.cap = softcap;
-  P.ld_logits = ld;
-  const TopParams all = P;
-  for (int64_t t0 = 0; t0 < T; t0 += rows) {
-    const int64_t n = std::min<int64_t>(rows, T - t0);
-    const DistFwdLayout L = dist_fwd_layout(n, V, d, di, di->sms, ld);
+  for (int64_t t0 = 0; t0 < T; t0 += K.rows) {
+    const int64_t n = std::min<int64_t>(K.rows, T - t0);
+    const DistFwdLayout L = dist_fwd_layout(n, V, d, di, di->sms, K.row_bytes);
     const __nv_bfloat16* Hc = reinterpret_cast<const __nv_bfloat16*>(H) + t0 * ldh;
     alignas(64) CUtensorMap ta, tb, to;
     if ((rc = map_bf16(&ta, Hc, d, n, ldh, BK, 128, "hidden"))) return rc;
     if ((rc = map_bf16(&tb, W, d, V, d, BK, b_box_rows(L.cg), "embedding"))) return rc;
-    if ((rc = map_store_f32(&to, ws + L.logits_off, V, n, ld, "logits store"))) return rc;
     LP_CUDA_TRY(cudaMemsetAsync(ws, 0, sizeof(unsigned), st));
     GemmParams p{};
     p.s = L.s;
@@ -1295,30 +1322,42 @@ int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
     p.e.part = reinterpret_cast<float2*>(ws + L.part_off);
     p.e.part_a = reinterpret_cast<float*>(ws + L.part_a_off);
     set_hints(p, G_FWD);
-    if ((rc = launch_gemm_cap<EPI_DIST_LOGITS, false, false>(softcap > 0.f, st, ta, tb, to, p, di, "top_gemm")))
-      return rc;
-    P = all;
+    if (K.groups) {
+      p.e.top = reinterpret_cast<float2*>(ws + L.keys_off);
+      rc = launch_gemm_cap<EPI_DIST_TOP, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "top_gemm");
+    } else {
+      if ((rc = map_store_f32(&to, ws + L.keys_off, V, n, K.ld, "logits store"))) return rc;
+      rc = launch_gemm_cap<EPI_DIST_LOGITS, false, false>(softcap > 0.f, st, ta, tb, to, p, di, "top_gemm");
+    }
+    if (rc) return rc;
+    TopParams P = all;
     P.part = p.e.part;
     P.part_a = p.e.part_a;
     P.n_parts = 2 * L.s.n_groups;
     P.T = (int)n;
     P.H = Hc;
-    P.logits = reinterpret_cast<const float*>(ws + L.logits_off);
-    ProfScope prof(st, "top_select");
+    P.ldh = ldh;
+    P.W = reinterpret_cast<const __nv_bfloat16*>(W);
+    P.d = d;
+    P.V = V;
+    P.cap = softcap;
+    if (K.groups) P.groups = p.e.top; else P.logits = reinterpret_cast<const float*>(ws + L.keys_off);
+    P.ld_keys = K.ld;
+    P.n_keys = K.n;
     if (sample) {
       P.uniform = all.uniform + t0;
       P.sampled = all.sampled + t0;
       P.logps = all.logps + t0;
-      top_select_kernel<true><<<(unsigned)n, kTopThreads, 0, st>>>(P);
+      rc = K.groups ? launch_top_select<true, true>(st, P, n) : launch_top_select<true, false>(st, P, n);
     } else {
       P.tokens = all.tokens != nullptr ? all.tokens + t0 : nullptr;
       P.ids = all.ids + t0 * all.k;
       P.logps = all.logps + t0 * all.k;
       P.entropy = all.entropy + t0;
       P.token_logps = all.token_logps != nullptr ? all.token_logps + t0 : nullptr;
-      top_select_kernel<false><<<(unsigned)n, kTopThreads, 0, st>>>(P);
+      rc = K.groups ? launch_top_select<false, true>(st, P, n) : launch_top_select<false, false>(st, P, n);
     }
-    LP_LAUNCH_CHECK("top_select_kernel");
+    if (rc) return rc;
   }
   return LP_OK;
 }
@@ -1427,11 +1466,11 @@ int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, 
                   token_chunk, workspace, workspace_bytes, nullptr, &dg);
 }
 
-size_t lp_top_workspace_bytes(int64_t T, int64_t V) {
+size_t lp_top_workspace_bytes(int64_t T, int64_t V, int k) {
   DeviceInfo* di = nullptr;
   const bool have = current_device_info(&di) == LP_OK;
-  if (T <= 0 || V <= 0) return 256;
-  return top_workspace(T, V, have ? di : nullptr, 148);
+  if (T <= 0 || V <= 0 || k < 1) return 256;
+  return top_workspace(T, V, k, have ? di : nullptr, 148);
 }
 
 int lp_top(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t V, float softcap,

@@ -230,14 +230,22 @@ __global__ void dist_dz_targets_kernel(const int32_t* __restrict__ y, const floa
 
 // ----------------------------------------------------------------------------- selection
 // The k most likely tokens of a row, in the order of the exact dot products h . W_v (softcap is
-// monotone), the lowest id first among equals. The GEMM's f32 logits only nominate candidates:
-// the k + kTopSpare largest are scored again in f64 and ranked by that, so a rounding of the f32
-// accumulation can exchange neighbours only if more than kTopSpare logits lie within it of the
-// k-th.
+// monotone), the lowest id first among equals. The GEMM only nominates: a key is either one
+// accumulator (f32) or the largest of 32 neighbours with the second largest beside it. The
+// k + kTopSpare largest keys are selected; of a selected group every column is a candidate if its
+// second largest reaches the k-th largest value seen, else only its largest is. Candidates are
+// scored again in f64 and ranked by that, so a rounding of the nomination (f32 accumulation, 2^-18
+// for a group's low bits) can exchange neighbours only if more than kTopSpare values lie within it
+// of the k-th.
 constexpr int kTopMax = 128;
 constexpr int kTopSpare = 16;
-constexpr int kTopCand = 1024;  // candidate slots
+constexpr int kTopGroup = 32;
 constexpr int kTopThreads = 512;
+// selected keys: at most k + 2 kTopSpare, or any number up to this of equal ones
+constexpr int kTopSel = kTopMax + 2 * kTopSpare;
+constexpr int kTopCand = kTopSel * kTopGroup;
+constexpr int kTopCandBytes = kTopCand * (int)(sizeof(double) + sizeof(int));
+constexpr int kTopKeyBytes = 200 * 1024 - 16 * 1024;  // keys kept in shared memory, beside the static part
 
 // Order-preserving map of f32 to u32; NaN comes last.
 __device__ __forceinline__ uint32_t ordered_key(float x) {
@@ -245,6 +253,8 @@ __device__ __forceinline__ uint32_t ordered_key(float x) {
   const uint32_t b = __float_as_uint(x);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+// A group's value without its column bits.
+__device__ __forceinline__ float group_value(float x) { return __uint_as_float(__float_as_uint(x) & ~31u); }
 
 struct TopParams {
   const float2* part;
@@ -256,8 +266,11 @@ struct TopParams {
   const __nv_bfloat16* W;
   long long d, V;
   float cap;
-  const float* logits;  // [T, ld_logits]
-  long long ld_logits;
+  const float* logits;  // [T, ld_keys] accumulators, or
+  const float2* groups;  // [T, ld_keys] the two largest of every 32
+  long long ld_keys;
+  int n_keys;
+  int keys_in_smem;
   int k;
   const int32_t* tokens;  // [T] or null
   int32_t* ids;           // top: [T, k]
@@ -266,117 +279,179 @@ struct TopParams {
   float* token_logps;     // top: [T] (with tokens)
   const float* uniform;   // sample: [T] in [0, 1)
   float temperature, top_p;
-  int32_t* sampled;       // sample: [T]
+  int32_t* sampled;  // sample: [T]
 };
 
-__device__ __forceinline__ int block_sum(int v, int* warp_s, int* out_s) {
+__device__ __forceinline__ int block_sum(int v, int* warp_s) {
   v = __reduce_add_sync(0xffffffffu, v);
   if ((threadIdx.x & 31) == 0) warp_s[threadIdx.x >> 5] = v;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    int x = threadIdx.x < blockDim.x / 32 ? warp_s[threadIdx.x] : 0;
-    x = __reduce_add_sync(0xffffffffu, x);
-    if (threadIdx.x == 0) *out_s = x;
-  }
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < kTopThreads / 32; ++w) sum += warp_s[w];
   __syncthreads();
-  return *out_s;
+  return sum;
 }
 
-template <bool SAMPLE>
+template <bool SAMPLE, bool GROUPS>
 __global__ void __launch_bounds__(kTopThreads) top_select_kernel(const TopParams P) {
-  __shared__ DistAcc acc_s[kTopThreads];
-  __shared__ int warp_s[32];
-  __shared__ int sum_s, n_cand_s;
-  __shared__ int cand_id[kTopCand];
-  __shared__ double cand_z[kTopCand];
+  // keys while selecting, then the candidates' f64 scores and ids
+  extern __shared__ __align__(16) uint8_t dyn_s[];
+  uint32_t* keys_s = reinterpret_cast<uint32_t*>(dyn_s);
+  double* cand_z = reinterpret_cast<double*>(dyn_s);
+  int* cand_id = reinterpret_cast<int*>(dyn_s + kTopCand * sizeof(double));
+  __shared__ DistAcc acc_s[kTopThreads / 32];
+  __shared__ int warp_s[kTopThreads / 32];
+  __shared__ int n_sel_s, n_cand_s;
+  __shared__ int sel_key[kTopSel];
+  __shared__ float sel_v[2 * kTopSel];  // values of the selected keys: [0, n) largest, [n, 2n) second
+  __shared__ float kth_s;
   __shared__ double best_z[kTopMax];
   __shared__ int best_id[kTopMax];
   const int t = blockIdx.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n_keys = (int)P.V;
-  const float* keys = P.logits + (size_t)t * P.ld_logits;
+  const int n_keys = P.n_keys;
+  const __nv_bfloat16* h = P.H + (size_t)t * P.ldh;
 
+  auto load_key = [&](int i) -> uint32_t {
+    if constexpr (GROUPS) return ordered_key(group_value(P.groups[(size_t)t * P.ld_keys + i].x));
+    else return ordered_key(P.logits[(size_t)t * P.ld_keys + i]);
+  };
+  auto key = [&](int i) -> uint32_t { return P.keys_in_smem ? keys_s[i] : load_key(i); };
+
+  // a row of zeros: every logit is exactly 0
+  int nonzero = 0;
+  for (long long i = tid; i < P.d / 8; i += kTopThreads) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(h) + i);
+    nonzero |= ((a.x | a.y | a.z | a.w) & 0x7fff7fffu) != 0u;
+  }
+  if (P.keys_in_smem)
+    for (int i = tid; i < n_keys; i += kTopThreads) keys_s[i] = load_key(i);
   // row statistics
   DistAcc acc{-INFINITY, 0.f, 0.f};
   for (int g = tid; g < P.n_parts; g += kTopThreads) {
     const float2 p = P.part[(size_t)g * P.T + t];
     acc = dist_merge(acc, DistAcc{p.x, p.y, P.part_a[(size_t)g * P.T + t]});
   }
-  acc_s[tid] = acc;
-  if (tid == 0) n_cand_s = 0;
-  __syncthreads();
-  for (int o = kTopThreads / 2; o > 0; o >>= 1) {
-    if (tid < o) acc_s[tid] = dist_merge(acc_s[tid], acc_s[tid + o]);
-    __syncthreads();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    DistAcc b;
+    b.m = __shfl_xor_sync(0xffffffffu, acc.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, acc.s, o);
+    b.a = __shfl_xor_sync(0xffffffffu, acc.a, o);
+    acc = (lane & o) ? dist_merge(b, acc) : dist_merge(acc, b);
   }
+  if (lane == 0) acc_s[warp] = acc;
+  if (tid == 0) n_sel_s = n_cand_s = 0;
+  nonzero = __syncthreads_or(nonzero);
   acc = acc_s[0];
+#pragma unroll
+  for (int w = 1; w < kTopThreads / 32; ++w) acc = dist_merge(acc, acc_s[w]);
   const float lse = dist_lse(acc);
 
-  // Bisection on the ordered keys: count(key >= lo) >= n always holds, count(key >= hi) < n.
-  const int n = min(n_keys, P.k + kTopSpare);
-  uint32_t lo = 0u;
-  unsigned long long hi = 1ull << 32;
-  int c_lo = n_keys;
-  while (c_lo > n + kTopSpare && hi - lo > 1) {
-    const uint32_t mid = (uint32_t)(lo + (hi - lo) / 2);
-    int c = 0;
-    for (int i = tid; i < n_keys; i += kTopThreads) c += ordered_key(keys[i]) >= mid ? 1 : 0;
-    c = block_sum(c, warp_s, &sum_s);
-    if (c >= n) {
-      lo = mid;
-      c_lo = c;
-    } else {
-      hi = mid;
+  if (nonzero) {
+    // Bisection on the ordered keys: count(key >= lo) >= n always holds, count(key >= hi) < n.
+    const int n = min(n_keys, P.k + kTopSpare);
+    uint32_t lo = 0u;
+    unsigned long long hi = 1ull << 32;
+    int c_lo = n_keys;
+    while (c_lo > n + kTopSpare && hi - lo > 1) {
+      const uint32_t mid = (uint32_t)(lo + (hi - lo) / 2);
+      int c = 0;
+      for (int i = tid; i < n_keys; i += kTopThreads) c += key(i) >= mid ? 1 : 0;
+      c = block_sum(c, warp_s);
+      if (c >= n) {
+        lo = mid;
+        c_lo = c;
+      } else {
+        hi = mid;
+      }
     }
-  }
-  const bool ties = c_lo > kTopCand;  // then hi = lo + 1: more equal keys than slots
-  for (int i = tid; i < n_keys; i += kTopThreads) {
-    const uint32_t key = ordered_key(keys[i]);
-    if (ties ? key > lo : key >= lo) cand_id[atomicAdd(&n_cand_s, 1)] = i;
+    const bool ties = c_lo > kTopSel;  // then hi = lo + 1: more equal keys than slots
+    for (int i = tid; i < n_keys; i += kTopThreads) {
+      const uint32_t x = key(i);
+      if (ties ? x > lo : x >= lo) sel_key[atomicAdd(&n_sel_s, 1)] = i;
+    }
+    __syncthreads();
+    if (ties) {
+      // fewer than n keys lie above the tie; fill up to n with the lowest of the tie
+      int have = n_sel_s;
+      __syncthreads();
+      for (int base = 0; base < n_keys && have < n; base += kTopThreads) {
+        const int i = base + tid;
+        const bool hit = i < n_keys && key(i) == lo;
+        const unsigned ballot = __ballot_sync(0xffffffffu, hit);
+        if (lane == 0) warp_s[warp] = __popc(ballot);
+        __syncthreads();
+        int before = 0, total = 0;
+        for (int w = 0; w < kTopThreads / 32; ++w) {
+          before += w < warp ? warp_s[w] : 0;
+          total += warp_s[w];
+        }
+        const int slot = have + before + __popc(ballot & ((1u << lane) - 1u));
+        if (hit && slot < n) sel_key[slot] = i;
+        have = min(n, have + total);
+        __syncthreads();
+      }
+      if (tid == 0) n_sel_s = n;
+      __syncthreads();
+    }
+    const int n_sel = n_sel_s;  // the keys in shared memory are not read below
+    if constexpr (GROUPS) {
+      float b0 = -INFINITY, b1 = -INFINITY;
+      if (tid < n_sel) {
+        const float2 g = P.groups[(size_t)t * P.ld_keys + sel_key[tid]];
+        b0 = g.x;
+        b1 = group_value(g.y);
+        sel_v[tid] = group_value(b0);
+        sel_v[n_sel + tid] = b1;
+      }
+      if (tid == 0) kth_s = -INFINITY;
+      __syncthreads();
+      // the k-th largest of the values seen is a lower bound of the k-th largest logit
+      for (int i = tid; i < 2 * n_sel; i += kTopThreads) {
+        const float v = sel_v[i];
+        int above = 0;
+        for (int j = 0; j < 2 * n_sel; ++j) above += (sel_v[j] > v || (sel_v[j] == v && j < i)) ? 1 : 0;
+        if (above == P.k - 1) kth_s = v;
+      }
+      __syncthreads();
+      if (tid < n_sel) {
+        const long long first = (long long)sel_key[tid] * kTopGroup;
+        const int cols = (int)min((long long)kTopGroup, P.V - first);
+        // 2^-16 of slack for the accumulation and the bits cut off
+        const float least = kth_s - 1.52587890625e-05f * fabsf(kth_s);
+        if (!(b1 < least)) {
+          const int at = atomicAdd(&n_cand_s, cols);
+          for (int c = 0; c < cols; ++c) cand_id[at + c] = (int)first + c;
+        } else {
+          cand_id[atomicAdd(&n_cand_s, 1)] = (int)first + (int)(__float_as_uint(b0) & 31u);
+        }
+      }
+    } else {
+      if (tid < n_sel) cand_id[tid] = sel_key[tid];
+      if (tid == 0) n_cand_s = n_sel;
+    }
+  } else {
+    if (tid < P.k) cand_id[tid] = tid;
+    if (tid == 0) n_cand_s = P.k;
   }
   __syncthreads();
-  if (ties) {
-    // fewer than n keys lie above the tie; fill up to n with the lowest ids of the tie
-    int have = n_cand_s;
-    __syncthreads();
-    for (int base = 0; base < n_keys && have < n; base += kTopThreads) {
-      const int i = base + tid;
-      const bool hit = i < n_keys && ordered_key(keys[i]) == lo;
-      const unsigned ballot = __ballot_sync(0xffffffffu, hit);
-      if (lane == 0) warp_s[warp] = __popc(ballot);
-      __syncthreads();
-      int before = 0, total = 0;
-      for (int w = 0; w < kTopThreads / 32; ++w) {
-        before += w < warp ? warp_s[w] : 0;
-        total += warp_s[w];
-      }
-      const int slot = have + before + __popc(ballot & ((1u << lane) - 1u));
-      if (hit && slot < n) cand_id[slot] = i;
-      have = min(n, have + total);
-      __syncthreads();
-    }
-    if (tid == 0) n_cand_s = n;
-    __syncthreads();
-  }
   const int n_cand = n_cand_s;
 
-  const __nv_bfloat16* h = P.H + (size_t)t * P.ldh;
   for (int i = warp; i < n_cand; i += kTopThreads / 32) {
     const double z = warp_dot_f64(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);
-    if (lane == 0) cand_z[i] = z;
+    if (lane == 0) cand_z[i] = z == z ? z : -INFINITY;  // a NaN ranks last
   }
   __syncthreads();
-  // rank by (z descending, id ascending); a NaN ranks as -inf
+  // rank by (z descending, id ascending)
   for (int i = tid; i < n_cand; i += kTopThreads) {
-    const double z = cand_z[i] == cand_z[i] ? cand_z[i] : -INFINITY;
+    const double z = cand_z[i];
     const int id = cand_id[i];
     int rank = 0;
-    for (int j = 0; j < n_cand; ++j) {
-      const double o = cand_z[j] == cand_z[j] ? cand_z[j] : -INFINITY;
-      rank += (o > z || (o == z && cand_id[j] < id)) ? 1 : 0;
-    }
+    for (int j = 0; j < n_cand; ++j) rank += (cand_z[j] > z || (cand_z[j] == z && cand_id[j] < id)) ? 1 : 0;
     if (rank < P.k) {
-      best_z[rank] = P.cap > 0.f ? (double)P.cap * tanh(cand_z[i] / (double)P.cap) : cand_z[i];
+      best_z[rank] = P.cap > 0.f ? (double)P.cap * tanh(z / (double)P.cap) : z;
       best_id[rank] = id;
     }
   }

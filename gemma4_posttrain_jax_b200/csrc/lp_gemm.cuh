@@ -34,7 +34,9 @@
 //                 one partial of each per row per unit and column half.
 //   EPI_DIST    : softcap + running (max m, S = sum 2^(z-m), A = sum 2^(z-m) (z-m)) per row in
 //                 base 2, from which the log-normaliser and the entropy follow.
-//   EPI_DIST_LOGITS : EPI_DIST, with the softcapped logits stored as f32.
+//   EPI_DIST_LOGITS : EPI_DIST, with the accumulator stored as f32.
+//   EPI_DIST_TOP : EPI_DIST, with the two largest of every 32 accumulator columns (8 bytes, the
+//                 first's column in its low bits).
 //   EPI_DIST_DZ : recompute path of log-probabilities and entropy; every column of
 //                 dZ = -p * (a + b * log2 p) * softcap' (two row constants), written as bf16 as
 //                 EPI_BWD_DZ does.
@@ -93,13 +95,14 @@ enum : int {
   EPI_HEAD = 3,
   EPI_DIST = 4,
   EPI_DIST_LOGITS = 5,
-  EPI_DIST_DZ = 6
+  EPI_DIST_DZ = 6,
+  EPI_DIST_TOP = 7
 };
 
 // Epilogues that only read the accumulator: no store staging, the deepest operand ring.
 template <int EPI>
 __host__ __device__ constexpr bool epi_stages_output() {
-  return EPI != EPI_FWD_LSE && EPI != EPI_DIST;
+  return EPI != EPI_FWD_LSE && EPI != EPI_DIST && EPI != EPI_DIST_TOP;
 }
 
 enum : int { STORE_BF16 = 0, STORE_F32 = 1, STORE_F32_ADD = 2 };
@@ -158,6 +161,7 @@ struct EpiParams {
   float2* best;          // HEAD: [n_groups][M] (largest logit, its column as int bits)
   int store_logits;      // HEAD: store the logits through tmO (else only the row statistics)
   float* part_a;         // DIST: [n_groups][M] running A (part holds the running max and S)
+  float2* top;           // DIST_TOP: [M][8 * tiles_n] two largest columns of each 32
   const float* row_const;  // DIST_DZ: [3][row_ld] per row: a, b, log2 of the normaliser
   long long row_ld;        // DIST_DZ: row stride of row_const
   const float* g;        // DZ : [M] upstream d logp
@@ -298,6 +302,7 @@ static_assert(gemm_smem_bytes<1, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<1, 
                   gemm_smem_bytes<1, EPI_STORE>() <= 232448 && gemm_smem_bytes<1, EPI_HEAD>() <= 232448 &&
                   gemm_smem_bytes<2, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<2, EPI_BWD_DZ>() <= 232448 &&
                   gemm_smem_bytes<2, EPI_STORE>() <= 232448 && gemm_smem_bytes<2, EPI_HEAD>() <= 232448 &&
+                  gemm_smem_bytes<1, EPI_DIST_TOP>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_TOP>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST>() <= 232448 && gemm_smem_bytes<2, EPI_DIST>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST_LOGITS>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_LOGITS>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST_DZ>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_DZ>() <= 232448,
@@ -317,6 +322,14 @@ __device__ __forceinline__ uint32_t staging_offset(int r, int c) {
   if constexpr (RB == 128) return sw128_offset(r, c);
   else return sw64_offset(r, c);
 }
+
+// The tensor core's f32 accumulation drops the bits below its last one, so a sum of d products in
+// steps of 16 comes out too small in magnitude: by d * 2^-30 of itself, on average. Measured, mean
+// relative deficit over d * 2^-30 for d from 64 to 8192: 0.8 to 1.1 for normal operands, 1.1 to 1.2
+// at the largest logits of peaked rows, 1.2 to 4.4 where all products have one sign. The
+// distribution operators scale it back: at d = 2048 the entropy of a peaked row would be off by
+// 2.6e-6 of itself, ten times what the f32 rounding of the rest leaves.
+__device__ __forceinline__ float dist_scale(int d) { return fmaf((float)d, 9.313225746154785e-10f, 1.f); }
 
 // Moves the running (m, S, A) of a row to the maximum of m and `mx` (base 2). Nothing has been
 // summed while m is -inf, so the old sums count only from a finite m on.
@@ -640,7 +653,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uint32_t tc = 0;
     const EpiParams& E = P.e;
     const float cap = E.softcap;
-    const float k1 = HAS_CAP ? 2.0f * kLog2e / cap : 0.f;  // x -> 2x/c in base 2
+    // x of the distribution epilogues, with the accumulator's truncation made up for (dist_scale)
+    constexpr bool kDist = EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || EPI == EPI_DIST_TOP || EPI == EPI_DIST_DZ;
+    const float xs = kDist ? dist_scale(S.K) : 1.f;
+    const float xlog2e = kDist ? xs * kLog2e : kLog2e;
+    const float k1 = HAS_CAP ? 2.0f * xlog2e / cap : 0.f;  // x -> 2x/c in base 2
     const float c2 = HAS_CAP ? cap * kLog2e : 0.f;        // c in base 2
     bool ok = true;
     const bool dbg_warp = P.dbg != nullptr && warp == 2 && lane == 0;
@@ -875,20 +892,40 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               sb ^= 1;
             }
           }
-        } else if constexpr (EPI == EPI_DIST) {
+        } else if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_TOP) {
+          float2 left = make_float2(-INFINITY, -INFINITY);  // TOP: of the group before this one
 #pragma unroll 1
-          for (int c = 0; c < BN / 64; ++c) {
+          for (int c = 0; c < (row_base < S.M ? BN / 64 : 0); ++c) {
             uint32_t r[32];
             __syncwarp();
             tmem_ld32(taddr + c * 32, r);
             tmem_wait_ld(r);
             const int nvalid = S.N - (colh + c * 32);  // columns >= nvalid are vocabulary padding (warp-uniform)
+            if constexpr (EPI == EPI_DIST_TOP) {
+              // the order is that of x (softcap is monotone); the column within the group takes
+              // the low 5 bits, which costs 2^-18 of x in the nomination and nothing in the result
+              float b0 = -INFINITY, b1 = -INFINITY;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float x = __uint_as_float((r[j] & ~31u) | (uint32_t)j);
+                if (j < nvalid) {
+                  b1 = fmaxf(b1, fminf(b0, x));
+                  b0 = fmaxf(b0, x);
+                }
+              }
+              if (c & 1) {
+                if (row_ok)
+                  reinterpret_cast<float4*>(E.top + (size_t)row * (8 * S.tiles_n) + nt * 8 + h * 4)[c >> 1] =
+                      make_float4(left.x, left.y, b0, b1);
+              }
+              left = make_float2(b0, b1);
+            }
             if (nvalid <= 0) continue;
             float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               const float x = __uint_as_float(r[j]);
-              const float z = HAS_CAP ? fmaf(-2.f * c2, fast_rcp(1.f + fast_ex2(x * k1)), c2) : x * kLog2e;
+              const float z = HAS_CAP ? fmaf(-2.f * c2, fast_rcp(1.f + fast_ex2(x * k1)), c2) : x * xlog2e;
               r[j] = __float_as_uint(z);
               if (j < nvalid) {
                 if (j & 1) mx1 = fmaxf(mx1, z); else mx0 = fmaxf(mx0, z);
@@ -923,9 +960,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             run_a += a0 + a1;
           }
         } else if constexpr (EPI == EPI_DIST_LOGITS) {
-          // the same over 16-column pieces, each also stored as natural-unit f32 logits
+          // the same over 16-column pieces, each also stored as it is
 #pragma unroll 1
-          for (int pc = 0; pc < BN / 32; ++pc) {
+          for (int pc = 0; pc < (row_base < S.M ? BN / 32 : 0); ++pc) {
             uint32_t r[16];
             __syncwarp();
             tmem_ld16(taddr + pc * 16, r);
@@ -933,20 +970,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const int col0 = colh + pc * 16;
             const int nvalid = S.N - col0;
             if (nvalid <= 0) continue;
+            float z[16];
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float x = __uint_as_float(r[j]);
-              const float z = HAS_CAP ? fmaf(-2.f * cap, fast_rcp(1.f + fast_ex2(x * k1)), cap) : x;
-              r[j] = __float_as_uint(z);
-              if (j < nvalid) mx = fmaxf(mx, z);
+              z[j] = HAS_CAP ? fmaf(-2.f * c2, fast_rcp(1.f + fast_ex2(x * k1)), c2) : x * xlog2e;
+              if (j < nvalid) mx = fmaxf(mx, z[j]);
             }
-            dist_rescale(run_m, run_s, run_a, mx * kLog2e);
+            dist_rescale(run_m, run_s, run_a, mx);
             float s0 = 0.f, a0 = 0.f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               if (j < nvalid) {
-                const float d0 = fmaf(__uint_as_float(r[j]), kLog2e, -run_m);
+                const float d0 = z[j] - run_m;
                 const float e0 = fast_ex2(d0);
                 s0 += e0;
                 a0 = fmaf(e0, d0, a0);
@@ -971,7 +1008,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
         } else if constexpr (EPI == EPI_DIST_DZ) {
 #pragma unroll 1
-          for (int pc = 0; pc < BN / 64; ++pc) {
+          for (int pc = 0; pc < (row_base < S.M ? BN / 64 : 0); ++pc) {
             uint32_t r[32];
             __syncwarp();
             tmem_ld32(taddr + pc * 32, r);
@@ -991,7 +1028,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                   const float lp = fmaf(-2.f * c2, rr, c2 - l2);
                   v[i] = (-4.f * rr) * (1.f - rr) * (fast_ex2(lp) * fmaf(row_b, lp, row_a));
                 } else {
-                  const float lp = fmaf(x, kLog2e, -l2);
+                  const float lp = fmaf(x, xlog2e, -l2);
                   v[i] = -fast_ex2(lp) * fmaf(row_b, lp, row_a);
                 }
               }
@@ -1146,7 +1183,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // one (max, sum) partial per unit and column half
         if (row_ok) E.part[(size_t)(un.group * 2 + h) * S.M + row] = make_float2(run_m, run_s);
       }
-      if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_LOGITS) {
+      if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || EPI == EPI_DIST_TOP) {
         if (row_ok) {
           const size_t at = (size_t)(un.group * 2 + h) * S.M + row;
           E.part[at] = make_float2(run_m, run_s);

@@ -320,7 +320,7 @@ def top(
         h, ldh = _dense_rows(hidden)
         w = _dense_embed(embed)
         with torch.cuda.device(dev):
-            ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(T, V), dev)
+            ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(T, V, int(k)), dev)
             rc = lib.lp_top(
                 _stream(dev), _ptr(h), T, h.shape[1], ldh, _ptr(w), V, float(softcap or 0.0), int(k), _ptr(tokens),
                 _ptr(ids), _ptr(logps), _ptr(entropy), _ptr(token_logps), wsp, wsn,
@@ -349,7 +349,7 @@ def sample_top_k(
         h, ldh = _dense_rows(hidden)
         w = _dense_embed(embed)
         with torch.cuda.device(dev):
-            ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(B, V), dev)
+            ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(B, V, int(top_k)), dev)
             rc = lib.lp_sample_top_k(
                 _stream(dev), _ptr(h), B, h.shape[1], ldh, _ptr(w), V, float(softcap or 0.0), int(top_k), _ptr(uniform),
                 float(temperature), float(top_p), _ptr(token), _ptr(logp), wsp, wsn,

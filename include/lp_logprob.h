@@ -319,8 +319,8 @@ LP_API int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_
                        int64_t ld_dh, void* dW, int flags, int64_t token_chunk, void* workspace,
                        size_t workspace_bytes);
 
-/* Scratch bytes lp_top and lp_sample_top_k need for T rows against V vocabulary rows. */
-LP_API size_t lp_top_workspace_bytes(int64_t T, int64_t V);
+/* Scratch bytes lp_top and lp_sample_top_k need for k tokens of T rows against V vocabulary rows. */
+LP_API size_t lp_top_workspace_bytes(int64_t T, int64_t V, int k);
 
 /*
  * The k most likely tokens of each row, 1 <= k <= min(LP_TOP_MAX, V), over the whole vocabulary.
