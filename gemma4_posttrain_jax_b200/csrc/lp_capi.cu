@@ -1212,10 +1212,15 @@ int lp_peer_barrier(void* stream, const unsigned long long* signal_pads, int ran
 // ============================================================================= distribution operators
 namespace {
 
-// A pair's 256-row tile is half empty for at most 128 rows: those run as single CTAs.
+// CTA group of a launch over T rows. An odd number of 128-row tiles leaves half of the last pair's
+// tile empty, and up to 15 tiles that costs more than pairs gain. Measured against the 262144 x 2048
+// head, single CTAs / pairs: 128 rows 179 / 215 us, 256 rows 250 / 224, 301 rows 381 / 403, 512 rows
+// 462 / 434, 1100 rows 1013 / 1110, 2048 rows 1766 / 1733.
 int cta_group_dist(int64_t T) {
   const int f = forced_cta_group();
-  return f ? f : (T <= 128 ? 1 : cta_group_for(CG_FWD));
+  if (f) return f;
+  const int64_t tiles = cdiv(T, 128);
+  return tiles % 2 == 1 && tiles <= 15 ? 1 : cta_group_for(CG_FWD);
 }
 
 struct DistFwdLayout {
@@ -1237,6 +1242,24 @@ DistFwdLayout dist_fwd_layout(int64_t T, int64_t Vs, int64_t d, const DeviceInfo
   return L;
 }
 
+// Rows of the hidden operand's box: of a single M tile only the rows there are (in eights, the
+// swizzle's period). Loading 128 with all but a few out of bounds took 224 us for one row of the
+// 262144 x 2048 head.
+uint32_t a_box_rows(const DistFwdLayout& L, int64_t T) {
+  return L.cg == 1 && T < 128 ? (uint32_t)align_up((size_t)T, 8) : 128u;
+}
+uint32_t a_box_bytes(const DistFwdLayout& L, int64_t T) {
+  const uint32_t rows = a_box_rows(L, T);
+  return rows < 128 ? rows * BK * 2 : 0;
+}
+
+// A head that a single M tile streams once leaves the L2 to what is read again: the partials, the
+// keys and the next kernel's code.
+void dist_hints(GemmParams& p) {
+  set_hints(p, G_FWD);
+  if (p.s.tiles_m == 1 && p.e.b_l2 == L2_NORMAL) p.e.b_l2 = L2_EVICT_FIRST;
+}
+
 int check_dist(const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs, const int32_t* y,
                int64_t K) {
   if (K < 0 || K > LP_DIST_MAX_TOKENS) return fail(LP_EINVAL, "K=%lld tokens per row, at most %d", (long long)K,
@@ -1246,13 +1269,12 @@ int check_dist(const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, 
   return check_common(H, T, d, ldh, W, Vs, K > 0 ? y : &none);
 }
 
-// Selection keys of a row. From kTopGroupRatio groups of 32 columns per selected token on, two
-// values per group: an eighth of the bytes of the f32 logits to write and to search, and few groups
-// that hold two of the most likely tokens, whose 32 columns have to be scored again. Fewer groups
-// and the logits themselves are the keys.
-constexpr int kTopGroupRatio = 8;
+// Selection keys of a row: two values per group of 32 or 8 columns, or the f32 logits. Larger groups
+// are fewer bytes to write and to search, but two of the n = k + kTopSpare selected tokens fall into
+// one group n^2 / (2 V / group) times, and then its other columns are scored again. A group size is
+// taken where that adds at most half as many scores again: V >= 992 n for 32, 56 n for 8.
 struct TopKeys {
-  bool groups;
+  int group;   // columns per key
   int64_t ld;  // keys per row in memory
   int n;       // keys per row
   size_t row_bytes;
@@ -1260,10 +1282,11 @@ struct TopKeys {
 };
 TopKeys top_keys(int64_t T, int64_t V, int k) {
   TopKeys K;
-  K.groups = cdiv(V, kTopGroup) >= (int64_t)kTopGroupRatio * k;
-  K.n = (int)(K.groups ? cdiv(V, kTopGroup) : V);
-  K.ld = K.groups ? cdiv(V, BN) * (BN / kTopGroup) : (V + 3) / 4 * 4;
-  K.row_bytes = (size_t)K.ld * (K.groups ? sizeof(float2) : sizeof(float));
+  const int64_t n = k + kTopSpare;
+  K.group = V >= 992 * n ? 32 : (V >= 56 * n ? 8 : 1);
+  K.n = (int)cdiv(V, K.group);
+  K.ld = K.group > 1 ? cdiv(V, BN) * (BN / K.group) : (V + 3) / 4 * 4;
+  K.row_bytes = (size_t)K.ld * (K.group > 1 ? sizeof(float2) : sizeof(float));
   K.rows = std::max<int64_t>(1, std::min<int64_t>(T, (int64_t)(((size_t)1 << 30) / K.row_bytes)));
   return K;
 }
@@ -1275,12 +1298,12 @@ size_t top_workspace(int64_t T, int64_t V, int k, const DeviceInfo* di, int sms)
   return need;
 }
 
-template <bool SAMPLE, bool GROUPS>
+template <bool SAMPLE, int G>
 int launch_top_select(cudaStream_t st, TopParams& P, int64_t rows) {
   const size_t key_bytes = (size_t)P.n_keys * sizeof(uint32_t);
   P.keys_in_smem = key_bytes <= (size_t)kTopKeyBytes;
   const size_t smem = std::max<size_t>(P.keys_in_smem ? key_bytes : 0, kTopCandBytes);
-  auto kern = top_select_kernel<SAMPLE, GROUPS>;
+  auto kern = top_select_kernel<SAMPLE, G>;
   static bool configured[kMaxDevices] = {};
   int dev = 0;
   LP_CUDA_TRY(cudaGetDevice(&dev));
@@ -1292,6 +1315,12 @@ int launch_top_select(cudaStream_t st, TopParams& P, int64_t rows) {
   kern<<<(unsigned)rows, kTopThreads, smem, st>>>(P);
   LP_LAUNCH_CHECK("top_select_kernel");
   return LP_OK;
+}
+
+template <bool SAMPLE>
+int launch_top_select(int group, cudaStream_t st, TopParams& P, int64_t rows) {
+  return group == 32 ? launch_top_select<SAMPLE, 32>(st, P, rows)
+                     : (group == 8 ? launch_top_select<SAMPLE, 8>(st, P, rows) : launch_top_select<SAMPLE, 1>(st, P, rows));
 }
 
 // The selection of lp_top and lp_sample_top_k over all rows; `all` holds the outputs and options.
@@ -1312,19 +1341,21 @@ int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
     const DistFwdLayout L = dist_fwd_layout(n, V, d, di, di->sms, K.row_bytes);
     const __nv_bfloat16* Hc = reinterpret_cast<const __nv_bfloat16*>(H) + t0 * ldh;
     alignas(64) CUtensorMap ta, tb, to;
-    if ((rc = map_bf16(&ta, Hc, d, n, ldh, BK, 128, "hidden"))) return rc;
+    if ((rc = map_bf16(&ta, Hc, d, n, ldh, BK, a_box_rows(L, n), "hidden"))) return rc;
     if ((rc = map_bf16(&tb, W, d, V, d, BK, b_box_rows(L.cg), "embedding"))) return rc;
     LP_CUDA_TRY(cudaMemsetAsync(ws, 0, sizeof(unsigned), st));
     GemmParams p{};
     p.s = L.s;
+    p.a_box_bytes = a_box_bytes(L, n);
     p.sched = reinterpret_cast<unsigned*>(ws);
     p.e.softcap = softcap;
     p.e.part = reinterpret_cast<float2*>(ws + L.part_off);
     p.e.part_a = reinterpret_cast<float*>(ws + L.part_a_off);
-    set_hints(p, G_FWD);
-    if (K.groups) {
+    dist_hints(p);
+    if (K.group > 1) {
       p.e.top = reinterpret_cast<float2*>(ws + L.keys_off);
-      rc = launch_gemm_cap<EPI_DIST_TOP, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "top_gemm");
+      rc = K.group == 32 ? launch_gemm_cap<EPI_DIST_TOP32, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "top_gemm")
+                         : launch_gemm_cap<EPI_DIST_TOP8, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "top_gemm");
     } else {
       if ((rc = map_store_f32(&to, ws + L.keys_off, V, n, K.ld, "logits store"))) return rc;
       rc = launch_gemm_cap<EPI_DIST_LOGITS, false, false>(softcap > 0.f, st, ta, tb, to, p, di, "top_gemm");
@@ -1341,21 +1372,21 @@ int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
     P.d = d;
     P.V = V;
     P.cap = softcap;
-    if (K.groups) P.groups = p.e.top; else P.logits = reinterpret_cast<const float*>(ws + L.keys_off);
+    if (K.group > 1) P.groups = p.e.top; else P.logits = reinterpret_cast<const float*>(ws + L.keys_off);
     P.ld_keys = K.ld;
     P.n_keys = K.n;
     if (sample) {
       P.uniform = all.uniform + t0;
       P.sampled = all.sampled + t0;
       P.logps = all.logps + t0;
-      rc = K.groups ? launch_top_select<true, true>(st, P, n) : launch_top_select<true, false>(st, P, n);
+      rc = launch_top_select<true>(K.group, st, P, n);
     } else {
       P.tokens = all.tokens != nullptr ? all.tokens + t0 : nullptr;
       P.ids = all.ids + t0 * all.k;
       P.logps = all.logps + t0 * all.k;
       P.entropy = all.entropy + t0;
       P.token_logps = all.token_logps != nullptr ? all.token_logps + t0 : nullptr;
-      rc = K.groups ? launch_top_select<false, true>(st, P, n) : launch_top_select<false, false>(st, P, n);
+      rc = launch_top_select<false>(K.group, st, P, n);
     }
     if (rc) return rc;
   }
@@ -1397,16 +1428,17 @@ int lp_dist_fwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   char* ws = reinterpret_cast<char*>(workspace);
   alignas(64) CUtensorMap ta, tb;
-  if ((rc = map_bf16(&ta, H, d, T, ldh, BK, 128, "hidden"))) return rc;
+  if ((rc = map_bf16(&ta, H, d, T, ldh, BK, a_box_rows(L, T), "hidden"))) return rc;
   if ((rc = map_bf16(&tb, W, d, Vs, d, BK, b_box_rows(L.cg), "embedding"))) return rc;
   LP_CUDA_TRY(cudaMemsetAsync(ws, 0, sizeof(unsigned), st));
   GemmParams p{};
   p.s = L.s;
+  p.a_box_bytes = a_box_bytes(L, T);
   p.sched = reinterpret_cast<unsigned*>(ws);
   p.e.softcap = softcap;
   p.e.part = reinterpret_cast<float2*>(ws + L.part_off);
   p.e.part_a = reinterpret_cast<float*>(ws + L.part_a_off);
-  set_hints(p, G_FWD);
+  dist_hints(p);
   if ((rc = launch_gemm_cap<EPI_DIST, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "dist_fwd_gemm"))) return rc;
   ProfScope prof(st, "dist_finalize");
   const __nv_bfloat16* Hb = reinterpret_cast<const __nv_bfloat16*>(H);

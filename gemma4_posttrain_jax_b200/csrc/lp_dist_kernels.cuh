@@ -61,25 +61,55 @@ __device__ __forceinline__ float warp_dot(const __nv_bfloat16* __restrict__ h, c
   return acc;
 }
 
-// The same in f64. The products are exact and a sum of bf16 products rarely needs more than 53
-// bits, so equal dot products compare equal whatever the order of the sum.
-__device__ __forceinline__ double warp_dot_f64(const __nv_bfloat16* __restrict__ h,
-                                               const __nv_bfloat16* __restrict__ w, long long d, int lane) {
-  double acc0 = 0., acc1 = 0.;
-  for (long long i = lane; i < d / 8; i += 32) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(h) + i);
-    const uint4 b = __ldg(reinterpret_cast<const uint4*>(w) + i);
-    const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+// Sum of f32 terms held as s + e, exact but for the rounding of e (about 2^-48 of the terms): each
+// addition's rounding error is itself an f32 number, which e collects (Knuth's two-sum).
+struct TwoSum {
+  float s = 0.f, e = 0.f;
+  __device__ __forceinline__ void add(float p) {
+    const float t = s + p;
+    const float b = t - s;
+    e += (s - (t - b)) + (p - b);
+    s = t;
+  }
+  __device__ __forceinline__ void add(const TwoSum& o) {
+    add(o.s);
+    e += o.e;
+  }
+};
+
+// h . w over one warp (complete in lane 0), to about 2^-48 of sum |h w|: products of two bf16 numbers
+// are exact in f32. f64 would convert every product, which took three times as long.
+__device__ __forceinline__ double warp_dot_exact(const __nv_bfloat16* __restrict__ h,
+                                                 const __nv_bfloat16* __restrict__ w, long long d, int lane) {
+  TwoSum a, b;
+  const int n = (int)(d / 8);
+  for (int i0 = lane; i0 - lane < n; i0 += 256) {
+    // up to 2048 columns of w in flight; h is in L1
+    uint4 w4[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      acc0 += (double)(__uint_as_float(av[j] << 16) * __uint_as_float(bv[j] << 16));
-      acc1 += (double)(__uint_as_float(av[j] & 0xffff0000u) * __uint_as_float(bv[j] & 0xffff0000u));
+    for (int u = 0; u < 8; ++u)
+      w4[u] = i0 + 32 * u < n ? __ldg(reinterpret_cast<const uint4*>(w) + i0 + 32 * u) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (i0 - lane + 32 * u >= n) break;  // warp-uniform
+      const uint4 h4 = i0 + 32 * u < n ? __ldg(reinterpret_cast<const uint4*>(h) + i0 + 32 * u) : make_uint4(0, 0, 0, 0);
+      const uint32_t hv[4] = {h4.x, h4.y, h4.z, h4.w}, wv[4] = {w4[u].x, w4[u].y, w4[u].z, w4[u].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        a.add(__fmul_rn(__uint_as_float(hv[j] << 16), __uint_as_float(wv[j] << 16)));
+        b.add(__fmul_rn(__uint_as_float(hv[j] & 0xffff0000u), __uint_as_float(wv[j] & 0xffff0000u)));
+      }
     }
   }
-  double acc = acc0 + acc1;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  return acc;
+  a.add(b);
+#pragma unroll 1
+  for (int o = 16; o > 0; o >>= 1) {
+    TwoSum x;
+    x.s = __shfl_down_sync(0xffffffffu, a.s, o);
+    x.e = __shfl_down_sync(0xffffffffu, a.e, o);
+    a.add(x);
+  }
+  return (double)a.s + (double)a.e;
 }
 
 // Merges the GEMM's partials of R consecutive rows per block and computes the given tokens'
@@ -230,22 +260,25 @@ __global__ void dist_dz_targets_kernel(const int32_t* __restrict__ y, const floa
 
 // ----------------------------------------------------------------------------- selection
 // The k most likely tokens of a row, in the order of the exact dot products h . W_v (softcap is
-// monotone), the lowest id first among equals. The GEMM only nominates: a key is either one
-// accumulator (f32) or the largest of 32 neighbours with the second largest beside it. The
-// k + kTopSpare largest keys are selected; of a selected group every column is a candidate if its
-// second largest reaches the k-th largest value seen, else only its largest is. Candidates are
-// scored again in f64 and ranked by that, so a rounding of the nomination (f32 accumulation, 2^-18
-// for a group's low bits) can exchange neighbours only if more than kTopSpare values lie within it
-// of the k-th.
+// monotone), the lowest id first among equals. The GEMM only nominates: a key is one accumulator
+// (f32) or the largest of G neighbours with the second largest beside it. The k + kTopSpare largest
+// keys are selected; of a selected group every column is a candidate if its second largest could be
+// as large as the selected keys are, else only its largest is. Candidates are scored again to 2^-48
+// and ranked by that, so a rounding of the nomination (f32 accumulation, 2^-18 for a group's low
+// bits) can exchange neighbours only if more than kTopSpare values lie within it of the k-th.
+//
+// Finding the keys: each thread keeps the largest of the keys it loads; the n-th largest of those
+// kTopThreads maxima is a lower bound of the n-th largest key, and few more than n keys reach it
+// (about n^2 / (2 kTopThreads), the keys that share a thread). Only when more than kTopSel do, a
+// bisection over all keys follows.
 constexpr int kTopMax = 128;
-constexpr int kTopSpare = 16;
-constexpr int kTopGroup = 32;
+constexpr int kTopSpare = 8;
 constexpr int kTopThreads = 512;
-// selected keys: at most k + 2 kTopSpare, or any number up to this of equal ones
-constexpr int kTopSel = kTopMax + 2 * kTopSpare;
-constexpr int kTopCand = kTopSel * kTopGroup;
-constexpr int kTopCandBytes = kTopCand * (int)(sizeof(double) + sizeof(int));
-constexpr int kTopKeyBytes = 200 * 1024 - 16 * 1024;  // keys kept in shared memory, beside the static part
+constexpr int kTopSel = kTopMax + 8 * kTopSpare;  // most selected keys
+constexpr int kTopBatch = 384;                    // candidates scored and ranked at a time,
+constexpr int kTopCand = kTopBatch + kTopMax;     // beside the best of those before them
+constexpr int kTopCandBytes = kTopCand * (int)(sizeof(long long) + sizeof(int));
+constexpr int kTopKeyBytes = 184 * 1024;  // most key bytes kept in shared memory, beside the static part
 
 // Order-preserving map of f32 to u32; NaN comes last.
 __device__ __forceinline__ uint32_t ordered_key(float x) {
@@ -254,7 +287,10 @@ __device__ __forceinline__ uint32_t ordered_key(float x) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 // A group's value without its column bits.
-__device__ __forceinline__ float group_value(float x) { return __uint_as_float(__float_as_uint(x) & ~31u); }
+template <int G>
+__device__ __forceinline__ float group_value(float x) {
+  return __uint_as_float(__float_as_uint(x) & ~(uint32_t)(G - 1));
+}
 
 struct TopParams {
   const float2* part;
@@ -267,7 +303,7 @@ struct TopParams {
   long long d, V;
   float cap;
   const float* logits;  // [T, ld_keys] accumulators, or
-  const float2* groups;  // [T, ld_keys] the two largest of every 32
+  const float2* groups;  // [T, ld_keys] the two largest of every G columns
   long long ld_keys;
   int n_keys;
   int keys_in_smem;
@@ -293,167 +329,328 @@ __device__ __forceinline__ int block_sum(int v, int* warp_s) {
   return sum;
 }
 
-template <bool SAMPLE, bool GROUPS>
-__global__ void __launch_bounds__(kTopThreads) top_select_kernel(const TopParams P) {
-  // keys while selecting, then the candidates' f64 scores and ids
+// f64 to i64 with the same order (a NaN first, as a -inf).
+__device__ __forceinline__ long long ordered_i64(double z) {
+  if (z != z) z = -INFINITY;
+  const long long b = __double_as_longlong(z == 0. ? 0. : z);
+  return b < 0 ? b ^ 0x7fffffffffffffffll : b;
+}
+__device__ __forceinline__ double ordered_f64(long long b) {
+  return __longlong_as_double(b < 0 ? b ^ 0x7fffffffffffffffll : b);
+}
+
+// G: columns per key (1: the keys are the accumulators).
+template <bool SAMPLE, int G>
+__global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopParams P) {
+  constexpr bool GROUPS = G > 1;
+  // keys while selecting, then the candidates' scores and ids
   extern __shared__ __align__(16) uint8_t dyn_s[];
   uint32_t* keys_s = reinterpret_cast<uint32_t*>(dyn_s);
-  double* cand_z = reinterpret_cast<double*>(dyn_s);
-  int* cand_id = reinterpret_cast<int*>(dyn_s + kTopCand * sizeof(double));
-  __shared__ DistAcc acc_s[kTopThreads / 32];
-  __shared__ int warp_s[kTopThreads / 32];
+  long long* cand_z = reinterpret_cast<long long*>(dyn_s);
+  int* cand_id = reinterpret_cast<int*>(dyn_s + kTopCand * sizeof(long long));
+  constexpr int kWarps = kTopThreads / 32;
+  __shared__ __align__(16) uint32_t max_s[kTopThreads];
+  __shared__ float red_s[3][kWarps];
+  __shared__ int warp_s[kWarps];
   __shared__ int n_sel_s, n_cand_s;
+  __shared__ uint32_t lo_s;
   __shared__ int sel_key[kTopSel];
-  __shared__ float sel_v[2 * kTopSel];  // values of the selected keys: [0, n) largest, [n, 2n) second
-  __shared__ float kth_s;
+  __shared__ int sel_at[kTopSel];  // a selected key's first candidate
+  __shared__ long long best_i[kTopMax];
   __shared__ double best_z[kTopMax];
   __shared__ int best_id[kTopMax];
   const int t = blockIdx.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n_keys = P.n_keys;
   const __nv_bfloat16* h = P.H + (size_t)t * P.ldh;
+  const float2* groups = GROUPS ? P.groups + (size_t)t * P.ld_keys : nullptr;
+  const float* logits = GROUPS ? nullptr : P.logits + (size_t)t * P.ld_keys;
 
   auto load_key = [&](int i) -> uint32_t {
-    if constexpr (GROUPS) return ordered_key(group_value(P.groups[(size_t)t * P.ld_keys + i].x));
-    else return ordered_key(P.logits[(size_t)t * P.ld_keys + i]);
+    if constexpr (GROUPS) return ordered_key(group_value<G>(groups[i].x));
+    else return ordered_key(logits[i]);
   };
   auto key = [&](int i) -> uint32_t { return P.keys_in_smem ? keys_s[i] : load_key(i); };
 
+  // ---- loads: the row's partials (up to four per thread at once), hidden state and keys
+  constexpr int PN = 4;
+  float2 pv[PN];
+  float pa[PN];
+#pragma unroll
+  for (int j = 0; j < PN; ++j) {
+    const int g = tid + j * kTopThreads;
+    pv[j] = g < P.n_parts ? P.part[(size_t)g * P.T + t] : make_float2(-INFINITY, 0.f);
+    pa[j] = g < P.n_parts ? P.part_a[(size_t)g * P.T + t] : 0.f;
+  }
   // a row of zeros: every logit is exactly 0
   int nonzero = 0;
   for (long long i = tid; i < P.d / 8; i += kTopThreads) {
     const uint4 a = __ldg(reinterpret_cast<const uint4*>(h) + i);
     nonzero |= ((a.x | a.y | a.z | a.w) & 0x7fff7fffu) != 0u;
   }
-  if (P.keys_in_smem)
-    for (int i = tid; i < n_keys; i += kTopThreads) keys_s[i] = load_key(i);
-  // row statistics
-  DistAcc acc{-INFINITY, 0.f, 0.f};
-  for (int g = tid; g < P.n_parts; g += kTopThreads) {
-    const float2 p = P.part[(size_t)g * P.T + t];
-    acc = dist_merge(acc, DistAcc{p.x, p.y, P.part_a[(size_t)g * P.T + t]});
+  uint32_t best_key = 0u;
+  {
+    // 16 bytes per load: two groups, or four logits (rows are padded to that)
+    constexpr int KV = GROUPS ? 2 : 4;
+    const float4* src = GROUPS ? reinterpret_cast<const float4*>(groups) : reinterpret_cast<const float4*>(logits);
+    const int n_vec = (n_keys + KV - 1) / KV;
+#pragma unroll 8
+    for (int i = tid; i < n_vec; i += kTopThreads) {
+      const float4 x = __ldg(src + i);
+      uint32_t k[KV];
+      if constexpr (GROUPS) {
+        k[0] = ordered_key(group_value<G>(x.x));
+        k[1] = ordered_key(group_value<G>(x.z));
+      } else {
+        k[0] = ordered_key(x.x);
+        k[1] = ordered_key(x.y);
+        k[2] = ordered_key(x.z);
+        k[3] = ordered_key(x.w);
+      }
+#pragma unroll
+      for (int j = 0; j < KV; ++j) {
+        const int at = i * KV + j;
+        if (at < n_keys) {
+          best_key = max(best_key, k[j]);
+          if (P.keys_in_smem) keys_s[at] = k[j];
+        }
+      }
+    }
   }
+  max_s[tid] = best_key;
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < PN; ++j) m = fmaxf(m, pv[j].x);
+  for (int g = tid + PN * kTopThreads; g < P.n_parts; g += kTopThreads) m = fmaxf(m, P.part[(size_t)g * P.T + t].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) red_s[0][warp] = m;
+  if (tid == 0) n_sel_s = 0;
+  nonzero = __syncthreads_or(nonzero);
+
+  // ---- row statistics: the partials at the row's maximum, summed in a fixed order
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red_s[0][w]);
+  float s = 0.f, a = 0.f;
+  auto add_part = [&](float2 p, float av) {
+    if (p.y != 0.f) {
+      const float dm = p.x - m, e = exp2f(dm);
+      s = fmaf(p.y, e, s);
+      a = fmaf(fmaf(p.y, dm, av), e, a);
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < PN; ++j) add_part(pv[j], pa[j]);
+  for (int g = tid + PN * kTopThreads; g < P.n_parts; g += kTopThreads)
+    add_part(P.part[(size_t)g * P.T + t], P.part_a[(size_t)g * P.T + t]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    DistAcc b;
-    b.m = __shfl_xor_sync(0xffffffffu, acc.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, acc.s, o);
-    b.a = __shfl_xor_sync(0xffffffffu, acc.a, o);
-    acc = (lane & o) ? dist_merge(b, acc) : dist_merge(acc, b);
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    a += __shfl_xor_sync(0xffffffffu, a, o);
   }
-  if (lane == 0) acc_s[warp] = acc;
-  if (tid == 0) n_sel_s = n_cand_s = 0;
-  nonzero = __syncthreads_or(nonzero);
-  acc = acc_s[0];
-#pragma unroll
-  for (int w = 1; w < kTopThreads / 32; ++w) acc = dist_merge(acc, acc_s[w]);
-  const float lse = dist_lse(acc);
+  if (lane == 0) {
+    red_s[1][warp] = s;
+    red_s[2][warp] = a;
+  }
 
+  uint32_t lo = 0u;
   if (nonzero) {
-    // Bisection on the ordered keys: count(key >= lo) >= n always holds, count(key >= hi) < n.
     const int n = min(n_keys, P.k + kTopSpare);
-    uint32_t lo = 0u;
-    unsigned long long hi = 1ull << 32;
-    int c_lo = n_keys;
-    while (c_lo > n + kTopSpare && hi - lo > 1) {
-      const uint32_t mid = (uint32_t)(lo + (hi - lo) / 2);
-      int c = 0;
-      for (int i = tid; i < n_keys; i += kTopThreads) c += key(i) >= mid ? 1 : 0;
-      c = block_sum(c, warp_s);
-      if (c >= n) {
-        lo = mid;
-        c_lo = c;
-      } else {
-        hi = mid;
+    // ---- a threshold that at least n keys reach, by bisection on the threads' maxima
+    if (n < n_keys && warp == 0) {
+      uint32_t v[kTopThreads / 32];
+      uint32_t low = 0xffffffffu, top = 0u;
+#pragma unroll
+      for (int j = 0; j < kTopThreads / 128; ++j) {
+        const uint4 x = reinterpret_cast<const uint4*>(max_s)[j * 32 + lane];
+        v[4 * j] = x.x;
+        v[4 * j + 1] = x.y;
+        v[4 * j + 2] = x.z;
+        v[4 * j + 3] = x.w;
       }
-    }
-    const bool ties = c_lo > kTopSel;  // then hi = lo + 1: more equal keys than slots
-    for (int i = tid; i < n_keys; i += kTopThreads) {
-      const uint32_t x = key(i);
-      if (ties ? x > lo : x >= lo) sel_key[atomicAdd(&n_sel_s, 1)] = i;
+#pragma unroll
+      for (int j = 0; j < kTopThreads / 32; ++j) {
+        low = min(low, v[j]);
+        top = max(top, v[j]);
+      }
+      uint32_t at = __reduce_min_sync(0xffffffffu, low);
+      unsigned long long hi = (unsigned long long)__reduce_max_sync(0xffffffffu, top) + 1;
+      int c_at = kTopThreads;
+      while (c_at > n + kTopSpare / 2 && hi - at > 1) {
+        const uint32_t mid = (uint32_t)(at + (hi - at) / 2);
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < kTopThreads / 32; ++j) c += v[j] >= mid ? 1 : 0;
+        c = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
+        if (c >= n) {
+          at = mid;
+          c_at = c;
+        } else {
+          hi = mid;
+        }
+      }
+      if (lane == 0) lo_s = at;
+    } else if (n >= n_keys && tid == 0) {
+      lo_s = 0u;
     }
     __syncthreads();
-    if (ties) {
-      // fewer than n keys lie above the tie; fill up to n with the lowest of the tie
-      int have = n_sel_s;
-      __syncthreads();
-      for (int base = 0; base < n_keys && have < n; base += kTopThreads) {
-        const int i = base + tid;
-        const bool hit = i < n_keys && key(i) == lo;
-        const unsigned ballot = __ballot_sync(0xffffffffu, hit);
-        if (lane == 0) warp_s[warp] = __popc(ballot);
-        __syncthreads();
-        int before = 0, total = 0;
-        for (int w = 0; w < kTopThreads / 32; ++w) {
-          before += w < warp ? warp_s[w] : 0;
-          total += warp_s[w];
-        }
-        const int slot = have + before + __popc(ballot & ((1u << lane) - 1u));
-        if (hit && slot < n) sel_key[slot] = i;
-        have = min(n, have + total);
-        __syncthreads();
+    lo = lo_s;
+    for (int i = tid; i < n_keys; i += kTopThreads) {
+      if (key(i) >= lo) {
+        const int at = atomicAdd(&n_sel_s, 1);
+        if (at < kTopSel) sel_key[at] = i;
       }
-      if (tid == 0) n_sel_s = n;
-      __syncthreads();
     }
-    const int n_sel = n_sel_s;  // the keys in shared memory are not read below
-    if constexpr (GROUPS) {
-      float b0 = -INFINITY, b1 = -INFINITY;
-      if (tid < n_sel) {
-        const float2 g = P.groups[(size_t)t * P.ld_keys + sel_key[tid]];
-        b0 = g.x;
-        b1 = group_value(g.y);
-        sel_v[tid] = group_value(b0);
-        sel_v[n_sel + tid] = b1;
-      }
-      if (tid == 0) kth_s = -INFINITY;
-      __syncthreads();
-      // the k-th largest of the values seen is a lower bound of the k-th largest logit
-      for (int i = tid; i < 2 * n_sel; i += kTopThreads) {
-        const float v = sel_v[i];
-        int above = 0;
-        for (int j = 0; j < 2 * n_sel; ++j) above += (sel_v[j] > v || (sel_v[j] == v && j < i)) ? 1 : 0;
-        if (above == P.k - 1) kth_s = v;
-      }
-      __syncthreads();
-      if (tid < n_sel) {
-        const long long first = (long long)sel_key[tid] * kTopGroup;
-        const int cols = (int)min((long long)kTopGroup, P.V - first);
-        // 2^-16 of slack for the accumulation and the bits cut off
-        const float least = kth_s - 1.52587890625e-05f * fabsf(kth_s);
-        if (!(b1 < least)) {
-          const int at = atomicAdd(&n_cand_s, cols);
-          for (int c = 0; c < cols; ++c) cand_id[at + c] = (int)first + c;
+    __syncthreads();
+    if (n_sel_s > kTopSel) {
+      // ---- bisection over all keys: count(key >= lo) >= n always holds, count(key >= hi) < n
+      int c_lo = n_sel_s;
+      unsigned long long hi = 1ull << 32;
+      while (c_lo > kTopSel && hi - lo > 1) {
+        const uint32_t mid = (uint32_t)(lo + (hi - lo) / 2);
+        int c = 0;
+        for (int i = tid; i < n_keys; i += kTopThreads) c += key(i) >= mid ? 1 : 0;
+        c = block_sum(c, warp_s);
+        if (c >= n) {
+          lo = mid;
+          c_lo = c;
         } else {
-          cand_id[atomicAdd(&n_cand_s, 1)] = (int)first + (int)(__float_as_uint(b0) & 31u);
+          hi = mid;
         }
       }
-    } else {
-      if (tid < n_sel) cand_id[tid] = sel_key[tid];
-      if (tid == 0) n_cand_s = n_sel;
+      const bool ties = c_lo > kTopSel;  // then hi = lo + 1: more equal keys than slots
+      if (tid == 0) n_sel_s = 0;
+      __syncthreads();
+      for (int i = tid; i < n_keys; i += kTopThreads) {
+        const uint32_t x = key(i);
+        if (ties ? x > lo : x >= lo) sel_key[atomicAdd(&n_sel_s, 1)] = i;
+      }
+      __syncthreads();
+      if (ties) {
+        // fewer than n keys lie above the tie; fill up to n with the lowest of the tie
+        int have = n_sel_s;
+        __syncthreads();
+        for (int base = 0; base < n_keys && have < n; base += kTopThreads) {
+          const int i = base + tid;
+          const bool hit = i < n_keys && key(i) == lo;
+          const unsigned ballot = __ballot_sync(0xffffffffu, hit);
+          if (lane == 0) warp_s[warp] = __popc(ballot);
+          __syncthreads();
+          int before = 0, total = 0;
+          for (int w = 0; w < kWarps; ++w) {
+            before += w < warp ? warp_s[w] : 0;
+            total += warp_s[w];
+          }
+          const int slot = have + before + __popc(ballot & ((1u << lane) - 1u));
+          if (hit && slot < n) sel_key[slot] = i;
+          have = min(n, have + total);
+          __syncthreads();
+        }
+        if (tid == 0) n_sel_s = n;
+        __syncthreads();
+      }
     }
   } else {
-    if (tid < P.k) cand_id[tid] = tid;
-    if (tid == 0) n_cand_s = P.k;
+    // every logit is exactly 0: the first k tokens, or every column of the groups that hold them
+    if (tid < P.k) sel_key[tid] = tid;
+    if (tid == 0) n_sel_s = (P.k + G - 1) / G;
+    __syncthreads();
+  }
+  // ---- candidates of the selected keys: where each key's first one is
+  const int n_sel = n_sel_s;  // the keys in shared memory are not read below
+  int first = 0, cols = 0;    // this thread's key
+  if (tid < n_sel) {
+    first = sel_key[tid] * G;
+    cols = 1;
+    if constexpr (GROUPS) {
+      const float2 g = groups[sel_key[tid]];
+      // the second largest against the least selected key, with 2^-16 of slack for the
+      // accumulation and the bits cut off
+      float b1 = group_value<G>(g.y);
+      b1 = b1 + 1.52587890625e-05f * fabsf(b1);
+      if (!nonzero || ordered_key(b1) >= lo) cols = (int)min((long long)G, P.V - first);
+      else first += (int)(__float_as_uint(g.x) & (uint32_t)(G - 1));
+    }
+  }
+  if constexpr (GROUPS) {
+    // exclusive scan over the threads (keys of threads beyond n_sel have none)
+    int x = cols;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_s[warp] = x;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      before += w < warp ? warp_s[w] : 0;
+      total += warp_s[w];
+    }
+    if (tid < n_sel) sel_at[tid] = before + x - cols;
+    if (tid == 0) n_cand_s = total;
+  } else {
+    if (tid < n_sel) sel_at[tid] = tid;
+    if (tid == 0) n_cand_s = n_sel;
   }
   __syncthreads();
   const int n_cand = n_cand_s;
-
-  for (int i = warp; i < n_cand; i += kTopThreads / 32) {
-    const double z = warp_dot_f64(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);
-    if (lane == 0) cand_z[i] = z == z ? z : -INFINITY;  // a NaN ranks last
+  const int my_at = tid < n_sel ? sel_at[tid] : 0;
+  s = a = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    s += red_s[1][w];
+    a += red_s[2][w];
   }
-  __syncthreads();
-  // rank by (z descending, id ascending)
-  for (int i = tid; i < n_cand; i += kTopThreads) {
-    const double z = cand_z[i];
-    const int id = cand_id[i];
-    int rank = 0;
-    for (int j = 0; j < n_cand; ++j) rank += (cand_z[j] > z || (cand_z[j] == z && cand_id[j] < id)) ? 1 : 0;
-    if (rank < P.k) {
-      best_z[rank] = P.cap > 0.f ? (double)P.cap * tanh(z / (double)P.cap) : z;
-      best_id[rank] = id;
+  const DistAcc acc{m, s, a};
+  const float lse = dist_lse(acc);
+
+  // ---- batches of candidates; the best k so far take part in the next batch's ranking
+  for (int b0 = 0; b0 < n_cand; b0 += kTopBatch) {
+    const int have = b0 == 0 ? 0 : P.k;  // a batch before this one was full, so it had k
+    const int count = have + min(kTopBatch, n_cand - b0);
+    if (tid < have) {
+      cand_z[tid] = best_i[tid];
+      cand_id[tid] = best_id[tid];
     }
+    for (int c = max(0, b0 - my_at); c < min(cols, b0 + kTopBatch - my_at); ++c) cand_id[have + my_at + c - b0] = first + c;
+    __syncthreads();
+    // The candidates' rows of W come from all over it: ask for all of them at once, so that their
+    // latencies (HBM and address translation) pass together and not once per round of the warps.
+    const int lines = (int)((P.d * 2 + 127) / 128);
+    for (int i = tid; i < (count - have) * lines; i += kTopThreads)
+      prefetch_l2(reinterpret_cast<const char*>(P.W + (size_t)cand_id[have + i / lines] * P.d) + (size_t)(i % lines) * 128);
+#pragma unroll 1
+    for (int i = have + warp; i < count; i += kWarps) {
+      const double z = warp_dot_exact(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);
+      if (lane == 0) cand_z[i] = ordered_i64(z);
+    }
+    __syncthreads();
+    // rank by (score descending, id ascending), four threads per candidate
+    for (int i0 = 0; i0 < count; i0 += kTopThreads / 4) {
+      const int i = i0 + tid / 4;
+      const long long z = i < count ? cand_z[i] : 0;
+      const int id = i < count ? cand_id[i] : 0;
+      int rank = 0;
+#pragma unroll 4
+      for (int j = tid % 4; j < count; j += 4) {
+        const long long o = cand_z[j];
+        rank += (o > z || (o == z && cand_id[j] < id)) ? 1 : 0;
+      }
+      rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+      rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+      if (tid % 4 == 0 && i < count && rank < P.k) {
+        best_i[rank] = z;
+        best_id[rank] = id;
+      }
+    }
+    __syncthreads();
+  }
+  if (tid < P.k) {
+    const double x = ordered_f64(best_i[tid]);
+    if constexpr (SAMPLE) best_z[tid] = P.cap > 0.f ? (double)P.cap * tanh(x / (double)P.cap) : x;
+    else best_z[tid] = (double)softcap_exact((float)x, P.cap);
   }
   __syncthreads();
 
@@ -469,7 +666,11 @@ __global__ void __launch_bounds__(kTopThreads) top_select_kernel(const TopParams
       if (v >= 0 && v < P.V) lp = dist_logp(softcap_exact(warp_dot(h, P.W + (size_t)v * P.d, P.d, lane), P.cap), lse);
       if (lane == 0) P.token_logps[t] = lp;
     }
-  } else if (warp == 0) {
+  } else {
+    __shared__ double weight_s[kTopMax];
+    if (tid < P.k) weight_s[tid] = exp((best_z[tid] - best_z[0]) / (double)P.temperature);
+    __syncthreads();
+    if (warp != 0) return;
     // Inverse of the cumulative distribution of the kept prefix, in f64: kTopMax / 32 consecutive
     // ranks per lane and a scan over the lanes.
     constexpr int Q = kTopMax / 32;
@@ -478,7 +679,7 @@ __global__ void __launch_bounds__(kTopThreads) top_select_kernel(const TopParams
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int j = lane * Q + q;
-      w[q] = j < P.k ? exp((best_z[j] - best_z[0]) / (double)P.temperature) : 0.;
+      w[q] = j < P.k ? weight_s[j] : 0.;
       run += w[q];
       upto[q] = run;
     }

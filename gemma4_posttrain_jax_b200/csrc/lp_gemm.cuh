@@ -35,8 +35,8 @@
 //   EPI_DIST    : softcap + running (max m, S = sum 2^(z-m), A = sum 2^(z-m) (z-m)) per row in
 //                 base 2, from which the log-normaliser and the entropy follow.
 //   EPI_DIST_LOGITS : EPI_DIST, with the accumulator stored as f32.
-//   EPI_DIST_TOP : EPI_DIST, with the two largest of every 32 accumulator columns (8 bytes, the
-//                 first's column in its low bits).
+//   EPI_DIST_TOP32, EPI_DIST_TOP8 : EPI_DIST, with the two largest of every 32 (8) accumulator
+//                 columns (8 bytes, the first's column in its low bits).
 //   EPI_DIST_DZ : recompute path of log-probabilities and entropy; every column of
 //                 dZ = -p * (a + b * log2 p) * softcap' (two row constants), written as bf16 as
 //                 EPI_BWD_DZ does.
@@ -96,13 +96,20 @@ enum : int {
   EPI_DIST = 4,
   EPI_DIST_LOGITS = 5,
   EPI_DIST_DZ = 6,
-  EPI_DIST_TOP = 7
+  EPI_DIST_TOP32 = 7,
+  EPI_DIST_TOP8 = 8
 };
+
+// Columns per selection key of an epilogue (0: none).
+template <int EPI>
+__host__ __device__ constexpr int top_group() {
+  return EPI == EPI_DIST_TOP32 ? 32 : (EPI == EPI_DIST_TOP8 ? 8 : 0);
+}
 
 // Epilogues that only read the accumulator: no store staging, the deepest operand ring.
 template <int EPI>
 __host__ __device__ constexpr bool epi_stages_output() {
-  return EPI != EPI_FWD_LSE && EPI != EPI_DIST && EPI != EPI_DIST_TOP;
+  return EPI != EPI_FWD_LSE && EPI != EPI_DIST && top_group<EPI>() == 0;
 }
 
 enum : int { STORE_BF16 = 0, STORE_F32 = 1, STORE_F32_ADD = 2 };
@@ -161,7 +168,7 @@ struct EpiParams {
   float2* best;          // HEAD: [n_groups][M] (largest logit, its column as int bits)
   int store_logits;      // HEAD: store the logits through tmO (else only the row statistics)
   float* part_a;         // DIST: [n_groups][M] running A (part holds the running max and S)
-  float2* top;           // DIST_TOP: [M][8 * tiles_n] two largest columns of each 32
+  float2* top;           // DIST_TOP: [M][BN / group * tiles_n] two largest columns of each group
   const float* row_const;  // DIST_DZ: [3][row_ld] per row: a, b, log2 of the normaliser
   long long row_ld;        // DIST_DZ: row stride of row_const
   const float* g;        // DZ : [M] upstream d logp
@@ -199,6 +206,10 @@ struct GemmParams {
   // MN-major operands with 3-D tensor maps (64 columns, K, 64-column chunks): the CTA's
   // tile of that operand is one TMA instruction instead of one per 64-column chunk.
   int a_mn3d, b_mn3d;
+  // CG = 1, one M tile of fewer than 128 rows: bytes of the A box (its rows only; the rest of the
+  // stage keeps what it holds, which the MMA turns into accumulator rows that nothing reads).
+  // 0: all 128 rows.
+  uint32_t a_box_bytes;
 };
 
 __device__ __forceinline__ unsigned long long clk64() { return (unsigned long long)clock64(); }
@@ -302,7 +313,8 @@ static_assert(gemm_smem_bytes<1, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<1, 
                   gemm_smem_bytes<1, EPI_STORE>() <= 232448 && gemm_smem_bytes<1, EPI_HEAD>() <= 232448 &&
                   gemm_smem_bytes<2, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<2, EPI_BWD_DZ>() <= 232448 &&
                   gemm_smem_bytes<2, EPI_STORE>() <= 232448 && gemm_smem_bytes<2, EPI_HEAD>() <= 232448 &&
-                  gemm_smem_bytes<1, EPI_DIST_TOP>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_TOP>() <= 232448 &&
+                  gemm_smem_bytes<1, EPI_DIST_TOP32>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_TOP32>() <= 232448 &&
+                  gemm_smem_bytes<1, EPI_DIST_TOP8>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_TOP8>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST>() <= 232448 && gemm_smem_bytes<2, EPI_DIST>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST_LOGITS>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_LOGITS>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST_DZ>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_DZ>() <= 232448,
@@ -341,6 +353,61 @@ __device__ __forceinline__ void dist_rescale(float& m, float& s, float& a, float
     a = m == -INFINITY ? 0.f : fmaf(s, dm, a) * scale;
     s *= scale;
     m = nm;
+  }
+}
+
+// Adds 32 accumulator columns of a row (the first nvalid of them unless FULL) to its running
+// (m, S, A). A's terms are all of one sign, so it keeps full relative accuracy however flat or
+// peaked the row is; log-normaliser - sum p z would cancel.
+template <bool HAS_CAP, bool FULL>
+__device__ __forceinline__ void dist_accumulate(const uint32_t (&r)[32], int nvalid, float k1, float c2, float xlog2e,
+                                                float& m, float& s, float& a) {
+  float z[32];
+  float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float x = __uint_as_float(r[j]);
+    z[j] = HAS_CAP ? fmaf(-2.f * c2, fast_rcp(1.f + fast_ex2(x * k1)), c2) : x * xlog2e;
+    if (FULL || j < nvalid) {
+      if (j & 1) mx1 = fmaxf(mx1, z[j]); else mx0 = fmaxf(mx0, z[j]);
+    }
+  }
+  dist_rescale(m, s, a, fmaxf(mx0, mx1));
+  float s0 = 0.f, s1 = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    if (FULL || j < nvalid) {
+      const float d = z[j] - m, e = fast_ex2(d);
+      if (j & 1) {
+        s1 += e;
+        a1 = fmaf(e, d, a1);
+      } else {
+        s0 += e;
+        a0 = fmaf(e, d, a0);
+      }
+    }
+  }
+  s += s0 + s1;
+  a += a0 + a1;
+}
+
+// The two largest of every G of 32 accumulator columns. The order is that of x (softcap is
+// monotone); the column within the group takes the low bits, which costs 2^-18 of x in the
+// nomination and nothing in the result.
+template <int G, bool FULL>
+__device__ __forceinline__ void top_keys_of(const uint32_t (&r)[32], int nvalid, float2 (&key)[32 / G]) {
+#pragma unroll
+  for (int g = 0; g < 32 / G; ++g) {
+    float b0 = -INFINITY, b1 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const float x = __uint_as_float((r[g * G + j] & ~(uint32_t)(G - 1)) | (uint32_t)j);
+      if (FULL || g * G + j < nvalid) {
+        b1 = fmaxf(b1, fminf(b0, x));
+        b0 = fmaxf(b0, x);
+      }
+    }
+    key[g] = make_float2(b0, b1);
   }
 }
 
@@ -477,7 +544,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             uint8_t* b = a + A_STAGE_BYTES;
             const int k0 = kb * BK;
             if constexpr (CG == 1) {
-              mbar_arrive_expect_tx(&full_bar[s], C::STAGE_BYTES);
+              mbar_arrive_expect_tx(&full_bar[s], P.a_box_bytes ? P.a_box_bytes + C::B_STAGE_BYTES : C::STAGE_BYTES);
               if (!A_MN) {
                 ld1(a, &tmA, &full_bar[s], k0, a_row, hint_a, pol_a);
               } else if (P.a_mn3d) {
@@ -654,7 +721,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const EpiParams& E = P.e;
     const float cap = E.softcap;
     // x of the distribution epilogues, with the accumulator's truncation made up for (dist_scale)
-    constexpr bool kDist = EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || EPI == EPI_DIST_TOP || EPI == EPI_DIST_DZ;
+    constexpr bool kDist = EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || top_group<EPI>() > 0 || EPI == EPI_DIST_DZ;
     const float xs = kDist ? dist_scale(S.K) : 1.f;
     const float xlog2e = kDist ? xs * kLog2e : kLog2e;
     const float k1 = HAS_CAP ? 2.0f * xlog2e / cap : 0.f;  // x -> 2x/c in base 2
@@ -892,8 +959,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               sb ^= 1;
             }
           }
-        } else if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_TOP) {
-          float2 left = make_float2(-INFINITY, -INFINITY);  // TOP: of the group before this one
+        } else if constexpr (EPI == EPI_DIST || top_group<EPI>() > 0) {
+          float2 left = make_float2(-INFINITY, -INFINITY);  // TOP32: the key of the group before this one
 #pragma unroll 1
           for (int c = 0; c < (row_base < S.M ? BN / 64 : 0); ++c) {
             uint32_t r[32];
@@ -901,63 +968,29 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             tmem_ld32(taddr + c * 32, r);
             tmem_wait_ld(r);
             const int nvalid = S.N - (colh + c * 32);  // columns >= nvalid are vocabulary padding (warp-uniform)
-            if constexpr (EPI == EPI_DIST_TOP) {
-              // the order is that of x (softcap is monotone); the column within the group takes
-              // the low 5 bits, which costs 2^-18 of x in the nomination and nothing in the result
-              float b0 = -INFINITY, b1 = -INFINITY;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const float x = __uint_as_float((r[j] & ~31u) | (uint32_t)j);
-                if (j < nvalid) {
-                  b1 = fmaxf(b1, fminf(b0, x));
-                  b0 = fmaxf(b0, x);
-                }
-              }
-              if (c & 1) {
-                if (row_ok)
-                  reinterpret_cast<float4*>(E.top + (size_t)row * (8 * S.tiles_n) + nt * 8 + h * 4)[c >> 1] =
-                      make_float4(left.x, left.y, b0, b1);
-              }
-              left = make_float2(b0, b1);
-            }
-            if (nvalid <= 0) continue;
-            float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float x = __uint_as_float(r[j]);
-              const float z = HAS_CAP ? fmaf(-2.f * c2, fast_rcp(1.f + fast_ex2(x * k1)), c2) : x * xlog2e;
-              r[j] = __float_as_uint(z);
-              if (j < nvalid) {
-                if (j & 1) mx1 = fmaxf(mx1, z); else mx0 = fmaxf(mx0, z);
-              }
-            }
-            dist_rescale(run_m, run_s, run_a, fmaxf(mx0, mx1));
-            // A's terms are all of one sign, so it keeps full relative accuracy however flat or
-            // peaked the row is; -(sum p z) + log-normaliser would cancel
-            float s0 = 0.f, s1 = 0.f, a0 = 0.f, a1 = 0.f;
+            constexpr int G = top_group<EPI>();
+            float2 key[G > 0 ? 32 / (G > 0 ? G : 1) : 1];
             if (nvalid >= 32) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const float d0 = __uint_as_float(r[j]) - run_m, d1 = __uint_as_float(r[j + 1]) - run_m;
-                const float e0 = fast_ex2(d0), e1 = fast_ex2(d1);
-                s0 += e0;
-                s1 += e1;
-                a0 = fmaf(e0, d0, a0);
-                a1 = fmaf(e1, d1, a1);
-              }
+              if constexpr (G > 0) top_keys_of<G, true>(r, 32, key);
+              dist_accumulate<HAS_CAP, true>(r, 32, k1, c2, xlog2e, run_m, run_s, run_a);
             } else {
+              if constexpr (G > 0) top_keys_of<G, false>(r, nvalid, key);
+              if (nvalid > 0) dist_accumulate<HAS_CAP, false>(r, nvalid, k1, c2, xlog2e, run_m, run_s, run_a);
+            }
+            if constexpr (G > 0) {
+              float2* out = E.top + (size_t)row * (BN / G * S.tiles_n) + nt * (BN / G) + h * (BN / 2 / G);
+              if constexpr (G == 32) {
+                // 16 bytes at a time: every second group
+                if ((c & 1) && row_ok)
+                  reinterpret_cast<float4*>(out)[c >> 1] = make_float4(left.x, left.y, key[0].x, key[0].y);
+                left = key[0];
+              } else if (row_ok) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                if (j < nvalid) {
-                  const float d0 = __uint_as_float(r[j]) - run_m;
-                  const float e0 = fast_ex2(d0);
-                  s0 += e0;
-                  a0 = fmaf(e0, d0, a0);
-                }
+                for (int g = 0; g < 32 / G; g += 2)
+                  reinterpret_cast<float4*>(out)[(c * (32 / G) + g) / 2] =
+                      make_float4(key[g].x, key[g].y, key[g + 1].x, key[g + 1].y);
               }
             }
-            run_s += s0 + s1;
-            run_a += a0 + a1;
           }
         } else if constexpr (EPI == EPI_DIST_LOGITS) {
           // the same over 16-column pieces, each also stored as it is
@@ -1183,7 +1216,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // one (max, sum) partial per unit and column half
         if (row_ok) E.part[(size_t)(un.group * 2 + h) * S.M + row] = make_float2(run_m, run_s);
       }
-      if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || EPI == EPI_DIST_TOP) {
+      if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || top_group<EPI>() > 0) {
         if (row_ok) {
           const size_t at = (size_t)(un.group * 2 + h) * S.M + row;
           E.part[at] = make_float2(run_m, run_s);

@@ -324,7 +324,8 @@ LP_API size_t lp_top_workspace_bytes(int64_t T, int64_t V, int k);
 
 /*
  * The k most likely tokens of each row, 1 <= k <= min(LP_TOP_MAX, V), over the whole vocabulary.
- * They are ranked by their dot products H[t] . W[v] in f64, the lowest id first among equals.
+ * They are ranked by their dot products H[t] . W[v] (to 2^-48 of sum |H W|), the lowest id first
+ * among equals.
  *   tokens       int32 [T] or NULL: one given token per row
  *   ids          int32 [T, k]; logps f32 [T, k]: their log-probabilities, most likely first
  *   entropy      f32 [T]
