@@ -1286,7 +1286,7 @@ TopKeys top_keys(int64_t T, int64_t V, int k) {
   K.group = V >= 992 * n ? 32 : (V >= 56 * n ? 8 : 1);
   K.n = (int)cdiv(V, K.group);
   K.ld = K.group > 1 ? cdiv(V, BN) * (BN / K.group) : (V + 3) / 4 * 4;
-  K.row_bytes = (size_t)K.ld * (K.group > 1 ? sizeof(float2) : sizeof(float));
+  K.row_bytes = (size_t)K.ld * (K.group > 1 ? 2 : 1) * sizeof(float);
   K.rows = std::max<int64_t>(1, std::min<int64_t>(T, (int64_t)(((size_t)1 << 30) / K.row_bytes)));
   return K;
 }
@@ -1300,7 +1300,7 @@ size_t top_workspace(int64_t T, int64_t V, int k, const DeviceInfo* di, int sms)
 
 template <bool SAMPLE, int G>
 int launch_top_select(cudaStream_t st, TopParams& P, int64_t rows) {
-  const size_t key_bytes = (size_t)P.n_keys * sizeof(uint32_t);
+  const size_t key_bytes = align_up((size_t)P.n_keys * sizeof(uint32_t), 16);
   P.keys_in_smem = key_bytes <= (size_t)kTopKeyBytes;
   const size_t smem = std::max<size_t>(P.keys_in_smem ? key_bytes : 0, kTopCandBytes);
   auto kern = top_select_kernel<SAMPLE, G>;
@@ -1353,7 +1353,7 @@ int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
     p.e.part_a = reinterpret_cast<float*>(ws + L.part_a_off);
     dist_hints(p);
     if (K.group > 1) {
-      p.e.top = reinterpret_cast<float2*>(ws + L.keys_off);
+      p.e.top = reinterpret_cast<float*>(ws + L.keys_off);
       rc = K.group == 32 ? launch_gemm_cap<EPI_DIST_TOP32, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "top_gemm")
                          : launch_gemm_cap<EPI_DIST_TOP8, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "top_gemm");
     } else {

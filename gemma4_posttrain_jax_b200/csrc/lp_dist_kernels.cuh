@@ -83,16 +83,19 @@ __device__ __forceinline__ double warp_dot_exact(const __nv_bfloat16* __restrict
                                                  const __nv_bfloat16* __restrict__ w, long long d, int lane) {
   TwoSum a, b;
   const int n = (int)(d / 8);
-  for (int i0 = lane; i0 - lane < n; i0 += 256) {
-    // up to 2048 columns of w in flight; h is in L1
-    uint4 w4[8];
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += 128) {
+    uint4 w4[4];
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      w4[u] = i0 + 32 * u < n ? __ldg(reinterpret_cast<const uint4*>(w) + i0 + 32 * u) : make_uint4(0, 0, 0, 0);
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + 32 * u + lane;
+      w4[u] = i < n ? __ldg(reinterpret_cast<const uint4*>(w) + i) : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (i0 - lane + 32 * u >= n) break;  // warp-uniform
-      const uint4 h4 = i0 + 32 * u < n ? __ldg(reinterpret_cast<const uint4*>(h) + i0 + 32 * u) : make_uint4(0, 0, 0, 0);
+    for (int u = 0; u < 4; ++u) {
+      if (i0 + 32 * u >= n) break;
+      // a row of h is in L1; beyond its end w is 0
+      const uint4 h4 = __ldg(reinterpret_cast<const uint4*>(h) + min(i0 + 32 * u + lane, n - 1));
       const uint32_t hv[4] = {h4.x, h4.y, h4.z, h4.w}, wv[4] = {w4[u].x, w4[u].y, w4[u].z, w4[u].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -262,10 +265,11 @@ __global__ void dist_dz_targets_kernel(const int32_t* __restrict__ y, const floa
 // The k most likely tokens of a row, in the order of the exact dot products h . W_v (softcap is
 // monotone), the lowest id first among equals. The GEMM only nominates: a key is one accumulator
 // (f32) or the largest of G neighbours with the second largest beside it. The k + kTopSpare largest
-// keys are selected; of a selected group every column is a candidate if its second largest could be
-// as large as the selected keys are, else only its largest is. Candidates are scored again to 2^-48
-// and ranked by that, so a rounding of the nomination (f32 accumulation, 2^-18 for a group's low
-// bits) can exchange neighbours only if more than kTopSpare values lie within it of the k-th.
+// keys are selected. The k-th largest of the values seen there (keys and second largest) is a lower
+// bound of the k-th logit: a key below it, beyond rounding, is dropped, and a group whose second
+// largest reaches it has all its columns scored. Candidates are scored again to 2^-48 and ranked by
+// that, so a rounding of the nomination (f32 accumulation, 2^-18 for a group's low bits) can
+// exchange neighbours only if more than kTopSpare values lie within it of the k-th.
 //
 // Finding the keys: each thread keeps the largest of the keys it loads; the n-th largest of those
 // kTopThreads maxima is a lower bound of the n-th largest key, and few more than n keys reach it
@@ -303,7 +307,7 @@ struct TopParams {
   long long d, V;
   float cap;
   const float* logits;  // [T, ld_keys] accumulators, or
-  const float2* groups;  // [T, ld_keys] the two largest of every G columns
+  const float* groups;  // [2, T, ld_keys] the largest and the second of every G columns
   long long ld_keys;
   int n_keys;
   int keys_in_smem;
@@ -341,7 +345,7 @@ __device__ __forceinline__ double ordered_f64(long long b) {
 
 // G: columns per key (1: the keys are the accumulators).
 template <bool SAMPLE, int G>
-__global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopParams P) {
+__global__ void __launch_bounds__(kTopThreads, 3) top_select_kernel(const TopParams P) {
   constexpr bool GROUPS = G > 1;
   // keys while selecting, then the candidates' scores and ids
   extern __shared__ __align__(16) uint8_t dyn_s[];
@@ -352,10 +356,11 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
   __shared__ __align__(16) uint32_t max_s[kTopThreads];
   __shared__ float red_s[3][kWarps];
   __shared__ int warp_s[kWarps];
-  __shared__ int n_sel_s, n_cand_s;
+  __shared__ int n_sel_s;
   __shared__ uint32_t lo_s;
   __shared__ int sel_key[kTopSel];
-  __shared__ int sel_at[kTopSel];  // a selected key's first candidate
+  __shared__ float sel_v[2 * kTopSel];  // of the selected keys: [0, n) the keys, [n, 2 n) the second
+  __shared__ float kth_s;
   __shared__ long long best_i[kTopMax];
   __shared__ double best_z[kTopMax];
   __shared__ int best_id[kTopMax];
@@ -363,12 +368,10 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n_keys = P.n_keys;
   const __nv_bfloat16* h = P.H + (size_t)t * P.ldh;
-  const float2* groups = GROUPS ? P.groups + (size_t)t * P.ld_keys : nullptr;
-  const float* logits = GROUPS ? nullptr : P.logits + (size_t)t * P.ld_keys;
+  const float* values = (GROUPS ? P.groups : P.logits) + (size_t)t * P.ld_keys;
 
   auto load_key = [&](int i) -> uint32_t {
-    if constexpr (GROUPS) return ordered_key(group_value<G>(groups[i].x));
-    else return ordered_key(logits[i]);
+    return ordered_key(group_value<G>(values[i]));
   };
   auto key = [&](int i) -> uint32_t { return P.keys_in_smem ? keys_s[i] : load_key(i); };
 
@@ -390,31 +393,17 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
   }
   uint32_t best_key = 0u;
   {
-    // 16 bytes per load: two groups, or four logits (rows are padded to that)
-    constexpr int KV = GROUPS ? 2 : 4;
-    const float4* src = GROUPS ? reinterpret_cast<const float4*>(groups) : reinterpret_cast<const float4*>(logits);
-    const int n_vec = (n_keys + KV - 1) / KV;
-#pragma unroll 8
+    const int n_vec = (n_keys + 3) / 4;  // rows are padded to whole vectors
+#pragma unroll 4
     for (int i = tid; i < n_vec; i += kTopThreads) {
-      const float4 x = __ldg(src + i);
-      uint32_t k[KV];
-      if constexpr (GROUPS) {
-        k[0] = ordered_key(group_value<G>(x.x));
-        k[1] = ordered_key(group_value<G>(x.z));
-      } else {
-        k[0] = ordered_key(x.x);
-        k[1] = ordered_key(x.y);
-        k[2] = ordered_key(x.z);
-        k[3] = ordered_key(x.w);
-      }
-#pragma unroll
-      for (int j = 0; j < KV; ++j) {
-        const int at = i * KV + j;
-        if (at < n_keys) {
-          best_key = max(best_key, k[j]);
-          if (P.keys_in_smem) keys_s[at] = k[j];
-        }
-      }
+      const float4 x = __ldg(reinterpret_cast<const float4*>(values) + i);
+      uint4 k = make_uint4(ordered_key(group_value<G>(x.x)), ordered_key(group_value<G>(x.y)),
+                           ordered_key(group_value<G>(x.z)), ordered_key(group_value<G>(x.w)));
+      if (4 * i + 1 >= n_keys) k.y = 0u;
+      if (4 * i + 2 >= n_keys) k.z = 0u;
+      if (4 * i + 3 >= n_keys) k.w = 0u;
+      best_key = max(max(best_key, max(k.x, k.y)), max(k.z, k.w));
+      if (P.keys_in_smem) reinterpret_cast<uint4*>(keys_s)[i] = k;
     }
   }
   max_s[tid] = best_key;
@@ -425,7 +414,10 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) red_s[0][warp] = m;
-  if (tid == 0) n_sel_s = 0;
+  if (tid == 0) {
+    n_sel_s = 0;
+    kth_s = -INFINITY;
+  }
   nonzero = __syncthreads_or(nonzero);
 
   // ---- row statistics: the partials at the row's maximum, summed in a fixed order
@@ -559,44 +551,49 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
   // ---- candidates of the selected keys: where each key's first one is
   const int n_sel = n_sel_s;  // the keys in shared memory are not read below
   int first = 0, cols = 0;    // this thread's key
+  float v0 = -INFINITY, v1 = -INFINITY;
   if (tid < n_sel) {
-    first = sel_key[tid] * G;
-    cols = 1;
-    if constexpr (GROUPS) {
-      const float2 g = groups[sel_key[tid]];
-      // the second largest against the least selected key, with 2^-16 of slack for the
-      // accumulation and the bits cut off
-      float b1 = group_value<G>(g.y);
-      b1 = b1 + 1.52587890625e-05f * fabsf(b1);
-      if (!nonzero || ordered_key(b1) >= lo) cols = (int)min((long long)G, P.V - first);
-      else first += (int)(__float_as_uint(g.x) & (uint32_t)(G - 1));
-    }
-  }
-  if constexpr (GROUPS) {
-    // exclusive scan over the threads (keys of threads beyond n_sel have none)
-    int x = cols;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) warp_s[warp] = x;
-    __syncthreads();
-    int before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      before += w < warp ? warp_s[w] : 0;
-      total += warp_s[w];
-    }
-    if (tid < n_sel) sel_at[tid] = before + x - cols;
-    if (tid == 0) n_cand_s = total;
-  } else {
-    if (tid < n_sel) sel_at[tid] = tid;
-    if (tid == 0) n_cand_s = n_sel;
+    v0 = values[sel_key[tid]];
+    if constexpr (GROUPS) v1 = group_value<G>(values[(size_t)P.T * P.ld_keys + sel_key[tid]]);
+    sel_v[tid] = group_value<G>(v0);
+    sel_v[n_sel + tid] = v1;
   }
   __syncthreads();
-  const int n_cand = n_cand_s;
-  const int my_at = tid < n_sel ? sel_at[tid] : 0;
+  constexpr int kSeen = GROUPS ? 2 : 1;
+  if (tid < kSeen * n_sel) {
+    const float v = sel_v[tid];
+    int above = 0;
+#pragma unroll 4
+    for (int j = 0; j < kSeen * n_sel; ++j) above += (sel_v[j] > v || (sel_v[j] == v && j < tid)) ? 1 : 0;
+    if (above == P.k - 1) kth_s = v;
+  }
+  __syncthreads();
+  if (tid < n_sel) {
+    // 2^-16 of slack for the accumulation and the bits cut off; comparisons that a NaN fails keep
+    const float least = kth_s - 1.52587890625e-05f * fabsf(kth_s);
+    first = sel_key[tid] * G;
+    cols = !nonzero || !(group_value<G>(v0) < least) ? 1 : 0;
+    if constexpr (GROUPS) {
+      if (!nonzero || !(v1 < least)) cols = (int)min((long long)G, P.V - first);
+      else first += (int)(__float_as_uint(v0) & (uint32_t)(G - 1));
+    }
+  }
+  // exclusive scan over the threads
+  int my_at = cols;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, my_at, o);
+    if (lane >= o) my_at += y;
+  }
+  if (lane == 31) warp_s[warp] = my_at;
+  __syncthreads();
+  my_at -= cols;
+  int n_cand = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    my_at += w < warp ? warp_s[w] : 0;
+    n_cand += warp_s[w];
+  }
   s = a = 0.f;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
@@ -618,9 +615,9 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
     __syncthreads();
     // The candidates' rows of W come from all over it: ask for all of them at once, so that their
     // latencies (HBM and address translation) pass together and not once per round of the warps.
-    const int lines = (int)((P.d * 2 + 127) / 128);
-    for (int i = tid; i < (count - have) * lines; i += kTopThreads)
-      prefetch_l2(reinterpret_cast<const char*>(P.W + (size_t)cand_id[have + i / lines] * P.d) + (size_t)(i % lines) * 128);
+    for (int i = have + warp; i < count; i += kWarps)
+      for (int l = lane * 128; l < (int)P.d * 2; l += 32 * 128)
+        prefetch_l2(reinterpret_cast<const char*>(P.W + (size_t)cand_id[i] * P.d) + l);
 #pragma unroll 1
     for (int i = have + warp; i < count; i += kWarps) {
       const double z = warp_dot_exact(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);

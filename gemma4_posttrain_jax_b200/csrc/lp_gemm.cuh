@@ -36,7 +36,7 @@
 //                 base 2, from which the log-normaliser and the entropy follow.
 //   EPI_DIST_LOGITS : EPI_DIST, with the accumulator stored as f32.
 //   EPI_DIST_TOP32, EPI_DIST_TOP8 : EPI_DIST, with the two largest of every 32 (8) accumulator
-//                 columns (8 bytes, the first's column in its low bits).
+//                 columns, the first's column in its low bits.
 //   EPI_DIST_DZ : recompute path of log-probabilities and entropy; every column of
 //                 dZ = -p * (a + b * log2 p) * softcap' (two row constants), written as bf16 as
 //                 EPI_BWD_DZ does.
@@ -168,7 +168,7 @@ struct EpiParams {
   float2* best;          // HEAD: [n_groups][M] (largest logit, its column as int bits)
   int store_logits;      // HEAD: store the logits through tmO (else only the row statistics)
   float* part_a;         // DIST: [n_groups][M] running A (part holds the running max and S)
-  float2* top;           // DIST_TOP: [M][BN / group * tiles_n] two largest columns of each group
+  float* top;            // DIST_TOP: [2][M][BN / group * tiles_n] largest and second of each group
   const float* row_const;  // DIST_DZ: [3][row_ld] per row: a, b, log2 of the normaliser
   long long row_ld;        // DIST_DZ: row stride of row_const
   const float* g;        // DZ : [M] upstream d logp
@@ -960,7 +960,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             }
           }
         } else if constexpr (EPI == EPI_DIST || top_group<EPI>() > 0) {
-          float2 left = make_float2(-INFINITY, -INFINITY);  // TOP32: the key of the group before this one
+          float4 k1st, k2nd;  // TOP32: this warp's four groups of the tile
 #pragma unroll 1
           for (int c = 0; c < (row_base < S.M ? BN / 64 : 0); ++c) {
             uint32_t r[32];
@@ -978,17 +978,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               if (nvalid > 0) dist_accumulate<HAS_CAP, false>(r, nvalid, k1, c2, xlog2e, run_m, run_s, run_a);
             }
             if constexpr (G > 0) {
-              float2* out = E.top + (size_t)row * (BN / G * S.tiles_n) + nt * (BN / G) + h * (BN / 2 / G);
+              const int ld = BN / G * S.tiles_n;
+              float* out = E.top + (size_t)row * ld + nt * (BN / G) + h * (BN / 2 / G);
               if constexpr (G == 32) {
-                // 16 bytes at a time: every second group
-                if ((c & 1) && row_ok)
-                  reinterpret_cast<float4*>(out)[c >> 1] = make_float4(left.x, left.y, key[0].x, key[0].y);
-                left = key[0];
+                k1st.x = c == 0 ? key[0].x : k1st.x;
+                k2nd.x = c == 0 ? key[0].y : k2nd.x;
+                k1st.y = c == 1 ? key[0].x : k1st.y;
+                k2nd.y = c == 1 ? key[0].y : k2nd.y;
+                k1st.z = c == 2 ? key[0].x : k1st.z;
+                k2nd.z = c == 2 ? key[0].y : k2nd.z;
+                k1st.w = key[0].x;
+                k2nd.w = key[0].y;
+                if (c == 3 && row_ok) {
+                  *reinterpret_cast<float4*>(out) = k1st;
+                  *reinterpret_cast<float4*>(out + (size_t)S.M * ld) = k2nd;
+                }
               } else if (row_ok) {
-#pragma unroll
-                for (int g = 0; g < 32 / G; g += 2)
-                  reinterpret_cast<float4*>(out)[(c * (32 / G) + g) / 2] =
-                      make_float4(key[g].x, key[g].y, key[g + 1].x, key[g + 1].y);
+                *reinterpret_cast<float4*>(out + c * 4) = make_float4(key[0].x, key[1].x, key[2].x, key[3].x);
+                *reinterpret_cast<float4*>(out + c * 4 + (size_t)S.M * ld) =
+                    make_float4(key[0].y, key[1].y, key[2].y, key[3].y);
               }
             }
           }
