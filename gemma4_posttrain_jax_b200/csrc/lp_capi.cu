@@ -220,6 +220,9 @@ int current_device_info(DeviceInfo** out) {
   int dev = 0;
   LP_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kMaxDevices) return fail(LP_EINVAL, "device ordinal %d out of range", dev);
+  // a thread that has made no runtime call yet (one of autograd's, say) has a current device but no
+  // context, which the driver's tensor-map encoder needs
+  LP_CUDA_TRY(cudaSetDevice(dev));
   std::lock_guard<std::mutex> lk(g_dev_mu);
   DeviceInfo& d = g_dev[dev];
   if (!d.ready) {
@@ -386,9 +389,14 @@ int launch_gemm_cg(cudaStream_t st, const CUtensorMap& a, const CUtensorMap& b, 
   const int grid = CG * std::max(1, std::min(p.s.num_units, workers(di, CG)));
   GemmParams pp = p;
   pp.dbg = dbg_ptr(tag);
-  // callers that keep a zeroed counter of their own (in their workspace) pass it in
+  // a caller that keeps a counter of its own (in its workspace) passes it in; where every worker
+  // has one unit it needs no counter and no memset (the distribution operators' small calls)
   if (pp.sched == nullptr) {
     if (int rc = sched_slot(st, &pp.sched)) return rc;
+  } else if (p.s.num_units * CG <= grid) {
+    pp.sched = nullptr;
+  } else if (!p.sched_zeroed) {
+    LP_CUDA_TRY(cudaMemsetAsync(pp.sched, 0, sizeof(unsigned), st));
   }
   ProfScope prof(st, tag);
   if constexpr (CG == 1) {
@@ -829,6 +837,20 @@ struct MeshSum {
   unsigned long long limit_ns;
 };
 
+// CTA group of the distribution operators' GEMMs [M, N]. At equal tile counts pairs are faster (a
+// 256-row tile takes 0.94 of the time of two 128-row tiles: 512 rows of the 262144 x 2048 head 434
+// against 462 us, 1024 rows 826 / 868), but a last half-empty pair tile or a last round that pairs
+// fill badly costs more (128 rows 215 / 179 us, 301 rows 403 / 381, 1100 rows 1110 / 1013). Rounds
+// of the persistent workers decide, single CTAs' against 0.94 of the pairs'.
+int cta_group_dist(int64_t M, int64_t N, const DeviceInfo* di, CgUse use) {
+  const int f = forced_cta_group();
+  if (f) return f;
+  const int w1 = di != nullptr ? workers(di, 1) : 148, w2 = di != nullptr ? workers(di, 2) : 74;
+  const int64_t tn = cdiv(N, BN);
+  const double one = (double)cdiv(cdiv(M, 128) * tn, w1), two = 0.94 * (double)cdiv(cdiv(M, 256) * tn, w2);
+  return one <= two ? 1 : cta_group_for(use);
+}
+
 // The backward of given tokens' log-probabilities and the entropy (lp_dist_bwd): K tokens per row
 // and two row constants take the place of one target and its gradient.
 struct DistGrad {
@@ -837,18 +859,28 @@ struct DistGrad {
   const float *zt, *lse, *entropy, *g, *ge;
 };
 
-// Scratch of lp_dist_bwd before the layout of lp_bwd: the work counters of every GEMM launch
-// (three per chunk), then the row constants. In the workspace, not in the library's rotating
+// Plan and scratch of lp_dist_bwd: the work counters of every GEMM launch (three per chunk) and the
+// row constants, before the layout of lp_bwd. In the workspace, not in the library's rotating
 // slots, a counter belongs to the call (or to the captured graph) that zeroes it.
-struct DistBwdLayout {
-  size_t counters_bytes, row_off, base;
+struct DistBwdPlan {
+  int cg_dz, cg_dh;
+  bool split_dh;  // whether the dH GEMM may split K
+  BwdLayout L;
+  size_t row_off, base;
 };
-DistBwdLayout dist_bwd_layout(int64_t T, int64_t chunks) {
-  DistBwdLayout L;
-  L.counters_bytes = align_up((size_t)std::max<int64_t>(chunks, 1) * 3 * sizeof(unsigned), 1024);
-  L.row_off = L.counters_bytes;
-  L.base = L.row_off + align_up((size_t)T * 3 * sizeof(float), 1024);
-  return L;
+DistBwdPlan dist_bwd_plan(int64_t T, int64_t d, int64_t Vs, int64_t token_chunk, int flags, const DeviceInfo* di) {
+  DistBwdPlan P;
+  const int64_t tc = token_chunk > 0 ? std::min<int64_t>(token_chunk, T) : default_token_chunk(T, Vs, d);
+  P.cg_dz = cta_group_dist(tc, Vs, di, CG_DZ);
+  // rows of one M tile waste half of a pair whatever the split of K; and a reduce launch takes
+  // about as long as 16 K blocks
+  P.split_dh = cdiv(Vs, BK) > 32;
+  P.cg_dh = forced_cta_group() == 0 && tc <= 128 ? 1 : cta_group_for(CG_DH);
+  if (!P.split_dh) flags |= LP_BWD_NO_DH;  // no room for partials
+  P.L = bwd_layout(T, d, Vs, token_chunk, flags, di != nullptr ? workers(di, P.cg_dh) : 148 / P.cg_dh, 128 * P.cg_dh);
+  P.row_off = align_up((size_t)std::max<int64_t>(P.L.chunks, 1) * 3 * sizeof(unsigned), 1024);
+  P.base = P.row_off + align_up((size_t)T * 3 * sizeof(float), 1024);
+  return P;
 }
 
 int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs, int64_t v_off,
@@ -871,31 +903,37 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
     if (want_dw) LP_CUDA_TRY(cudaMemsetAsync(dW, 0, (size_t)Vs * d * (dw_bf16 ? 2 : 4), st));
     return LP_OK;
   }
-  const int cg_dz = cta_group_for(CG_DZ), cg_dh = cta_group_for(CG_DH);
+  DistBwdPlan DP{};
+  if (dist != nullptr) DP = dist_bwd_plan(T, d, Vs, token_chunk, flags, di);
+  const int cg_dz = dist != nullptr ? DP.cg_dz : cta_group_for(CG_DZ);
+  const int cg_dh = dist != nullptr ? DP.cg_dh : cta_group_for(CG_DH);
+  const bool split_dh = dist != nullptr ? DP.split_dh : ms == nullptr;
   if (ms != nullptr && want_dh) {
     // chunks start on 256-row boundaries (the row-block counters are per 128 rows)
     if (token_chunk <= 0) token_chunk = default_token_chunk(T, Vs, d);
     if (token_chunk < T) token_chunk = std::max<int64_t>(256, token_chunk / 256 * 256);
   }
-  const BwdLayout L = bwd_layout(T, d, Vs, token_chunk, flags, workers(di, cg_dh), 128 * cg_dh);
-  DistBwdLayout DL{};
-  if (dist != nullptr) DL = dist_bwd_layout(T, L.chunks);
-  if (workspace == nullptr || workspace_bytes < DL.base + L.total)
+  const BwdLayout L =
+      dist != nullptr ? DP.L : bwd_layout(T, d, Vs, token_chunk, flags, workers(di, cg_dh), 128 * cg_dh);
+  if (workspace == nullptr || workspace_bytes < DP.base + L.total)
     return fail(LP_EWORKSPACE, "%s needs %zu workspace bytes, got %zu", dist != nullptr ? "lp_dist_bwd" : "lp_bwd",
-                DL.base + L.total, workspace_bytes);
+                DP.base + L.total, workspace_bytes);
   if ((reinterpret_cast<uintptr_t>(workspace) & 1023) != 0) return fail(LP_EINVAL, "workspace must be 1024-byte aligned");
   unsigned* counters = nullptr;  // the next launch's work counter (dist only)
   float* row_const = nullptr;
   if (dist != nullptr) {
     counters = reinterpret_cast<unsigned*>(workspace);
-    row_const = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + DL.row_off);
-    LP_CUDA_TRY(cudaMemsetAsync(counters, 0, DL.counters_bytes, st));
-    ProfScope prof(st, "dist_row_const");
-    dist_row_const_kernel<<<(unsigned)cdiv(T, 256), 256, 0, st>>>(dist->lse, dist->entropy, y, dist->g, dist->ge,
-                                                                  (int)T, dist->K, dist->V, row_const);
-    LP_LAUNCH_CHECK("dist_row_const_kernel");
+    row_const = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + DP.row_off);
+    if (dist->K == 1) {
+      row_const = nullptr;  // the dZ epilogue takes one token per row itself
+    } else {
+      ProfScope prof(st, "dist_row_const");
+      dist_row_const_kernel<<<(unsigned)cdiv(T, 256), 256, 0, st>>>(dist->lse, dist->entropy, y, dist->g, dist->ge,
+                                                                    (int)T, dist->K, dist->V, row_const);
+      LP_LAUNCH_CHECK("dist_row_const_kernel");
+    }
   }
-  char* ws = reinterpret_cast<char*>(workspace) + DL.base;
+  char* ws = reinterpret_cast<char*>(workspace) + DP.base;
   __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>(ws + L.dz_off);
   float* part = reinterpret_cast<float*>(ws + L.part_off);
   float* dw_acc = (want_dw && dw_bf16 && L.chunks > 1) ? reinterpret_cast<float*>(ws + L.dwacc_off)
@@ -919,11 +957,21 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
       p.e.softcap = softcap;
       set_hints(p, G_DZ);
       if (dist != nullptr) {
-        p.e.row_const = row_const + t0;
-        p.e.row_ld = T;
+        if (row_const != nullptr) {
+          p.e.row_const = row_const + t0;
+          p.e.row_ld = T;
+        } else {
+          p.e.y = y + t0;
+          p.e.v_off = v_off;
+          p.e.vocab = dist->V;
+          p.e.g = dist->g != nullptr ? dist->g + t0 : nullptr;
+          p.e.ge = dist->ge != nullptr ? dist->ge + t0 : nullptr;
+          p.e.lse = dist->lse + t0;
+          p.e.entropy = dist->entropy + t0;
+        }
         p.sched = counters++;
         if ((rc = launch_gemm_cap<EPI_DIST_DZ, false, false>(cap, st, ta, tb, to, p, di, "dist_dz_gemm"))) return rc;
-        const int64_t slots = tcur * dist->K;
+        const int64_t slots = row_const != nullptr ? tcur * dist->K : 0;
         if (slots > 0) {
           ProfScope prof(st, "dist_dz_targets");
           dist_dz_targets_kernel<<<(unsigned)cdiv(slots, 256), 256, 0, st>>>(
@@ -950,7 +998,7 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
       else rc = map_bf16(&tb, W, d, Vs, d, 64, 64, "embedding as MN-major B");
       if (rc) return rc;
       const int wk = workers(di, cg_dh);
-      p.s = plan_gemm(tcur, d, Vs, wk, ms == nullptr, 1, 128 * cg_dh);
+      p.s = plan_gemm(tcur, d, Vs, wk, split_dh, 1, 128 * cg_dh);
       char* dh_c = reinterpret_cast<char*>(dH) + (size_t)t0 * ld_dh * (dh_f32 ? 4 : 2);
       if (ms != nullptr) {
         // partial tiles stored (bf16) into this rank's copy, summed across ranks by the
@@ -1212,17 +1260,6 @@ int lp_peer_barrier(void* stream, const unsigned long long* signal_pads, int ran
 // ============================================================================= distribution operators
 namespace {
 
-// CTA group of a launch over T rows. An odd number of 128-row tiles leaves half of the last pair's
-// tile empty, and up to 15 tiles that costs more than pairs gain. Measured against the 262144 x 2048
-// head, single CTAs / pairs: 128 rows 179 / 215 us, 256 rows 250 / 224, 301 rows 381 / 403, 512 rows
-// 462 / 434, 1100 rows 1013 / 1110, 2048 rows 1766 / 1733.
-int cta_group_dist(int64_t T) {
-  const int f = forced_cta_group();
-  if (f) return f;
-  const int64_t tiles = cdiv(T, 128);
-  return tiles % 2 == 1 && tiles <= 15 ? 1 : cta_group_for(CG_FWD);
-}
-
 struct DistFwdLayout {
   GemmSched s;
   int cg;
@@ -1233,7 +1270,7 @@ struct DistFwdLayout {
 // rows' selection keys.
 DistFwdLayout dist_fwd_layout(int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di, int sms, size_t key_row_bytes) {
   DistFwdLayout L{};
-  L.cg = cta_group_dist(T);
+  L.cg = cta_group_dist(T, Vs, di, CG_FWD);
   L.s = plan_fwd(T, Vs, d, di != nullptr ? workers(di, L.cg) : sms / L.cg, 128 * L.cg);
   L.part_off = 256;
   L.part_a_off = L.part_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float2), 256);
@@ -1343,7 +1380,6 @@ int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
     alignas(64) CUtensorMap ta, tb, to;
     if ((rc = map_bf16(&ta, Hc, d, n, ldh, BK, a_box_rows(L, n), "hidden"))) return rc;
     if ((rc = map_bf16(&tb, W, d, V, d, BK, b_box_rows(L.cg), "embedding"))) return rc;
-    LP_CUDA_TRY(cudaMemsetAsync(ws, 0, sizeof(unsigned), st));
     GemmParams p{};
     p.s = L.s;
     p.a_box_bytes = a_box_bytes(L, n);
@@ -1430,7 +1466,6 @@ int lp_dist_fwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, 
   alignas(64) CUtensorMap ta, tb;
   if ((rc = map_bf16(&ta, H, d, T, ldh, BK, a_box_rows(L, T), "hidden"))) return rc;
   if ((rc = map_bf16(&tb, W, d, Vs, d, BK, b_box_rows(L.cg), "embedding"))) return rc;
-  LP_CUDA_TRY(cudaMemsetAsync(ws, 0, sizeof(unsigned), st));
   GemmParams p{};
   p.s = L.s;
   p.a_box_bytes = a_box_bytes(L, T);
@@ -1479,8 +1514,10 @@ int lp_dist_combine(void* stream, const float* shard_stats, const float* shard_z
 
 size_t lp_dist_bwd_workspace_bytes(int64_t T, int64_t d, int64_t Vs, int64_t token_chunk, int flags) {
   if (T <= 0 || Vs <= 0 || d <= 0) return 256;
-  const int64_t tc = token_chunk > 0 ? std::min<int64_t>(token_chunk, T) : default_token_chunk(T, Vs, d);
-  return dist_bwd_layout(T, cdiv(T, tc)).base + lp_bwd_workspace_bytes(T, d, Vs, token_chunk, flags);
+  DeviceInfo* di = nullptr;
+  const bool have = current_device_info(&di) == LP_OK;
+  const DistBwdPlan P = dist_bwd_plan(T, d, Vs, token_chunk, flags, have ? di : nullptr);
+  return P.base + P.L.total;
 }
 
 int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs,

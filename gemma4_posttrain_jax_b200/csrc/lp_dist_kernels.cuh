@@ -77,11 +77,24 @@ struct TwoSum {
   }
 };
 
+// Two such sums side by side; a - b is an FMA with -1, rounded once as a subtraction is.
+struct TwoSum2 {
+  f32x2 s = 0, e = 0;
+  __device__ __forceinline__ void add(f32x2 p, f32x2 minus_one) {
+    const f32x2 t = add_f32x2(s, p);
+    const f32x2 b = fma_f32x2(s, minus_one, t);
+    const f32x2 c = fma_f32x2(b, minus_one, t);
+    e = add_f32x2(e, add_f32x2(fma_f32x2(c, minus_one, s), fma_f32x2(b, minus_one, p)));
+    s = t;
+  }
+};
+
 // h . w over one warp (complete in lane 0), to about 2^-48 of sum |h w|: products of two bf16 numbers
 // are exact in f32. f64 would convert every product, which took three times as long.
 __device__ __forceinline__ double warp_dot_exact(const __nv_bfloat16* __restrict__ h,
                                                  const __nv_bfloat16* __restrict__ w, long long d, int lane) {
-  TwoSum a, b;
+  TwoSum2 both;  // of the even and of the odd columns
+  const f32x2 minus_one = pack_f32x2(-1.f, -1.f);
   const int n = (int)(d / 8);
 #pragma unroll 1
   for (int i0 = 0; i0 < n; i0 += 128) {
@@ -98,12 +111,15 @@ __device__ __forceinline__ double warp_dot_exact(const __nv_bfloat16* __restrict
       const uint4 h4 = __ldg(reinterpret_cast<const uint4*>(h) + min(i0 + 32 * u + lane, n - 1));
       const uint32_t hv[4] = {h4.x, h4.y, h4.z, h4.w}, wv[4] = {w4[u].x, w4[u].y, w4[u].z, w4[u].w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a.add(__fmul_rn(__uint_as_float(hv[j] << 16), __uint_as_float(wv[j] << 16)));
-        b.add(__fmul_rn(__uint_as_float(hv[j] & 0xffff0000u), __uint_as_float(wv[j] & 0xffff0000u)));
-      }
+      for (int j = 0; j < 4; ++j)
+        both.add(mul_f32x2(pack_f32x2(__uint_as_float(hv[j] << 16), __uint_as_float(hv[j] & 0xffff0000u)),
+                           pack_f32x2(__uint_as_float(wv[j] << 16), __uint_as_float(wv[j] & 0xffff0000u))),
+                 minus_one);
     }
   }
+  TwoSum a, b;
+  unpack_f32x2(both.s, a.s, b.s);
+  unpack_f32x2(both.e, a.e, b.e);
   a.add(b);
 #pragma unroll 1
   for (int o = 16; o > 0; o >>= 1) {
@@ -135,6 +151,15 @@ __global__ void __launch_bounds__(kDistThreads)
   const int t0 = blockIdx.x * R;
   const int r = threadIdx.x % R;
   const int t = t0 + r;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows = min(R, T - t0);
+  // the tokens' rows of W come from all over it: ask for them before the partials are merged
+  for (int i = warp; i < rows * K; i += kDistThreads / 32) {
+    const long long v = (long long)y[(size_t)(t0 + i / K) * K + i % K] - v_off;
+    if (v >= 0 && v < Vs)
+      for (int l = lane * 128; l < (int)d * 2; l += 32 * 128)
+        prefetch_l2(reinterpret_cast<const char*>(W + (size_t)v * d) + l);
+  }
   DistAcc acc{-INFINITY, 0.f, 0.f};
   if (t < T) {
     for (int g = threadIdx.x / R; g < n_parts; g += kDistThreads / R) {
@@ -162,8 +187,6 @@ __global__ void __launch_bounds__(kDistThreads)
     if (entropy != nullptr) entropy[t] = dist_entropy(acc);
   }
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rows = min(R, T - t0);
   for (int i = warp; i < rows * K; i += kDistThreads / 32) {
     const int rr = i / K;
     const size_t at = (size_t)(t0 + rr) * K + i % K;
@@ -290,6 +313,11 @@ __device__ __forceinline__ uint32_t ordered_key(float x) {
   const uint32_t b = __float_as_uint(x);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+// Its inverse (0, a NaN's key, becomes -inf).
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k <= 0x007fffffu) return -INFINITY;
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
 // A group's value without its column bits.
 template <int G>
 __device__ __forceinline__ float group_value(float x) {
@@ -414,10 +442,7 @@ __global__ void __launch_bounds__(kTopThreads, 3) top_select_kernel(const TopPar
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) red_s[0][warp] = m;
-  if (tid == 0) {
-    n_sel_s = 0;
-    kth_s = -INFINITY;
-  }
+  if (tid == 0) n_sel_s = 0;
   nonzero = __syncthreads_or(nonzero);
 
   // ---- row statistics: the partials at the row's maximum, summed in a fixed order
@@ -559,13 +584,34 @@ __global__ void __launch_bounds__(kTopThreads, 3) top_select_kernel(const TopPar
     sel_v[n_sel + tid] = v1;
   }
   __syncthreads();
-  constexpr int kSeen = GROUPS ? 2 : 1;
-  if (tid < kSeen * n_sel) {
-    const float v = sel_v[tid];
-    int above = 0;
-#pragma unroll 4
-    for (int j = 0; j < kSeen * n_sel; ++j) above += (sel_v[j] > v || (sel_v[j] == v && j < tid)) ? 1 : 0;
-    if (above == P.k - 1) kth_s = v;
+  if (warp == 0) {
+    // a value that at least k of those seen reach, and nearly no more
+    constexpr int kSeen = (GROUPS ? 2 : 1) * kTopSel / 32;
+    uint32_t v[kSeen];
+    uint32_t top = 0u;
+#pragma unroll
+    for (int j = 0; j < kSeen; ++j) {
+      const int i = j * 32 + lane;
+      v[j] = i < (GROUPS ? 2 : 1) * n_sel ? ordered_key(sel_v[i]) : 0u;
+      top = max(top, v[j]);
+    }
+    uint32_t at = min(lo, __reduce_max_sync(0xffffffffu, top));
+    unsigned long long hi = (unsigned long long)__reduce_max_sync(0xffffffffu, top) + 1;
+    int c_at = 2 * kTopSel;
+    while (c_at > P.k && hi - at > 1) {
+      const uint32_t mid = (uint32_t)(at + (hi - at) / 2);
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < kSeen; ++j) c += v[j] >= mid ? 1 : 0;
+      c = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
+      if (c >= P.k) {
+        at = mid;
+        c_at = c;
+      } else {
+        hi = mid;
+      }
+    }
+    if (lane == 0) kth_s = key_value(at);
   }
   __syncthreads();
   if (tid < n_sel) {

@@ -37,9 +37,9 @@
 //   EPI_DIST_LOGITS : EPI_DIST, with the accumulator stored as f32.
 //   EPI_DIST_TOP32, EPI_DIST_TOP8 : EPI_DIST, with the two largest of every 32 (8) accumulator
 //                 columns, the first's column in its low bits.
-//   EPI_DIST_DZ : recompute path of log-probabilities and entropy; every column of
-//                 dZ = -p * (a + b * log2 p) * softcap' (two row constants), written as bf16 as
-//                 EPI_BWD_DZ does.
+//   EPI_DIST_DZ : recompute path of log-probabilities and entropy:
+//                 dZ = (g * onehot - p * (a + b * log2 p)) * softcap' with two row constants a, b,
+//                 written as bf16 as EPI_BWD_DZ does.
 //
 // Synchronisation (all waits bounded, see lp_ptx.cuh):
 //   full[s]   : TMA -> MMA. CG=2: lives in the leader, counts both CTAs' bytes.
@@ -169,8 +169,10 @@ struct EpiParams {
   int store_logits;      // HEAD: store the logits through tmO (else only the row statistics)
   float* part_a;         // DIST: [n_groups][M] running A (part holds the running max and S)
   float* top;            // DIST_TOP: [2][M][BN / group * tiles_n] largest and second of each group
-  const float* row_const;  // DIST_DZ: [3][row_ld] per row: a, b, log2 of the normaliser
-  long long row_ld;        // DIST_DZ: row stride of row_const
+  const float* row_const;  // DIST_DZ: [3][row_ld] per row: a, b, log2 of the normaliser; or null,
+  long long row_ld;        //          then one token per row: its y and g (above), the vocabulary's
+  long long vocab;         //          size, and per row the log-normaliser, the entropy and its
+  const float *lse, *entropy, *ge;  // gradient (null: none)
   const float* g;        // DZ : [M] upstream d logp
   const float* stats;    // DZ : [2][stats_ld] global (max, sum) in natural units
   long long stats_ld;    // DZ : row stride of stats
@@ -201,8 +203,10 @@ struct GemmParams {
   // issued, [6] epilogue-warp cycles from accumulator ready to hand-back (warp 2), [7] tiles.
   unsigned long long* dbg;
   // Dynamic work distribution: units are claimed in order with atomicAdd on this counter
-  // (zero at launch), so the units in flight always form a compact window of the unit order.
+  // (zero at launch), so the units in flight always form a compact window of the unit order. Null
+  // where every worker of the grid has one unit.
   unsigned int* sched;
+  int sched_zeroed;  // host side: sched is zero already
   // MN-major operands with 3-D tensor maps (64 columns, K, 64-column chunks): the CTA's
   // tile of that operand is one TMA instruction instead of one per 64-column chunk.
   int a_mn3d, b_mn3d;
@@ -512,7 +516,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                                      : mbar_wait_bounded_cluster(&sempty_bar[slot], sph ^ 1, abort_flag,
                                                                  DEV_TIMEOUT_PRODUCER);
           if (!free_slot) break;
-          const unsigned claimed = atomicAdd(P.sched, 1u);
+          // no counter: as many workers as units, one unit each
+          const unsigned claimed =
+              P.sched != nullptr ? atomicAdd(P.sched, 1u) : (i == 0 ? blockIdx.x / CG : (unsigned)S.num_units);
           u = claimed < (unsigned)S.num_units ? (int)claimed : -1;
           sched_u[slot] = u;
           if constexpr (CG == 2) {
@@ -760,10 +766,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       float run_a = 0.f;               // DIST: sum of 2^(z - run_m) (z - run_m)
       float row_a = 0.f, row_b = 0.f;  // DIST_DZ: the row's constants
       if (EPI == EPI_DIST_DZ) {
-        if (row_ok) {
+        if (row_ok && E.row_const != nullptr) {
           row_a = E.row_const[row];
           row_b = E.row_const[E.row_ld + row];
           l2 = E.row_const[2 * E.row_ld + row];
+        } else if (row_ok) {
+          // one token per row: its constants as in dist_row_const_kernel, its entry below
+          const long long v = (long long)E.y[row];
+          if (E.g != nullptr && v >= 0 && v < E.vocab) {
+            gv = E.g[row];
+            const long long t = v - E.v_off;
+            yl = (t >= 0 && t < (long long)S.N) ? (int)t : -1;
+          }
+          const float e = E.ge != nullptr ? E.ge[row] : 0.f;
+          row_a = e != 0.f ? fmaf(e, E.entropy[row], gv) : gv;
+          row_b = e * kLn2;
+          l2 = E.lse[row] * kLog2e;
         }
       }
       if (EPI == EPI_FWD_LSE) {
@@ -1055,26 +1073,34 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             tmem_ld32(taddr + pc * 32, r);
             tmem_wait_ld(r);
             const int col0 = colh + pc * 32;
-            // log2 p = z2 - l2, p = 2^(log2 p), dZ = -p * (a + b log2 p) * softcap'; the given
-            // tokens' own terms are written over these afterwards (dist_dz_targets_kernel)
-            uint32_t pk[16];
+            // log2 p = z2 - l2, p = 2^(log2 p), dZ = softcap' * (g [v = y] - p * (a + b log2 p)).
+            // The entries of several given tokens are written over these (dist_dz_targets_kernel).
+            const int tj = yl - col0;
+            float v[32];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float v[2];
+            for (int j = 0; j < 32; ++j) {
+              const float x = __uint_as_float(r[j]);
+              if (HAS_CAP) {
+                const float rr = fast_rcp(1.f + fast_ex2(x * k1));
+                const float lp = fmaf(-2.f * c2, rr, c2 - l2);
+                v[j] = (-4.f * rr) * (1.f - rr) * (fast_ex2(lp) * fmaf(row_b, lp, row_a));
+              } else {
+                const float lp = fmaf(x, xlog2e, -l2);
+                v[j] = -fast_ex2(lp) * fmaf(row_b, lp, row_a);
+              }
+            }
+            if ((unsigned)tj < 32u) {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const float x = __uint_as_float(r[2 * j + i]);
-                if (HAS_CAP) {
-                  const float rr = fast_rcp(1.f + fast_ex2(x * k1));
-                  const float lp = fmaf(-2.f * c2, rr, c2 - l2);
-                  v[i] = (-4.f * rr) * (1.f - rr) * (fast_ex2(lp) * fmaf(row_b, lp, row_a));
-                } else {
-                  const float lp = fmaf(x, xlog2e, -l2);
-                  v[i] = -fast_ex2(lp) * fmaf(row_b, lp, row_a);
+              for (int j = 0; j < 32; ++j) {
+                if (j == tj) {
+                  const float rr = HAS_CAP ? fast_rcp(1.f + fast_ex2(__uint_as_float(r[j]) * k1)) : 0.f;
+                  v[j] += HAS_CAP ? gv * (4.f * rr * (1.f - rr)) : gv;
                 }
               }
-              pk[j] = pack_bf16x2(v[0], v[1]);
             }
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) pk[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
             if (lane == 0) bulk_wait_read<1>();
             __syncwarp();
             uint8_t* buf_s = my_staging + sb * SBUF;

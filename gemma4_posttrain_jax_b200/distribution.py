@@ -49,84 +49,99 @@ def _as_int32(tokens: torch.Tensor) -> torch.Tensor:
 
 def _gather(rows: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
     """``rows`` [n] or [n, w] (f32 or int32) at ``idx``."""
-    return _gather_rows(rows.view(torch.float32), idx).view(rows.dtype)
+    return _gather_rows(rows.view(torch.float32), idx).view(rows.dtype) if rows.numel() else rows[: idx.numel()]
 
 
 class _TokenLogpsAndEntropy(torch.autograd.Function):
+    """hidden [..., d] and int32 tokens [T, K] to logps ``shape`` and entropy [...]. The reshapes are in
+    here: outside, each would be a node of the autograd graph of its own."""
+
     @staticmethod
-    def forward(ctx, embed, hidden, tokens, softcap, mesh, token_chunk, dh_reduce_f32, skip_zero_grad):
+    def forward(ctx, embed, hidden, tokens, shape, softcap, mesh, token_chunk, dh_reduce_f32, skip_zero_grad):
+        T, K = tokens.shape
+        h = hidden.reshape(T, hidden.shape[-1])
+        logp = torch.empty(shape, dtype=torch.float32, device=hidden.device)
+        entropy = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=hidden.device)
         P = mesh.size if mesh is not None else 1
-        vocab = embed.shape[0] * P
         off = 0
         if P > 1:
             off = vocab_offset(embed.shape[0], mesh)
-            stats, zt = ops.dist_forward(embed, hidden, tokens, softcap, vocab_offset=off, shard=True)
+            stats, zt = ops.dist_forward_shard(embed, h, tokens, softcap, off)
             with phase("stats_all_gather"):
                 both = all_gather_stats(torch.cat([stats.reshape(-1), zt.reshape(-1)]), mesh)
-            T, K = tokens.shape
-            logp, entropy, zt, lse = ops.dist_combine(
-                both[:, : 3 * T].reshape(P, 3, T), both[:, 3 * T :].reshape(P, T, K), tokens, vocab
+            saved = ops.dist_combine(
+                both[:, : 3 * T].reshape(P, 3, T), both[:, 3 * T :].reshape(P, T, K), tokens, embed.shape[0] * P, logp,
+                entropy,
             )
         else:
-            logp, entropy, zt, lse = ops.dist_forward(embed, hidden, tokens, softcap)
-        ctx.save_for_backward(embed, hidden, tokens, zt, lse, entropy)
-        ctx.meta = (softcap, mesh, P, off, vocab, token_chunk, dh_reduce_f32, skip_zero_grad)
+            saved = ops.dist_forward(embed, h, tokens, softcap, logp, entropy)
+        ctx.save_for_backward(embed, hidden, tokens, saved, entropy)
+        ctx.meta = (softcap, mesh, P, off, token_chunk, dh_reduce_f32, skip_zero_grad)
         ctx.set_materialize_grads(False)
         return logp, entropy
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, ge):
-        embed, hidden, tokens, zt, lse, entropy = ctx.saved_tensors
-        softcap, mesh, P, off, vocab, token_chunk, dh_reduce_f32, skip_zero_grad = ctx.meta
         need_dw, need_dh = ctx.needs_input_grad[:2]
-        none = (None,) * 8
+        none = (None,) * 7
         if (g is None and ge is None) or not (need_dw or need_dh):
-            return none
-        g = None if g is None else g.to(torch.float32).contiguous()
-        ge = None if ge is None else ge.to(torch.float32).contiguous()
-        T, d = hidden.shape
+            return None, None, *none
+        embed, hidden, tokens, saved, entropy = ctx.saved_tensors
+        softcap, mesh, P, off, token_chunk, dh_reduce_f32, skip_zero_grad = ctx.meta
+        T, K = tokens.shape
+        d = hidden.shape[-1]
         if T == 0:
-            return (torch.zeros_like(embed) if need_dw else None, torch.zeros_like(hidden) if need_dh else None) + none[2:]
-        sel = None
-        if skip_zero_grad and 6.0 * T * d * embed.shape[0] >= _SKIP_MIN_FLOPS and not torch.cuda.is_current_stream_capturing():
-            sent = torch.zeros((T,), dtype=torch.bool, device=hidden.device) if ge is None else ge != 0
-            if g is not None and g.shape[1] > 0:
-                sent = sent | (g != 0).any(dim=1)
-            sel = _nonzero_grad_rows(sent)
+            return (torch.zeros_like(embed) if need_dw else None), (torch.zeros_like(hidden) if need_dh else None), *none
+        g = None if g is None else g.contiguous()
+        ge = None if ge is None else ge.contiguous()
+        rows = hidden.reshape(T, d)
         pos = None
-        rows = hidden
-        if sel is not None:
-            idx, pos, m = sel
-            if m == 0:
-                dW = torch.zeros_like(embed) if need_dw else None
-                return (dW, torch.zeros_like(hidden) if need_dh else None) + none[2:]
-            rows = _gather_rows(hidden, idx)
-            tokens, zt, lse, entropy = (_gather(x, idx) if x.numel() else x[:m] for x in (tokens, zt, lse, entropy))
-            g = g if g is None else (_gather(g, idx) if g.numel() else g[:m])
-            ge = ge if ge is None else _gather(ge, idx)
+        if (
+            skip_zero_grad
+            and 6.0 * T * d * embed.shape[0] >= _SKIP_MIN_FLOPS
+            and not torch.cuda.is_current_stream_capturing()
+        ):
+            sent = torch.zeros((T,), dtype=torch.bool, device=hidden.device) if ge is None else ge.reshape(T) != 0
+            if g is not None and K > 0:
+                sent = sent | (g.reshape(T, K) != 0).any(dim=1)
+            sel = _nonzero_grad_rows(sent)
+            if sel is not None:
+                idx, pos, m = sel
+                if m == 0:
+                    return (
+                        (torch.zeros_like(embed) if need_dw else None), (torch.zeros_like(hidden) if need_dh else None), *none
+                    )
+                rows, entropy = _gather_rows(rows, idx), _gather(entropy.reshape(T), idx)
+                tokens = _gather(tokens, idx)
+                saved = torch.cat([_gather(saved[: T * K].view(T, K), idx).reshape(-1), _gather(saved[T * K :], idx)])
+                g = None if g is None else _gather(g.reshape(T, K), idx)
+                ge = None if ge is None else _gather(ge.reshape(T), idx)
         dh_dtype = torch.float32 if P > 1 and dh_reduce_f32 else torch.bfloat16
         dH, dW = ops.dist_backward(
-            embed, rows, tokens, softcap, zt, lse, entropy, g, ge, vocab_offset=off, vocab=vocab, need_dh=need_dh,
-            need_dw=need_dw, dh_dtype=dh_dtype, token_chunk=token_chunk,
+            embed, rows, tokens, softcap, saved, entropy, g, ge, vocab_offset=off, vocab=embed.shape[0] * P,
+            need_dh=need_dh, need_dw=need_dw, dh_dtype=dh_dtype, token_chunk=token_chunk,
         )
         if dH is not None:
             if P > 1:
                 with phase("dh_all_reduce"):
                     all_reduce_sum(dH, mesh)
             if pos is not None:
-                dH = ops.scatter_rows(dH, pos, torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device))
-            else:
+                dH = ops.scatter_rows(dH, pos, torch.empty((T, d), dtype=hidden.dtype, device=hidden.device))
+            elif dH.dtype != hidden.dtype:
                 dH = dH.to(hidden.dtype)
-        return (dW, dH) + none[2:]
+            if dH.shape != hidden.shape:
+                dH = dH.view(hidden.shape)
+        return dW, dH, *none
 
 
 # Autograd nodes of this operator's eager calls that are still alive, each with its leaves.
 _eager_graphs: weakref.WeakSet = weakref.WeakSet()
 
-# Rows without a gradient add nothing, and a backward of at least this much work (about 2 ms)
-# leaves them out; below it, finding them on the host costs more than computing them.
-_SKIP_MIN_FLOPS = 3e12
+# Rows without a gradient add nothing, and a backward of at least this much work (about 6 ms)
+# leaves them out. Below it, finding them on the host and gathering the others (0.15 ms) costs what a
+# tenth of the rows would; so do whole tiles of 256 rows that a few rows fewer do not save.
+_SKIP_MIN_FLOPS = 1e13
 
 
 def token_logps_and_entropy(
@@ -171,8 +186,7 @@ def token_logps_and_entropy(
         raise ValueError(f"at most {_lib.LP_DIST_MAX_TOKENS} tokens per position, got {K}")
     if mesh is not None and mesh.size > 1 and mesh.axis_names != ("d",):
         raise ValueError(f"vocab-parallel mesh needs axis 'd': {mesh.axis_names}")
-    n = math.prod(prefix)
-    leaves = [x for x in (embed_tokens, hidden) if torch.is_grad_enabled() and x.requires_grad and x.is_leaf]
+    leaves = [x for x in (embed_tokens, hidden) if x.requires_grad and x.is_leaf] if torch.is_grad_enabled() else []
     capturing = bool(leaves) and hidden.is_cuda and torch.cuda.is_current_stream_capturing()
     if capturing and any(ref() is x for node in _eager_graphs for ref in node.leaves for x in leaves):
         raise RuntimeError(
@@ -180,13 +194,13 @@ def token_logps_and_entropy(
             "before capturing this call"
         )
     logps, entropy = _TokenLogpsAndEntropy.apply(
-        embed_tokens, hidden.reshape(n, hidden.shape[-1]), _as_int32(tokens).reshape(n, K), softcap, mesh, token_chunk,
+        embed_tokens, hidden, _as_int32(tokens).view(math.prod(prefix), K), tuple(tokens.shape), softcap, mesh, token_chunk,
         dh_reduce_f32, skip_zero_grad,
     )
     if leaves and not capturing:
         logps.grad_fn.leaves = [weakref.ref(x) for x in leaves]
         _eager_graphs.add(logps.grad_fn)
-    return logps.reshape(tokens.shape), entropy.reshape(prefix)
+    return logps, entropy
 
 
 def top_token_logps(
@@ -209,16 +223,17 @@ def top_token_logps(
     if not 1 <= k <= min(_lib.LP_TOP_MAX, embed_tokens.shape[0]):
         raise ValueError(f"k must be between 1 and min({_lib.LP_TOP_MAX}, {embed_tokens.shape[0]}), got {k}")
     prefix = tuple(hidden.shape[:-1])
-    n = math.prod(prefix)
-    flat = None
+    token_logps = None
     if tokens is not None:
         if tuple(tokens.shape) != prefix:
             raise ValueError(f"hidden prefix {prefix} does not match tokens {tuple(tokens.shape)}")
-        flat = _as_int32(tokens).reshape(n)
-    ids, logps, entropy, token_logps = ops.top(
-        embed_tokens.detach(), hidden.detach().reshape(n, hidden.shape[-1]), softcap, int(k), flat
-    )
-    return TopTokenLogps(
-        ids.reshape(*prefix, k), logps.reshape(*prefix, k), entropy.reshape(prefix),
-        None if token_logps is None else token_logps.reshape(prefix),
-    )
+        tokens = _as_int32(tokens)
+        token_logps = torch.empty(prefix, dtype=torch.float32, device=hidden.device)
+    k = int(k)
+    ids = torch.empty((*prefix, k), dtype=torch.int32, device=hidden.device)
+    logps = torch.empty((*prefix, k), dtype=torch.float32, device=hidden.device)
+    entropy = torch.empty(prefix, dtype=torch.float32, device=hidden.device)
+    with torch.no_grad():
+        rows = hidden if hidden.ndim == 2 else hidden.reshape(math.prod(prefix), hidden.shape[-1])
+        ops.top(embed_tokens, rows, softcap, k, tokens, ids, logps, entropy, token_logps)
+    return TopTokenLogps(ids, logps, entropy, token_logps)

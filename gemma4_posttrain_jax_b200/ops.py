@@ -199,59 +199,97 @@ def _check_head(embed: torch.Tensor, hidden: torch.Tensor, *others: torch.Tensor
     return dev
 
 
+def _addr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _on_device(dev: torch.device, what: str, call) -> None:
+    """``call(stream)`` with ``dev`` current, and its return code checked."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if dev.index == torch.cuda.current_device():
+        rc = call(stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = call(stream)
+    _lib.check(rc, what)
+
+
 def dist_forward(
     embed: torch.Tensor,
     hidden: torch.Tensor,
     tokens: torch.Tensor,
     softcap: float | None,
-    *,
-    vocab_offset: int = 0,
-    shard: bool = False,
-) -> tuple[torch.Tensor, ...]:
-    """``lp_dist_fwd`` for int32 ``tokens`` [T, K]: (logp [T, K], entropy [T], zt [T, K], lse [T]),
-    or for one ``shard`` of the vocabulary (stats [3, T], zt [T, K])."""
+    logp: torch.Tensor,
+    entropy: torch.Tensor,
+) -> torch.Tensor:
+    """``lp_dist_fwd`` for int32 ``tokens`` [T, K] into f32 ``logp`` (T * K) and ``entropy`` (T). Returns
+    what the backward needs, f32 [T * K + T]: the tokens' logits, then the rows' log-normalisers."""
     dev = _check_head(embed, hidden, tokens)
     lib = _lib.load()
     T, K = tokens.shape
-    zt = torch.empty((T, K), dtype=torch.float32, device=dev)
-    stats = logp = row = None
-    if shard:
-        stats = torch.empty((3, T), dtype=torch.float32, device=dev)
-    else:
-        logp = torch.empty((T, K), dtype=torch.float32, device=dev)
-        row = torch.empty((2, T), dtype=torch.float32, device=dev)
+    saved = torch.empty((T * K + T,), dtype=torch.float32, device=dev)
     if T > 0:
         h, ldh = _dense_rows(hidden)
         w = _dense_embed(embed)
-        with torch.cuda.device(dev):
-            ws, wsp, wsn = _workspace(lib.lp_dist_fwd_workspace_bytes(T, w.shape[0]), dev)
-            rc = lib.lp_dist_fwd(
-                _stream(dev), _ptr(h), T, h.shape[1], ldh, _ptr(w), w.shape[0], int(vocab_offset), _ptr(tokens), K,
-                float(softcap or 0.0), _ptr(stats), _ptr(zt), _ptr(row) if row is None else _ptr(row[0]),
-                None if row is None else _ptr(row[1]), _ptr(logp), wsp, wsn,
+        V, d = w.shape
+
+        def call(stream):
+            ws, wsp, wsn = _workspace(lib.lp_dist_fwd_workspace_bytes(T, V), dev)
+            zt = saved.data_ptr()
+            return lib.lp_dist_fwd(
+                stream, h.data_ptr(), T, d, ldh, w.data_ptr(), V, 0, tokens.data_ptr(), K, softcap or 0.0, None, zt,
+                zt + 4 * T * K, entropy.data_ptr(), logp.data_ptr(), wsp, wsn,
             )
-        _lib.check(rc, "lp_dist_fwd")
-    return (stats, zt) if shard else (logp, row[1], zt, row[0])
+
+        _on_device(dev, "lp_dist_fwd", call)
+    return saved
+
+
+def dist_forward_shard(
+    embed: torch.Tensor, hidden: torch.Tensor, tokens: torch.Tensor, softcap: float | None, vocab_offset: int
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``lp_dist_fwd`` over one shard of the vocabulary: (stats [3, T], zt [T, K]) for ``dist_combine``."""
+    dev = _check_head(embed, hidden, tokens)
+    lib = _lib.load()
+    T, K = tokens.shape
+    stats = torch.empty((3, T), dtype=torch.float32, device=dev)
+    zt = torch.empty((T, K), dtype=torch.float32, device=dev)
+    if T > 0:
+        h, ldh = _dense_rows(hidden)
+        w = _dense_embed(embed)
+
+        def call(stream):
+            ws, wsp, wsn = _workspace(lib.lp_dist_fwd_workspace_bytes(T, w.shape[0]), dev)
+            return lib.lp_dist_fwd(
+                stream, h.data_ptr(), T, h.shape[1], ldh, w.data_ptr(), w.shape[0], int(vocab_offset),
+                tokens.data_ptr(), K, softcap or 0.0, stats.data_ptr(), zt.data_ptr(), None, None, None, wsp, wsn,
+            )
+
+        _on_device(dev, "lp_dist_fwd", call)
+    return stats, zt
 
 
 def dist_combine(
-    shard_stats: torch.Tensor, shard_zt: torch.Tensor, tokens: torch.Tensor, vocab: int
-) -> tuple[torch.Tensor, ...]:
-    """``lp_dist_combine``: [P, 3, T] and [P, T, K] -> (logp [T, K], entropy [T], zt [T, K], lse [T])."""
+    shard_stats: torch.Tensor,
+    shard_zt: torch.Tensor,
+    tokens: torch.Tensor,
+    vocab: int,
+    logp: torch.Tensor,
+    entropy: torch.Tensor,
+) -> torch.Tensor:
+    """``lp_dist_combine``: [P, 3, T] and [P, T, K] into f32 ``logp`` (T * K) and ``entropy`` (T);
+    returns what ``dist_forward`` returns."""
     dev = _require_cuda(shard_stats, shard_zt, tokens)
     lib = _lib.load()
     T, K = tokens.shape
-    P = shard_stats.shape[0]
-    logp = torch.empty((T, K), dtype=torch.float32, device=dev)
-    zt = torch.empty((T, K), dtype=torch.float32, device=dev)
-    row = torch.empty((2, T), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.lp_dist_combine(
-            _stream(dev), _ptr(shard_stats.contiguous()), _ptr(shard_zt.contiguous()), P, T, K, int(vocab), _ptr(tokens),
-            _ptr(row[0]), _ptr(row[1]), _ptr(zt), _ptr(logp),
-        )
-    _lib.check(rc, "lp_dist_combine")
-    return logp, row[1], zt, row[0]
+    saved = torch.empty((T * K + T,), dtype=torch.float32, device=dev)
+    stats, parts = shard_stats.contiguous(), shard_zt.contiguous()
+    zt = saved.data_ptr()
+    _on_device(dev, "lp_dist_combine", lambda stream: lib.lp_dist_combine(
+        stream, stats.data_ptr(), parts.data_ptr(), stats.shape[0], T, K, int(vocab), tokens.data_ptr(), zt + 4 * T * K,
+        entropy.data_ptr(), zt, logp.data_ptr(),
+    ))
+    return saved
 
 
 def dist_backward(
@@ -259,8 +297,7 @@ def dist_backward(
     hidden: torch.Tensor,
     tokens: torch.Tensor,
     softcap: float | None,
-    zt: torch.Tensor,
-    lse: torch.Tensor,
+    saved: torch.Tensor,
     entropy: torch.Tensor,
     grad_logp: torch.Tensor | None,
     grad_entropy: torch.Tensor | None,
@@ -273,9 +310,10 @@ def dist_backward(
     dw_dtype: torch.dtype = torch.bfloat16,
     token_chunk: int | None = None,
 ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
-    """``lp_dist_bwd``: (dH [T, d], partial over this shard; dW [Vs, d]) of f32 ``grad_logp`` [T, K]
-    and ``grad_entropy`` [T] (either may be None). ``vocab`` is the whole vocabulary's size."""
-    dev = _check_head(embed, hidden, tokens, zt, lse, entropy, grad_logp, grad_entropy)
+    """``lp_dist_bwd``: (dH [T, d], partial over this shard; dW [Vs, d]) of contiguous f32 ``grad_logp``
+    (T * K) and ``grad_entropy`` (T), either of which may be None. ``saved`` is the forward's;
+    ``vocab`` is the whole vocabulary's size."""
+    dev = _check_head(embed, hidden, tokens, saved, entropy, grad_logp, grad_entropy)
     lib = _lib.load()
     T, K = tokens.shape
     Vs, d = embed.shape
@@ -294,39 +332,49 @@ def dist_backward(
     h, ldh = _dense_rows(hidden) if T > 0 else (hidden, d)
     w = _dense_embed(embed)
     chunk = int(token_chunk) if token_chunk else 0
-    with torch.cuda.device(dev):
+
+    def call(stream):
         ws, wsp, wsn = _workspace(lib.lp_dist_bwd_workspace_bytes(T, d, Vs, chunk, flags), dev)
-        rc = lib.lp_dist_bwd(
-            _stream(dev), _ptr(h), T, d, ldh, _ptr(w), Vs, int(vocab_offset), int(vocab) if vocab else Vs, _ptr(tokens), K,
-            float(softcap or 0.0), _ptr(zt), _ptr(lse), _ptr(entropy), _ptr(grad_logp), _ptr(grad_entropy), _ptr(dH), d,
-            _ptr(dW), flags, chunk, wsp, wsn,
+        zt = saved.data_ptr()
+        return lib.lp_dist_bwd(
+            stream, h.data_ptr(), T, d, ldh, w.data_ptr(), Vs, int(vocab_offset), int(vocab) if vocab else Vs,
+            tokens.data_ptr(), K, softcap or 0.0, zt, zt + 4 * T * K, entropy.data_ptr(), _addr(grad_logp),
+            _addr(grad_entropy), _addr(dH), d, _addr(dW), flags, chunk, wsp, wsn,
         )
-    _lib.check(rc, "lp_dist_bwd")
+
+    _on_device(dev, "lp_dist_bwd", call)
     return dH, dW
 
 
 def top(
-    embed: torch.Tensor, hidden: torch.Tensor, softcap: float | None, k: int, tokens: torch.Tensor | None = None
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor | None]:
-    """``lp_top``: (ids int32 [T, k], logps [T, k], entropy [T], logps of int32 ``tokens`` [T] or None)."""
+    embed: torch.Tensor,
+    hidden: torch.Tensor,
+    softcap: float | None,
+    k: int,
+    tokens: torch.Tensor | None,
+    ids: torch.Tensor,
+    logps: torch.Tensor,
+    entropy: torch.Tensor,
+    token_logps: torch.Tensor | None,
+) -> None:
+    """``lp_top`` of hidden [T, d] into int32 ``ids`` and f32 ``logps`` (T * k), f32 ``entropy`` (T) and,
+    with int32 ``tokens`` (T), their ``token_logps`` (T)."""
     dev = _check_head(embed, hidden, tokens)
     lib = _lib.load()
     T, V = hidden.shape[0], embed.shape[0]
-    ids = torch.empty((T, k), dtype=torch.int32, device=dev)
-    logps = torch.empty((T, k), dtype=torch.float32, device=dev)
-    entropy = torch.empty((T,), dtype=torch.float32, device=dev)
-    token_logps = torch.empty((T,), dtype=torch.float32, device=dev) if tokens is not None else None
-    if T > 0:
-        h, ldh = _dense_rows(hidden)
-        w = _dense_embed(embed)
-        with torch.cuda.device(dev):
-            ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(T, V, int(k)), dev)
-            rc = lib.lp_top(
-                _stream(dev), _ptr(h), T, h.shape[1], ldh, _ptr(w), V, float(softcap or 0.0), int(k), _ptr(tokens),
-                _ptr(ids), _ptr(logps), _ptr(entropy), _ptr(token_logps), wsp, wsn,
-            )
-        _lib.check(rc, "lp_top")
-    return ids, logps, entropy, token_logps
+    if T == 0:
+        return
+    h, ldh = _dense_rows(hidden)
+    w = _dense_embed(embed)
+
+    def call(stream):
+        ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(T, V, k), dev)
+        return lib.lp_top(
+            stream, h.data_ptr(), T, h.shape[1], ldh, w.data_ptr(), V, softcap or 0.0, k, _addr(tokens), ids.data_ptr(),
+            logps.data_ptr(), entropy.data_ptr(), _addr(token_logps), wsp, wsn,
+        )
+
+    _on_device(dev, "lp_top", call)
 
 
 def sample_top_k(
@@ -345,16 +393,19 @@ def sample_top_k(
     B, V = hidden.shape[0], embed.shape[0]
     token = torch.empty((B,), dtype=torch.int32, device=dev)
     logp = torch.empty((B,), dtype=torch.float32, device=dev)
-    if B > 0:
-        h, ldh = _dense_rows(hidden)
-        w = _dense_embed(embed)
-        with torch.cuda.device(dev):
-            ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(B, V, int(top_k)), dev)
-            rc = lib.lp_sample_top_k(
-                _stream(dev), _ptr(h), B, h.shape[1], ldh, _ptr(w), V, float(softcap or 0.0), int(top_k), _ptr(uniform),
-                float(temperature), float(top_p), _ptr(token), _ptr(logp), wsp, wsn,
-            )
-        _lib.check(rc, "lp_sample_top_k")
+    if B == 0:
+        return token, logp
+    h, ldh = _dense_rows(hidden)
+    w = _dense_embed(embed)
+
+    def call(stream):
+        ws, wsp, wsn = _workspace(lib.lp_top_workspace_bytes(B, V, top_k), dev)
+        return lib.lp_sample_top_k(
+            stream, h.data_ptr(), B, h.shape[1], ldh, w.data_ptr(), V, softcap or 0.0, top_k, uniform.data_ptr(),
+            temperature, top_p, token.data_ptr(), logp.data_ptr(), wsp, wsn,
+        )
+
+    _on_device(dev, "lp_sample_top_k", call)
     return token, logp
 
 

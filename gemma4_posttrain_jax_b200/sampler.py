@@ -125,7 +125,8 @@ def sample_top_k(
         raise ValueError("top_p must be in (0, 1]")
     if tuple(uniform.shape) != (hidden.shape[0],) or uniform.dtype != torch.float32:
         raise ValueError(f"uniform must be float32 [{hidden.shape[0]}], got {uniform.dtype} {tuple(uniform.shape)}")
-    return ops.sample_top_k(
-        embed_tokens.detach(), hidden.detach(), softcap, uniform.contiguous(), temperature=float(temperature),
-        top_k=int(top_k), top_p=float(top_p),
-    )
+    with torch.no_grad():
+        return ops.sample_top_k(
+            embed_tokens, hidden, softcap, uniform.contiguous(), temperature=float(temperature), top_k=int(top_k),
+            top_p=float(top_p),
+        )

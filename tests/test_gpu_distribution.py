@@ -169,15 +169,16 @@ def test_shards_merge_to_the_whole(cuda_device, V, P):
     ref = Reference(W, H, 30.0)
     vs = V // P
     shards = [W[p * vs : (p + 1) * vs] for p in range(P)]
-    parts = [ops.dist_forward(w, H, y, 30.0, vocab_offset=p * vs, shard=True) for p, w in enumerate(shards)]
-    logp, entropy, zt, lse = ops.dist_combine(
-        torch.stack([s for s, _ in parts]), torch.stack([z for _, z in parts]), y, V
+    parts = [ops.dist_forward_shard(w, H, y, 30.0, p * vs) for p, w in enumerate(shards)]
+    logp, entropy = torch.empty((T, K), device=cuda_device), torch.empty((T,), device=cuda_device)
+    saved = ops.dist_combine(
+        torch.stack([s for s, _ in parts]), torch.stack([z for _, z in parts]), y, V, logp, entropy
     )
     picked = ref.picked(y)
     within(logp, picked, ref.logp_bound(picked), "logps")
     within(entropy, ref.entropy, ref.entropy_bound(), "entropy")
     grads = [
-        ops.dist_backward(w, H, y, 30.0, zt, lse, entropy, g, ge, vocab_offset=p * vs, vocab=V, dh_dtype=torch.float32)
+        ops.dist_backward(w, H, y, 30.0, saved, entropy, g, ge, vocab_offset=p * vs, vocab=V, dh_dtype=torch.float32)
         for p, w in enumerate(shards)
     ]
     dH, dW, bH, bW = ref.grads(y, g, ge)
