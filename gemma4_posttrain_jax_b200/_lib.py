@@ -75,16 +75,17 @@ _SIG = {
         [_P, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, _P, _I64, ctypes.c_int, _P, _P, _P, _P, ctypes.c_size_t],
     ),
     "lp_dist_fwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "lp_dist_kept_bytes": (ctypes.c_size_t, [_I64, _I64]),
     "lp_dist_fwd": (
         ctypes.c_int,
-        [_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, ctypes.c_float, _P, _P, _P, _P, _P, _P, ctypes.c_size_t],
+        [_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, ctypes.c_float, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t],
     ),
     "lp_dist_combine": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
     "lp_dist_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, ctypes.c_int]),
     "lp_dist_bwd": (
         ctypes.c_int,
-        [_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, _P, _P, _P, _P, _P, _P, _I64, _P,
-         ctypes.c_int, _I64, _P, ctypes.c_size_t],
+        [_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, _P, _P, _P, _P, _P, _P, _I64, _P, _P,
+         _I64, _P, ctypes.c_int, _I64, _P, ctypes.c_size_t],
     ),
     "lp_top_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, ctypes.c_int]),
     "lp_top": (

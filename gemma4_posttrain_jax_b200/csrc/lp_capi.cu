@@ -857,7 +857,25 @@ struct DistGrad {
   int K;
   int64_t V;  // the whole vocabulary
   const float *zt, *lse, *entropy, *g, *ge;
+  const void* kept;       // kept logits (dist_kept_layout of kept_rows rows), or null: recomputed
+  int64_t kept_rows;
+  const int32_t* row_of;  // row of the kept logits of each row, or null: the row itself
 };
+
+// Kept logits: 16 bits each [rows, ld] (16-byte rows), then the largest of every 32 columns
+// [rows, ld_max] in f32.
+struct KeptLayout {
+  int64_t ld, ld_max;
+  size_t max_off, total;
+};
+KeptLayout dist_kept_layout(int64_t rows, int64_t Vs) {
+  KeptLayout K;
+  K.ld = (Vs + 7) / 8 * 8;
+  K.ld_max = cdiv(Vs, BN) * (BN / 32);
+  K.max_off = align_up((size_t)rows * K.ld * 2, 256);
+  K.total = K.max_off + (size_t)rows * K.ld_max * sizeof(float);
+  return K;
+}
 
 // Plan and scratch of lp_dist_bwd: the work counters of every GEMM launch (three per chunk) and the
 // row constants, before the layout of lp_bwd. In the workspace, not in the library's rotating
@@ -946,8 +964,8 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
     const int64_t tcur = std::min<int64_t>(L.tc, T - t0);
     const __nv_bfloat16* Hc = Hb + t0 * ldh;
 
-    // 1) recompute logits tile by tile and write dZ (bf16) for this chunk
-    {
+    // 1) recompute logits tile by tile and write dZ (bf16) for this chunk (or take kept logits)
+    if (dist == nullptr || dist->kept == nullptr) {
       alignas(64) CUtensorMap ta, tb, to;
       if ((rc = map_bf16(&ta, Hc, d, tcur, ldh, BK, 128, "hidden chunk"))) return rc;
       if ((rc = map_bf16(&tb, W, d, Vs, d, BK, b_box_rows(cg_dz), "embedding"))) return rc;
@@ -971,14 +989,6 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
         }
         p.sched = counters++;
         if ((rc = launch_gemm_cap<EPI_DIST_DZ, false, false>(cap, st, ta, tb, to, p, di, "dist_dz_gemm"))) return rc;
-        const int64_t slots = row_const != nullptr ? tcur * dist->K : 0;
-        if (slots > 0) {
-          ProfScope prof(st, "dist_dz_targets");
-          dist_dz_targets_kernel<<<(unsigned)cdiv(slots, 256), 256, 0, st>>>(
-              y + t0 * dist->K, dist->zt + t0 * dist->K, dist->g != nullptr ? dist->g + t0 * dist->K : nullptr,
-              row_const + t0, T, (int)tcur, dist->K, v_off, Vs, softcap, dz, L.ldz);
-          LP_LAUNCH_CHECK("dist_dz_targets_kernel");
-        }
       } else {
         p.e.y = y + t0;
         p.e.v_off = v_off;
@@ -987,6 +997,62 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
         p.e.stats_ld = T;
         if ((rc = launch_gemm_cap<EPI_BWD_DZ, false, false>(cap, st, ta, tb, to, p, di, "bwd_dz_gemm"))) return rc;
       }
+    }
+    if (dist != nullptr && dist->kept != nullptr) {
+      const KeptLayout K = dist_kept_layout(dist->kept_rows, Vs);
+      DistDzParams z{};
+      // without row_of the kept rows are this call's rows
+      const int64_t first = dist->row_of != nullptr ? 0 : t0;
+      z.kept = reinterpret_cast<const uint16_t*>(dist->kept) + first * K.ld;
+      z.kept_max = reinterpret_cast<const float*>(reinterpret_cast<const char*>(dist->kept) + K.max_off) + first * K.ld_max;
+      z.row_of = dist->row_of != nullptr ? dist->row_of + t0 : nullptr;
+      z.ldk = K.ld;
+      z.ld_max = K.ld_max;
+      if (row_const != nullptr) {
+        z.row_const = row_const + t0;
+        z.row_ld = T;
+      } else {
+        z.y = y + t0;
+        z.g = dist->g != nullptr ? dist->g + t0 : nullptr;
+        z.ge = dist->ge != nullptr ? dist->ge + t0 : nullptr;
+        z.lse = dist->lse + t0;
+        z.entropy = dist->entropy + t0;
+      }
+      z.vocab = dist->V;
+      z.v_off = v_off;
+      z.Vs = Vs;
+      z.cap = softcap;
+      z.dz = dz;
+      z.ldz = L.ldz;
+      ProfScope prof(st, "dist_dz");
+      for (int64_t r = 0; r < tcur; r += 32768) {  // a grid has at most 65535 rows
+        const int64_t rows = std::min<int64_t>(32768, tcur - r);
+        DistDzParams zr = z;
+        if (z.row_of != nullptr) zr.row_of = z.row_of + r;
+        else {
+          zr.kept = z.kept + r * K.ld;
+          zr.kept_max = z.kept_max + r * K.ld_max;
+        }
+        if (row_const != nullptr) zr.row_const = z.row_const + r;
+        else {
+          zr.y = z.y + r;
+          zr.g = z.g != nullptr ? z.g + r : nullptr;
+          zr.ge = z.ge != nullptr ? z.ge + r : nullptr;
+          zr.lse = z.lse + r;
+          zr.entropy = z.entropy + r;
+        }
+        zr.dz = z.dz + r * L.ldz;
+        dist_dz_kernel<<<dim3((unsigned)cdiv(Vs, kDzCols), (unsigned)rows), 256, 0, st>>>(zr);
+        LP_LAUNCH_CHECK("dist_dz_kernel");
+      }
+    }
+    if (dist != nullptr && row_const != nullptr && dist->K > 0) {
+      // the given tokens' entries
+      ProfScope prof(st, "dist_dz_targets");
+      dist_dz_targets_kernel<<<(unsigned)cdiv(tcur * dist->K, 256), 256, 0, st>>>(
+          y + t0 * dist->K, dist->zt + t0 * dist->K, dist->g != nullptr ? dist->g + t0 * dist->K : nullptr,
+          row_const + t0, T, (int)tcur, dist->K, v_off, Vs, softcap, dz, L.ldz);
+      LP_LAUNCH_CHECK("dist_dz_targets_kernel");
     }
     // 2) dH[t0:t0+tcur] = dZ . W
     if (want_dh) {
@@ -1449,9 +1515,13 @@ size_t lp_dist_fwd_workspace_bytes(int64_t T, int64_t Vs) {
   return dist_fwd_layout(T, Vs, 64, have ? di : nullptr, 148, 0).total;
 }
 
+size_t lp_dist_kept_bytes(int64_t T, int64_t Vs) {
+  return T > 0 && Vs > 0 ? dist_kept_layout(T, Vs).total : 0;
+}
+
 int lp_dist_fwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs,
                 int64_t v_off, const int32_t* y, int64_t K, float softcap, float* stats, float* zt, float* lse,
-                float* entropy, float* logp, void* workspace, size_t workspace_bytes) {
+                float* entropy, float* logp, void* kept, void* workspace, size_t workspace_bytes) {
   int rc = check_dist(H, T, d, ldh, W, Vs, y, K);
   if (rc) return rc;
   if (T == 0) return LP_OK;
@@ -1474,7 +1544,16 @@ int lp_dist_fwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, 
   p.e.part = reinterpret_cast<float2*>(ws + L.part_off);
   p.e.part_a = reinterpret_cast<float*>(ws + L.part_a_off);
   dist_hints(p);
-  if ((rc = launch_gemm_cap<EPI_DIST, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "dist_fwd_gemm"))) return rc;
+  if (kept != nullptr) {
+    const KeptLayout KL = dist_kept_layout(T, Vs);
+    alignas(64) CUtensorMap to;
+    if ((rc = map_store_bf16(&to, kept, Vs, T, KL.ld, "kept logits"))) return rc;  // 16-bit elements
+    p.e.keep_max = reinterpret_cast<float*>(reinterpret_cast<char*>(kept) + KL.max_off);
+    rc = launch_gemm_cap<EPI_DIST_KEEP, false, false>(softcap > 0.f, st, ta, tb, to, p, di, "dist_fwd_gemm");
+  } else {
+    rc = launch_gemm_cap<EPI_DIST, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "dist_fwd_gemm");
+  }
+  if (rc) return rc;
   ProfScope prof(st, "dist_finalize");
   const __nv_bfloat16* Hb = reinterpret_cast<const __nv_bfloat16*>(H);
   const __nv_bfloat16* Wb = reinterpret_cast<const __nv_bfloat16*>(W);
@@ -1522,15 +1601,18 @@ size_t lp_dist_bwd_workspace_bytes(int64_t T, int64_t d, int64_t Vs, int64_t tok
 
 int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs,
                 int64_t v_off, int64_t V, const int32_t* y, int64_t K, float softcap, const float* zt, const float* lse,
-                const float* entropy, const float* g_logp, const float* g_entropy, void* dH, int64_t ld_dh, void* dW,
-                int flags, int64_t token_chunk, void* workspace, size_t workspace_bytes) {
+                const float* entropy, const float* g_logp, const float* g_entropy, const void* kept, int64_t kept_rows,
+                const int32_t* row_of, void* dH, int64_t ld_dh, void* dW, int flags, int64_t token_chunk,
+                void* workspace, size_t workspace_bytes) {
   if (int rc = check_dist(H, T, d, ldh, W, Vs, y, K)) return rc;
   if (v_off < 0 || v_off + Vs > V) return fail(LP_EINVAL, "shard [%lld, %lld) outside the vocabulary of %lld",
                                                (long long)v_off, (long long)(v_off + Vs), (long long)V);
   if (T > 0 && (lse == nullptr || entropy == nullptr || (K > 0 && zt == nullptr)))
     return fail(LP_EINVAL, "null lse, entropy or zt");
   static const int32_t none = 0;
-  const DistGrad dg{(int)K, V, zt, lse, entropy, K > 0 ? g_logp : nullptr, g_entropy};
+  if (kept != nullptr && ((reinterpret_cast<uintptr_t>(kept) & 15) != 0 || kept_rows < (row_of != nullptr ? 1 : T)))
+    return fail(LP_EINVAL, "kept logits must be 16-byte aligned and have a row for each row");
+  const DistGrad dg{(int)K, V, zt, lse, entropy, K > 0 ? g_logp : nullptr, g_entropy, kept, kept_rows, row_of};
   return bwd_impl(stream, H, T, d, ldh, W, Vs, v_off, K > 0 ? y : &none, softcap, nullptr, nullptr, dH, ld_dh, dW, flags,
                   token_chunk, workspace, workspace_bytes, nullptr, &dg);
 }

@@ -256,6 +256,88 @@ __global__ void dist_row_const_kernel(const float* __restrict__ lse, const float
   row_const[(size_t)2 * T + t] = lse[t] * kLog2e;
 }
 
+// dZ of a chunk from kept logits (EPI_DIST_KEEP) instead of a recomputed product: reads 2 bytes and
+// writes 2 per entry, where the recompute costs 2 d flops. The same formula as EPI_DIST_DZ's; with one
+// token per row its entry is in it, too. One block per row and 8192 columns, eight columns (16 bytes)
+// per thread and step. Bound by HBM: 4 T Vs bytes.
+struct DistDzParams {
+  const uint16_t* kept;   // [rows, ldk]
+  const float* kept_max;  // [rows, ld_max]
+  const int32_t* row_of;  // [T] row of the kept logits, or null: the row itself
+  long long ldk, ld_max;
+  const float* row_const;  // [3][row_ld], or null: one token per row and the pointers below
+  long long row_ld;
+  const int32_t* y;
+  const float *g, *ge, *lse, *entropy;
+  long long vocab, v_off, Vs;
+  float cap;
+  __nv_bfloat16* dz;
+  long long ldz;
+};
+constexpr int kDzCols = 8192;
+
+__global__ void __launch_bounds__(256) dist_dz_kernel(const DistDzParams P) {
+  const int t = blockIdx.y;
+  float a, b, l2, gv = 0.f;
+  long long yl = -1;
+  if (P.row_const != nullptr) {
+    a = P.row_const[t];
+    b = P.row_const[P.row_ld + t];
+    l2 = P.row_const[2 * P.row_ld + t];
+  } else {
+    const long long v = P.y[t];
+    if (P.g != nullptr && v >= 0 && v < P.vocab) {
+      gv = P.g[t];
+      yl = v - P.v_off;
+    }
+    const float e = P.ge != nullptr ? P.ge[t] : 0.f;
+    a = e != 0.f ? fmaf(e, P.entropy[t], gv) : gv;
+    b = e * kLn2;
+    l2 = P.lse[t] * kLog2e;
+  }
+  const long long from = P.row_of != nullptr ? P.row_of[t] : t;
+  const uint16_t* kept = P.kept + from * P.ldk;
+  const float* kept_max = P.kept_max + from * P.ld_max;
+  __nv_bfloat16* dz = P.dz + (size_t)t * P.ldz;
+  const float ucap = P.cap > 0.f ? kLn2 / P.cap : 0.f;  // z2 -> tanh(x / c)
+  const long long c0 = (long long)blockIdx.x * kDzCols + threadIdx.x * 8;
+  uint4 q[kDzCols / 2048];
+  float mx[kDzCols / 2048];
+#pragma unroll
+  for (int i = 0; i < kDzCols / 2048; ++i) {
+    const long long col = c0 + i * 2048;
+    if (col < P.Vs) {
+      q[i] = __ldcs(reinterpret_cast<const uint4*>(kept + col));
+      mx[i] = __ldg(kept_max + col / 32);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kDzCols / 2048; ++i) {
+    const long long col = c0 + i * 2048;
+    if (col >= P.Vs) break;
+    const float top = mx[i] - l2;  // log2 p of the largest of the 32
+    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+    uint32_t out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float v[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        // 2^23 + n, whose low bits are n, less 2^23
+        const float n = __uint_as_float(k == 0 ? (w[j] & 0xffffu) | 0x4b000000u : (w[j] >> 16) | 0x4b000000u) - 8388608.f;
+        const float lp = fmaf(n, -kKeepRange / 65535.f, top);
+        const float u = (lp + l2) * ucap;
+        float x = -fast_ex2(lp) * fmaf(b, lp, a);
+        if (col + 2 * j + k == yl) x += gv;
+        v[k] = fmaf(-u, u, 1.f) * x;
+      }
+      out[j] = pack_bf16x2(v[0], v[1]);
+    }
+    // rows of dZ are padded to 16 bytes
+    *reinterpret_cast<uint4*>(dz + col) = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+
 // The given tokens' entries of a chunk's dZ, computed from their f32 logits and rounded once:
 //   dZ[t, y] = softcap'(z) * (sum of g over the row's slots that hold y - p * (a + b log2 p))
 // softcap'(z) = 1 - (z / c)^2. The first slot of a token writes the entry, so a token that a row

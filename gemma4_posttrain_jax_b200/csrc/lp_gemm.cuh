@@ -35,6 +35,7 @@
 //   EPI_DIST    : softcap + running (max m, S = sum 2^(z-m), A = sum 2^(z-m) (z-m)) per row in
 //                 base 2, from which the log-normaliser and the entropy follow.
 //   EPI_DIST_LOGITS : EPI_DIST, with the accumulator stored as f32.
+//   EPI_DIST_KEEP : EPI_DIST, with the logits kept in 16 bits (keep_logits).
 //   EPI_DIST_TOP32, EPI_DIST_TOP8 : EPI_DIST, with the two largest of every 32 (8) accumulator
 //                 columns, the first's column in its low bits.
 //   EPI_DIST_DZ : recompute path of log-probabilities and entropy:
@@ -97,7 +98,8 @@ enum : int {
   EPI_DIST_LOGITS = 5,
   EPI_DIST_DZ = 6,
   EPI_DIST_TOP32 = 7,
-  EPI_DIST_TOP8 = 8
+  EPI_DIST_TOP8 = 8,
+  EPI_DIST_KEEP = 9
 };
 
 // Columns per selection key of an epilogue (0: none).
@@ -168,6 +170,7 @@ struct EpiParams {
   float2* best;          // HEAD: [n_groups][M] (largest logit, its column as int bits)
   int store_logits;      // HEAD: store the logits through tmO (else only the row statistics)
   float* part_a;         // DIST: [n_groups][M] running A (part holds the running max and S)
+  float* keep_max;       // DIST_KEEP: [M][8 * tiles_n] largest logit of every 32 columns (base 2)
   float* top;            // DIST_TOP: [2][M][BN / group * tiles_n] largest and second of each group
   const float* row_const;  // DIST_DZ: [3][row_ld] per row: a, b, log2 of the normaliser; or null,
   long long row_ld;        //          then one token per row: its y and g (above), the vocabulary's
@@ -317,6 +320,7 @@ static_assert(gemm_smem_bytes<1, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<1, 
                   gemm_smem_bytes<1, EPI_STORE>() <= 232448 && gemm_smem_bytes<1, EPI_HEAD>() <= 232448 &&
                   gemm_smem_bytes<2, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<2, EPI_BWD_DZ>() <= 232448 &&
                   gemm_smem_bytes<2, EPI_STORE>() <= 232448 && gemm_smem_bytes<2, EPI_HEAD>() <= 232448 &&
+                  gemm_smem_bytes<1, EPI_DIST_KEEP>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_KEEP>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST_TOP32>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_TOP32>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST_TOP8>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_TOP8>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST>() <= 232448 && gemm_smem_bytes<2, EPI_DIST>() <= 232448 &&
@@ -360,13 +364,11 @@ __device__ __forceinline__ void dist_rescale(float& m, float& s, float& a, float
   }
 }
 
-// Adds 32 accumulator columns of a row (the first nvalid of them unless FULL) to its running
-// (m, S, A). A's terms are all of one sign, so it keeps full relative accuracy however flat or
-// peaked the row is; log-normaliser - sum p z would cancel.
+// Base-2 logits of 32 accumulator columns of a row; returns the largest (of the first nvalid unless
+// FULL).
 template <bool HAS_CAP, bool FULL>
-__device__ __forceinline__ void dist_accumulate(const uint32_t (&r)[32], int nvalid, float k1, float c2, float xlog2e,
-                                                float& m, float& s, float& a) {
-  float z[32];
+__device__ __forceinline__ float dist_logits(const uint32_t (&r)[32], int nvalid, float k1, float c2, float xlog2e,
+                                             float (&z)[32]) {
   float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
@@ -376,7 +378,15 @@ __device__ __forceinline__ void dist_accumulate(const uint32_t (&r)[32], int nva
       if (j & 1) mx1 = fmaxf(mx1, z[j]); else mx0 = fmaxf(mx0, z[j]);
     }
   }
-  dist_rescale(m, s, a, fmaxf(mx0, mx1));
+  return fmaxf(mx0, mx1);
+}
+
+// Adds them to the row's running (m, S, A). A's terms are all of one sign, so it keeps full relative
+// accuracy however flat or peaked the row is; log-normaliser - sum p z would cancel.
+template <bool FULL>
+__device__ __forceinline__ void dist_accumulate(const float (&z)[32], int nvalid, float mx, float& m, float& s,
+                                                float& a) {
+  dist_rescale(m, s, a, mx);
   float s0 = 0.f, s1 = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
@@ -393,6 +403,22 @@ __device__ __forceinline__ void dist_accumulate(const uint32_t (&r)[32], int nva
   }
   s += s0 + s1;
   a += a0 + a1;
+}
+
+// Logits kept for the backward: 16 bits each, as the distance below the largest of their 32 columns
+// in steps of kKeepRange / 65535 (base 2), at most kKeepRange. A kept logit is off by at most
+// 3.7e-4 * ln2, so a probability by 2.5e-4 of itself, a fifteenth of what the bf16 rounding of dZ
+// that follows may add; what lies further below is kept at 2^-48 of the largest. The largest itself
+// is kept exactly (f32).
+constexpr float kKeepRange = 48.f;
+__device__ __forceinline__ void keep_logits(const float (&z)[32], float mx, uint32_t (&pk)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    // the low bits of 2^23 + n are n
+    const float lo = fmaf(fminf(mx - z[2 * j], kKeepRange), 65535.f / kKeepRange, 8388608.f);
+    const float hi = fmaf(fminf(mx - z[2 * j + 1], kKeepRange), 65535.f / kKeepRange, 8388608.f);
+    pk[j] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
+  }
 }
 
 // The two largest of every G of 32 accumulator columns. The order is that of x (softcap is
@@ -727,7 +753,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const EpiParams& E = P.e;
     const float cap = E.softcap;
     // x of the distribution epilogues, with the accumulator's truncation made up for (dist_scale)
-    constexpr bool kDist = EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || top_group<EPI>() > 0 || EPI == EPI_DIST_DZ;
+    constexpr bool kDist = EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || EPI == EPI_DIST_KEEP || top_group<EPI>() > 0 ||
+                           EPI == EPI_DIST_DZ;
     const float xs = kDist ? dist_scale(S.K) : 1.f;
     const float xlog2e = kDist ? xs * kLog2e : kLog2e;
     const float k1 = HAS_CAP ? 2.0f * xlog2e / cap : 0.f;  // x -> 2x/c in base 2
@@ -977,8 +1004,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               sb ^= 1;
             }
           }
-        } else if constexpr (EPI == EPI_DIST || top_group<EPI>() > 0) {
-          float4 k1st, k2nd;  // TOP32: this warp's four groups of the tile
+        } else if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_KEEP || top_group<EPI>() > 0) {
+          float4 k1st, k2nd;  // TOP32, KEEP: this warp's four 32-column groups of the tile
 #pragma unroll 1
           for (int c = 0; c < (row_base < S.M ? BN / 64 : 0); ++c) {
             uint32_t r[32];
@@ -988,12 +1015,44 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const int nvalid = S.N - (colh + c * 32);  // columns >= nvalid are vocabulary padding (warp-uniform)
             constexpr int G = top_group<EPI>();
             float2 key[G > 0 ? 32 / (G > 0 ? G : 1) : 1];
+            float z[32];
+            float mx = -INFINITY;
             if (nvalid >= 32) {
               if constexpr (G > 0) top_keys_of<G, true>(r, 32, key);
-              dist_accumulate<HAS_CAP, true>(r, 32, k1, c2, xlog2e, run_m, run_s, run_a);
+              mx = dist_logits<HAS_CAP, true>(r, 32, k1, c2, xlog2e, z);
+              dist_accumulate<true>(z, 32, mx, run_m, run_s, run_a);
             } else {
               if constexpr (G > 0) top_keys_of<G, false>(r, nvalid, key);
-              if (nvalid > 0) dist_accumulate<HAS_CAP, false>(r, nvalid, k1, c2, xlog2e, run_m, run_s, run_a);
+              if (nvalid > 0) {
+                mx = dist_logits<HAS_CAP, false>(r, nvalid, k1, c2, xlog2e, z);
+                dist_accumulate<false>(z, nvalid, mx, run_m, run_s, run_a);
+              }
+            }
+            if constexpr (EPI == EPI_DIST_KEEP) {
+              if (nvalid > 0) {
+                uint32_t pk[16];
+                keep_logits(z, mx, pk);
+                if (lane == 0) bulk_wait_read<1>();
+                __syncwarp();
+                uint8_t* buf_s = my_staging + sb * SBUF;
+                const uint32_t sbase = smem_u32(buf_s);
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4)
+                  st_shared_v4(sbase + sw64_offset(lane, i4), pk[4 * i4], pk[4 * i4 + 1], pk[4 * i4 + 2], pk[4 * i4 + 3]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  tma_store_2d(&tmO, buf_s, colh + c * 32, row_base);
+                  bulk_commit();
+                }
+                sb ^= 1;
+              }
+              k1st.x = c == 0 ? mx : k1st.x;
+              k1st.y = c == 1 ? mx : k1st.y;
+              k1st.z = c == 2 ? mx : k1st.z;
+              k1st.w = mx;
+              if (c == 3 && row_ok)
+                *reinterpret_cast<float4*>(E.keep_max + (size_t)row * (8 * S.tiles_n) + nt * 8 + h * 4) = k1st;
             }
             if constexpr (G > 0) {
               const int ld = BN / G * S.tiles_n;
@@ -1250,7 +1309,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // one (max, sum) partial per unit and column half
         if (row_ok) E.part[(size_t)(un.group * 2 + h) * S.M + row] = make_float2(run_m, run_s);
       }
-      if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || top_group<EPI>() > 0) {
+      if constexpr (EPI == EPI_DIST || EPI == EPI_DIST_LOGITS || EPI == EPI_DIST_KEEP || top_group<EPI>() > 0) {
         if (row_ok) {
           const size_t at = (size_t)(un.group * 2 + h) * S.M + row;
           E.part[at] = make_float2(run_m, run_s);

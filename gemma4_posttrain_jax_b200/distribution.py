@@ -57,16 +57,21 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
     here: outside, each would be a node of the autograd graph of its own."""
 
     @staticmethod
-    def forward(ctx, embed, hidden, tokens, shape, softcap, mesh, token_chunk, dh_reduce_f32, skip_zero_grad):
+    def forward(ctx, embed, hidden, tokens, shape, softcap, mesh, token_chunk, dh_reduce_f32, skip_zero_grad, keep_logits):
         T, K = tokens.shape
         h = hidden.reshape(T, hidden.shape[-1])
         logp = torch.empty(shape, dtype=torch.float32, device=hidden.device)
         entropy = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=hidden.device)
+        kept = None
+        if (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]) and keep_logits is not False:
+            nbytes = ops.dist_kept_bytes(T, embed.shape[0])
+            if keep_logits or nbytes <= _KEPT_MAX_BYTES:
+                kept = torch.empty((nbytes,), dtype=torch.uint8, device=hidden.device)
         P = mesh.size if mesh is not None else 1
         off = 0
         if P > 1:
             off = vocab_offset(embed.shape[0], mesh)
-            stats, zt = ops.dist_forward_shard(embed, h, tokens, softcap, off)
+            stats, zt = ops.dist_forward_shard(embed, h, tokens, softcap, off, kept)
             with phase("stats_all_gather"):
                 both = all_gather_stats(torch.cat([stats.reshape(-1), zt.reshape(-1)]), mesh)
             saved = ops.dist_combine(
@@ -74,8 +79,8 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
                 entropy,
             )
         else:
-            saved = ops.dist_forward(embed, h, tokens, softcap, logp, entropy)
-        ctx.save_for_backward(embed, hidden, tokens, saved, entropy)
+            saved = ops.dist_forward(embed, h, tokens, softcap, logp, entropy, kept)
+        ctx.save_for_backward(embed, hidden, tokens, saved, entropy, kept)
         ctx.meta = (softcap, mesh, P, off, token_chunk, dh_reduce_f32, skip_zero_grad)
         ctx.set_materialize_grads(False)
         return logp, entropy
@@ -84,10 +89,10 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g, ge):
         need_dw, need_dh = ctx.needs_input_grad[:2]
-        none = (None,) * 7
+        none = (None,) * 8
         if (g is None and ge is None) or not (need_dw or need_dh):
             return None, None, *none
-        embed, hidden, tokens, saved, entropy = ctx.saved_tensors
+        embed, hidden, tokens, saved, entropy, kept = ctx.saved_tensors
         softcap, mesh, P, off, token_chunk, dh_reduce_f32, skip_zero_grad = ctx.meta
         T, K = tokens.shape
         d = hidden.shape[-1]
@@ -96,7 +101,7 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
         g = None if g is None else g.contiguous()
         ge = None if ge is None else ge.contiguous()
         rows = hidden.reshape(T, d)
-        pos = None
+        pos = row_of = None
         if (
             skip_zero_grad
             and 6.0 * T * d * embed.shape[0] >= _SKIP_MIN_FLOPS
@@ -112,6 +117,7 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
                     return (
                         (torch.zeros_like(embed) if need_dw else None), (torch.zeros_like(hidden) if need_dh else None), *none
                     )
+                row_of = idx
                 rows, entropy = _gather_rows(rows, idx), _gather(entropy.reshape(T), idx)
                 tokens = _gather(tokens, idx)
                 saved = torch.cat([_gather(saved[: T * K].view(T, K), idx).reshape(-1), _gather(saved[T * K :], idx)])
@@ -119,8 +125,8 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
                 ge = None if ge is None else _gather(ge.reshape(T), idx)
         dh_dtype = torch.float32 if P > 1 and dh_reduce_f32 else torch.bfloat16
         dH, dW = ops.dist_backward(
-            embed, rows, tokens, softcap, saved, entropy, g, ge, vocab_offset=off, vocab=embed.shape[0] * P,
-            need_dh=need_dh, need_dw=need_dw, dh_dtype=dh_dtype, token_chunk=token_chunk,
+            embed, rows, tokens, softcap, saved, entropy, g, ge, kept=kept, kept_rows=T, row_of=row_of, vocab_offset=off,
+            vocab=embed.shape[0] * P, need_dh=need_dh, need_dw=need_dw, dh_dtype=dh_dtype, token_chunk=token_chunk,
         )
         if dH is not None:
             if P > 1:
@@ -137,6 +143,10 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
 
 # Autograd nodes of this operator's eager calls that are still alive, each with its leaves.
 _eager_graphs: weakref.WeakSet = weakref.WeakSet()
+
+# Logits are kept for the backward up to this many bytes (8064 rows of a vocabulary of 262144), the
+# size of the backward's own dZ scratch.
+_KEPT_MAX_BYTES = 4 << 30
 
 # Rows without a gradient add nothing, and a backward of at least this much work (about 6 ms)
 # leaves them out. Below it, finding them on the host and gathering the others (0.15 ms) costs what a
@@ -155,6 +165,7 @@ def token_logps_and_entropy(
     token_chunk: int | None = None,
     dh_reduce_f32: bool = False,
     skip_zero_grad: bool = True,
+    keep_logits: bool | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Log-probabilities of given tokens and the entropy of every position's distribution.
 
@@ -163,6 +174,10 @@ def token_logps_and_entropy(
     differentiable in ``embed_tokens`` and ``hidden``. An id outside the vocabulary (-1, say) is no
     token: its logp is 0 and sends no gradient, so lists of different lengths can be padded. A token
     named twice in a row counts twice.
+
+    A differentiable call keeps the logits in 16 bits each for its backward when they take at most
+    4 GiB, and recomputes them there otherwise; ``keep_logits`` says so either way. (A kept logit is
+    within 2.6e-4 of its value, which moves the gradients by a fifteenth of their bf16 rounding.)
 
     ``mesh``, ``token_chunk``, ``dh_reduce_f32`` and ``skip_zero_grad`` are those of
     ``per_token_logps``; over a mesh the shards' statistics are exchanged by one all-gather and the
@@ -195,7 +210,7 @@ def token_logps_and_entropy(
         )
     logps, entropy = _TokenLogpsAndEntropy.apply(
         embed_tokens, hidden, _as_int32(tokens).view(math.prod(prefix), K), tuple(tokens.shape), softcap, mesh, token_chunk,
-        dh_reduce_f32, skip_zero_grad,
+        dh_reduce_f32, skip_zero_grad, keep_logits,
     )
     if leaves and not capturing:
         logps.grad_fn.leaves = [weakref.ref(x) for x in leaves]

@@ -221,9 +221,11 @@ def dist_forward(
     softcap: float | None,
     logp: torch.Tensor,
     entropy: torch.Tensor,
+    kept: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """``lp_dist_fwd`` for int32 ``tokens`` [T, K] into f32 ``logp`` (T * K) and ``entropy`` (T). Returns
-    what the backward needs, f32 [T * K + T]: the tokens' logits, then the rows' log-normalisers."""
+    what the backward needs, f32 [T * K + T]: the tokens' logits, then the rows' log-normalisers.
+    ``kept`` (uint8, ``dist_kept_bytes``) receives the logits in 16 bits."""
     dev = _check_head(embed, hidden, tokens)
     lib = _lib.load()
     T, K = tokens.shape
@@ -238,15 +240,25 @@ def dist_forward(
             zt = saved.data_ptr()
             return lib.lp_dist_fwd(
                 stream, h.data_ptr(), T, d, ldh, w.data_ptr(), V, 0, tokens.data_ptr(), K, softcap or 0.0, None, zt,
-                zt + 4 * T * K, entropy.data_ptr(), logp.data_ptr(), wsp, wsn,
+                zt + 4 * T * K, entropy.data_ptr(), logp.data_ptr(), _addr(kept), wsp, wsn,
             )
 
         _on_device(dev, "lp_dist_fwd", call)
     return saved
 
 
+def dist_kept_bytes(rows: int, vocab_rows: int) -> int:
+    """Bytes of the kept logits of ``rows`` rows over a (shard of the) vocabulary."""
+    return int(_lib.load().lp_dist_kept_bytes(rows, vocab_rows))
+
+
 def dist_forward_shard(
-    embed: torch.Tensor, hidden: torch.Tensor, tokens: torch.Tensor, softcap: float | None, vocab_offset: int
+    embed: torch.Tensor,
+    hidden: torch.Tensor,
+    tokens: torch.Tensor,
+    softcap: float | None,
+    vocab_offset: int,
+    kept: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``lp_dist_fwd`` over one shard of the vocabulary: (stats [3, T], zt [T, K]) for ``dist_combine``."""
     dev = _check_head(embed, hidden, tokens)
@@ -262,7 +274,7 @@ def dist_forward_shard(
             ws, wsp, wsn = _workspace(lib.lp_dist_fwd_workspace_bytes(T, w.shape[0]), dev)
             return lib.lp_dist_fwd(
                 stream, h.data_ptr(), T, h.shape[1], ldh, w.data_ptr(), w.shape[0], int(vocab_offset),
-                tokens.data_ptr(), K, softcap or 0.0, stats.data_ptr(), zt.data_ptr(), None, None, None, wsp, wsn,
+                tokens.data_ptr(), K, softcap or 0.0, stats.data_ptr(), zt.data_ptr(), None, None, None, _addr(kept), wsp, wsn,
             )
 
         _on_device(dev, "lp_dist_fwd", call)
@@ -302,6 +314,9 @@ def dist_backward(
     grad_logp: torch.Tensor | None,
     grad_entropy: torch.Tensor | None,
     *,
+    kept: torch.Tensor | None = None,
+    kept_rows: int = 0,
+    row_of: torch.Tensor | None = None,
     vocab_offset: int = 0,
     vocab: int | None = None,
     need_dh: bool = True,
@@ -312,7 +327,8 @@ def dist_backward(
 ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """``lp_dist_bwd``: (dH [T, d], partial over this shard; dW [Vs, d]) of contiguous f32 ``grad_logp``
     (T * K) and ``grad_entropy`` (T), either of which may be None. ``saved`` is the forward's;
-    ``vocab`` is the whole vocabulary's size."""
+    ``vocab`` is the whole vocabulary's size. ``kept`` are the forward's kept logits of ``kept_rows``
+    rows, of which row t's are at ``row_of[t]`` (int32; None: t)."""
     dev = _check_head(embed, hidden, tokens, saved, entropy, grad_logp, grad_entropy)
     lib = _lib.load()
     T, K = tokens.shape
@@ -339,7 +355,7 @@ def dist_backward(
         return lib.lp_dist_bwd(
             stream, h.data_ptr(), T, d, ldh, w.data_ptr(), Vs, int(vocab_offset), int(vocab) if vocab else Vs,
             tokens.data_ptr(), K, softcap or 0.0, zt, zt + 4 * T * K, entropy.data_ptr(), _addr(grad_logp),
-            _addr(grad_entropy), _addr(dH), d, _addr(dW), flags, chunk, wsp, wsn,
+            _addr(grad_entropy), _addr(kept), kept_rows, _addr(row_of), _addr(dH), d, _addr(dW), flags, chunk, wsp, wsn,
         )
 
     _on_device(dev, "lp_dist_bwd", call)

@@ -288,10 +288,13 @@ LP_API size_t lp_dist_fwd_workspace_bytes(int64_t T, int64_t Vs);
  *   zt       f32 [T, K] or NULL: the tokens' logits, 0 where not owned
  *   lse, entropy  f32 [T] or NULL, logp  f32 [T, K] or NULL: meaningful when the shard is the
  *            whole vocabulary; logp is 0 for an id outside it
+ *   kept     lp_dist_kept_bytes(T, Vs) bytes (16-byte aligned) or NULL: the shard's logits in 16
+ *            bits each, with which lp_dist_bwd needs no recompute of them
  */
+LP_API size_t lp_dist_kept_bytes(int64_t T, int64_t Vs);
 LP_API int lp_dist_fwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs,
                        int64_t v_off, const int32_t* y, int64_t K, float softcap, float* stats, float* zt, float* lse,
-                       float* entropy, float* logp, void* workspace, size_t workspace_bytes);
+                       float* entropy, float* logp, void* kept, void* workspace, size_t workspace_bytes);
 
 /*
  * Merge of P shards: shard_stats f32 [P, 3, T] and shard_zt f32 [P, T, K] (lp_dist_fwd's stats
@@ -311,13 +314,15 @@ LP_API size_t lp_dist_bwd_workspace_bytes(int64_t T, int64_t d, int64_t Vs, int6
  * (the first sum inside the brackets runs over the ids of [0, V) only; dZ is rounded to bf16).
  *   zt, lse, entropy   the forward's (merged over the shards)
  *   g_logp   f32 [T, K] or NULL (no gradient)      g_entropy  f32 [T] or NULL
+ *   kept     the forward's kept logits of kept_rows rows, or NULL: they are recomputed. Row t's are
+ *            at row_of[t] (int32 [T]; NULL: t)
  * dH, dW, flags, token_chunk as lp_bwd.
  */
 LP_API int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t Vs,
                        int64_t v_off, int64_t V, const int32_t* y, int64_t K, float softcap, const float* zt,
-                       const float* lse, const float* entropy, const float* g_logp, const float* g_entropy, void* dH,
-                       int64_t ld_dh, void* dW, int flags, int64_t token_chunk, void* workspace,
-                       size_t workspace_bytes);
+                       const float* lse, const float* entropy, const float* g_logp, const float* g_entropy,
+                       const void* kept, int64_t kept_rows, const int32_t* row_of, void* dH, int64_t ld_dh, void* dW,
+                       int flags, int64_t token_chunk, void* workspace, size_t workspace_bytes);
 
 /* Scratch bytes lp_top and lp_sample_top_k need for k tokens of T rows against V vocabulary rows. */
 LP_API size_t lp_top_workspace_bytes(int64_t T, int64_t V, int k);

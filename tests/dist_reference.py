@@ -11,7 +11,10 @@ is ``delta``, the largest error of any logit of the row. From it:
                                        and of its factor (8 delta + 2^-18), of the magnitudes that
                                        enter it; and log p + E, which can cancel (to 0 where one token
                                        has all the mass), is off by the bounds of log p and of E,
-                                       which p times the entropy's gradient carries into dZ. dH and dW
+                                       which p times the entropy's gradient carries into dZ. Logits kept
+                                       in 16 bits are off by half a step, 24 ln2 / 65535, more (delta of
+                                       dZ alone), and one more than 48 ln2 below the largest of its
+                                       group has p up to 2^-48 of that one's. dH and dW
                                        sum these, and are rounded once more
 """
 
@@ -25,7 +28,7 @@ def _cap(x, c):
 
 
 class Reference:
-    def __init__(self, embed, hidden, softcap):
+    def __init__(self, embed, hidden, softcap, kept=False):
         self.w, self.h, self.c = embed.double(), hidden.double(), softcap
         self.raw = self.h @ self.w.T
         self.z = _cap(self.raw, softcap)
@@ -35,6 +38,8 @@ class Reference:
         self.entropy = -(self.p * self.logp).sum(-1)
         d = embed.shape[1]
         acc = (d / 16 + 4) * 2**-23 * (self.h.abs() @ self.w.abs().T).amax(-1)
+        self.half_step = 24 * 0.6931471805599453 / 65535 if kept else 0.0
+        self.floor = 2.0**-47 if kept else 0.0
         self.delta = acc + (2 * 2**-22 * softcap if softcap is not None else 0.0) + 2**-23 * self.z.abs().amax(-1)
 
     def picked(self, tokens):
@@ -61,11 +66,17 @@ class Reference:
         E = self.entropy[:, None]
         dz = slope * (hot - self.p * (G + ge[:, None] * (self.logp + E)))
         # the slope itself is off by at most 4 * 2^-22 + 2 delta / c where it is near 0
-        size = (slope + (0.0 if self.c is None else 2**-19)) * (
-            hot_abs + self.p * (G_abs + ge[:, None].abs() * (self.logp.abs() + E))
+        raw = hot_abs + self.p * (G_abs + ge[:, None].abs() * (self.logp.abs() + E))
+        size = (slope + (0.0 if self.c is None else 2**-19)) * raw
+        far = self.floor * (G_abs + ge[:, None].abs() * (40.0 + E))
+        # p is off by delta + half a step of itself, log p by as much, and the slope, 1 - (z / c)^2, by
+        # at most 2 / c of it whatever its own size
+        off = (1.01 * 2**-8 + 8 * (self.delta[:, None] + self.half_step) + 2**-18) * size + far
+        if self.c is not None:
+            off = off + 2 / self.c * (self.delta[:, None] + self.half_step) * raw
+        off = off + self.p * ge[:, None].abs() * (
+            self.logp_bound(self.logp) + self.entropy_bound()[:, None] + self.half_step
         )
-        off = (1.01 * 2**-8 + 8 * self.delta[:, None] + 2**-18) * size
-        off = off + self.p * ge[:, None].abs() * (self.logp_bound(self.logp) + self.entropy_bound()[:, None])
         # products and sums of the two gradient products in f32: far below the terms above
         bound = lambda ref, b: b + 1.01 * 2**-8 * ref.abs() + 1e-30  # noqa: E731
         dH, dW = dz @ self.w, dz.T @ self.h

@@ -91,7 +91,7 @@ def test_c_entries_refuse_before_the_device(lib):
         assert rc == _lib.LP_EINVAL and fragment in lib.lp_last_error().decode()
 
     def fwd(T=4, d=8, ldh=8, K=2, y=fake):
-        return lib.lp_dist_fwd(None, fake, T, d, ldh, fake, 10, 0, y, K, 0.0, None, fake, fake, fake, fake, fake, 1 << 20)
+        return lib.lp_dist_fwd(None, fake, T, d, ldh, fake, 10, 0, y, K, 0.0, None, fake, fake, fake, fake, None, fake, 1 << 20)
 
     refused(fwd(d=12), "multiple of 8")
     refused(fwd(ldh=4), "ldh")
@@ -102,14 +102,18 @@ def test_c_entries_refuse_before_the_device(lib):
     refused(lib.lp_dist_combine(None, fake, fake, 0, 4, 1, 10, fake, fake, fake, fake, fake), "bad P")
     refused(lib.lp_dist_combine(None, fake, None, 2, 4, 1, 10, fake, fake, fake, fake, fake), "null shard_zt")
 
-    def bwd(v_off=0, V=10, zt=fake, dH=fake, dW=fake):
-        return lib.lp_dist_bwd(None, fake, 4, 8, 8, fake, 10, v_off, V, fake, 2, 0.0, zt, fake, fake, fake, fake, dH, 8, dW, 0,
-                               0, fake, 1 << 20)
+    def bwd(v_off=0, V=10, zt=fake, dH=fake, dW=fake, kept=None, kept_rows=4, row_of=None):
+        return lib.lp_dist_bwd(None, fake, 4, 8, 8, fake, 10, v_off, V, fake, 2, 0.0, zt, fake, fake, fake, fake, kept,
+                               kept_rows, row_of, dH, 8, dW, 0, 0, fake, 1 << 20)
 
     refused(bwd(v_off=5), "outside the vocabulary")
     refused(bwd(zt=None), "null lse")
     refused(bwd(dH=None), "dH")
     refused(bwd(dW=None), "dW")
+    refused(bwd(kept=P(4100)), "kept logits")
+    refused(bwd(kept=fake, kept_rows=3), "kept logits")
+    assert lib.lp_dist_kept_bytes(3, 300) == 3 * 304 * 2 + 224 + 3 * 16 * 4  # 16-bit rows, 256-byte step, f32 maxima
+    assert lib.lp_dist_kept_bytes(0, 300) == 0
     for k in (0, 11, 129):
         refused(lib.lp_top(None, fake, 4, 8, 8, fake, 10, 0.0, k, None, fake, fake, fake, None, fake, 1 << 20), "k=")
     refused(lib.lp_top(None, fake, 4, 8, 8, fake, 10, 0.0, 2, fake, fake, fake, fake, None, fake, 1 << 20), "token_logps")

@@ -60,8 +60,9 @@ def test_logps_and_entropy(cuda_device, T, V, d, softcap, K):
 
 
 @pytest.mark.parametrize("T,V,d,softcap", SHAPES)
-@pytest.mark.parametrize("K,send", [(1, "both"), (5, "both"), (4, "logps"), (2, "entropy")])
-def test_gradients(cuda_device, T, V, d, softcap, K, send):
+@pytest.mark.parametrize("K,send", [(1, "both"), (1, "logps"), (1, "entropy"), (5, "both"), (4, "logps"), (2, "entropy")])
+@pytest.mark.parametrize("keep", [True, False])
+def test_gradients(cuda_device, T, V, d, softcap, K, send, keep):
     from gemma4_posttrain_jax_b200 import _lib, token_logps_and_entropy
 
     W, H, gen = _inputs(cuda_device, T, V, d)
@@ -70,28 +71,30 @@ def test_gradients(cuda_device, T, V, d, softcap, K, send):
     ge = torch.randn((T,), generator=gen, device=cuda_device) if send != "logps" else None
     W.requires_grad_(True)
     H.requires_grad_(True)
-    logps, entropy = token_logps_and_entropy(W, H, y, softcap=softcap)
+    logps, entropy = token_logps_and_entropy(W, H, y, softcap=softcap, keep_logits=keep)
     loss = 0.0 if g is None else (logps * g).sum()
     loss = loss if ge is None else loss + (entropy * ge).sum()
     loss.backward()
-    dH, dW, bH, bW = Reference(W.detach(), H.detach(), softcap).grads(y, g, ge)
+    dH, dW, bH, bW = Reference(W.detach(), H.detach(), softcap, kept=keep).grads(y, g, ge)
     within(H.grad, dH, bH, "d hidden")
     within(W.grad, dW, bW, "d embedding")
     assert _lib.device_error(0) == 0
 
 
 @pytest.mark.parametrize("frozen", ["embed", "hidden"])
-def test_one_gradient_alone_and_row_chunks(cuda_device, frozen):
+@pytest.mark.parametrize("K", [1, 3])
+@pytest.mark.parametrize("keep", [True, False])
+def test_one_gradient_alone_and_row_chunks(cuda_device, frozen, K, keep):
     from gemma4_posttrain_jax_b200 import token_logps_and_entropy
 
     T, V, d = 700, 1036, 128
     W, H, gen = _inputs(cuda_device, T, V, d)
-    y = _tokens(gen, cuda_device, T, V, 3)
-    g, ge = torch.randn((T, 3), generator=gen, device=cuda_device), torch.randn((T,), generator=gen, device=cuda_device)
+    y = _tokens(gen, cuda_device, T, V, K)
+    g, ge = torch.randn((T, K), generator=gen, device=cuda_device), torch.randn((T,), generator=gen, device=cuda_device)
     leaf = (H if frozen == "embed" else W).requires_grad_(True)
-    logps, entropy = token_logps_and_entropy(W, H, y, softcap=30.0, token_chunk=256)
+    logps, entropy = token_logps_and_entropy(W, H, y, softcap=30.0, token_chunk=256, keep_logits=keep)
     (got,) = torch.autograd.grad([logps, entropy], [leaf], [g, ge])
-    dH, dW, bH, bW = Reference(W.detach(), H.detach(), 30.0).grads(y, g, ge)
+    dH, dW, bH, bW = Reference(W.detach(), H.detach(), 30.0, kept=keep).grads(y, g, ge)
     within(got, dH if frozen == "embed" else dW, bH if frozen == "embed" else bW, "gradient")
 
 
@@ -128,7 +131,8 @@ def test_gradient_against_differences(cuda_device):
         assert (off <= 40 * 2.0**-20 / step + 2 * 2.0**-8 * size + 0.01 * (g.abs().sum(-1) + ge.abs())).all(), off.max()
 
 
-def test_rows_without_gradient_are_left_out(cuda_device, monkeypatch):
+@pytest.mark.parametrize("keep", [True, False])
+def test_rows_without_gradient_are_left_out(cuda_device, monkeypatch, keep):
     from gemma4_posttrain_jax_b200 import distribution, token_logps_and_entropy
 
     T, V, d = 300, 1036, 64
@@ -142,9 +146,9 @@ def test_rows_without_gradient_are_left_out(cuda_device, monkeypatch):
     results = []
     for least in (float("inf"), 0.0):
         monkeypatch.setattr(distribution, "_SKIP_MIN_FLOPS", least)
-        logps, entropy = token_logps_and_entropy(W, H, y, softcap=30.0)
+        logps, entropy = token_logps_and_entropy(W, H, y, softcap=30.0, keep_logits=keep)
         results.append(torch.autograd.grad([logps, entropy], [H, W], [g, ge]))
-    dH, dW, bH, bW = Reference(W.detach(), H.detach(), 30.0).grads(y, g, ge)
+    dH, dW, bH, bW = Reference(W.detach(), H.detach(), 30.0, kept=keep).grads(y, g, ge)
     for got_H, got_W in results:
         within(got_H, dH, bH, "d hidden")
         within(got_W, dW, bW, "d embedding")
@@ -156,7 +160,8 @@ def test_rows_without_gradient_are_left_out(cuda_device, monkeypatch):
 
 
 @pytest.mark.parametrize("V,P", [(1040, 4), (4098, 2)])
-def test_shards_merge_to_the_whole(cuda_device, V, P):
+@pytest.mark.parametrize("keep", [True, False])
+def test_shards_merge_to_the_whole(cuda_device, V, P, keep):
     """One GPU plays every rank of a vocabulary mesh in turn: the merged statistics and the summed
     partial gradients are the whole vocabulary's."""
     from gemma4_posttrain_jax_b200 import ops
@@ -166,10 +171,11 @@ def test_shards_merge_to_the_whole(cuda_device, V, P):
     W[V // P] *= 40  # one shard's maximum far above the others'
     y = _tokens(gen, cuda_device, T, V, K).to(torch.int32).contiguous()
     g, ge = torch.randn((T, K), generator=gen, device=cuda_device), torch.randn((T,), generator=gen, device=cuda_device)
-    ref = Reference(W, H, 30.0)
+    ref = Reference(W, H, 30.0, kept=keep)
     vs = V // P
+    kept = [torch.empty(ops.dist_kept_bytes(T, vs), dtype=torch.uint8, device=cuda_device) if keep else None for _ in range(P)]
     shards = [W[p * vs : (p + 1) * vs] for p in range(P)]
-    parts = [ops.dist_forward_shard(w, H, y, 30.0, p * vs) for p, w in enumerate(shards)]
+    parts = [ops.dist_forward_shard(w, H, y, 30.0, p * vs, kept[p]) for p, w in enumerate(shards)]
     logp, entropy = torch.empty((T, K), device=cuda_device), torch.empty((T,), device=cuda_device)
     saved = ops.dist_combine(
         torch.stack([s for s, _ in parts]), torch.stack([z for _, z in parts]), y, V, logp, entropy
@@ -178,12 +184,32 @@ def test_shards_merge_to_the_whole(cuda_device, V, P):
     within(logp, picked, ref.logp_bound(picked), "logps")
     within(entropy, ref.entropy, ref.entropy_bound(), "entropy")
     grads = [
-        ops.dist_backward(w, H, y, 30.0, saved, entropy, g, ge, vocab_offset=p * vs, vocab=V, dh_dtype=torch.float32)
+        ops.dist_backward(w, H, y, 30.0, saved, entropy, g, ge, vocab_offset=p * vs, vocab=V, dh_dtype=torch.float32, kept=kept[p],
+                          kept_rows=T)
         for p, w in enumerate(shards)
     ]
     dH, dW, bH, bW = ref.grads(y, g, ge)
     within(sum(a for a, _ in grads), dH, bH, "d hidden")
     within(torch.cat([b for _, b in grads]), dW, bW, "d embedding")
+
+
+def test_logits_far_below_the_largest(cuda_device):
+    """Kept logits reach 2^-48 of the largest of their 32 columns: what lies lower has no gradient to
+    speak of, and where all of a row's mass is elsewhere, a group's own scale still holds."""
+    from gemma4_posttrain_jax_b200 import token_logps_and_entropy
+
+    T, V, d = 64, 640, 64
+    W, H, gen = _inputs(cuda_device, T, V, d)
+    W[32:64] *= 30  # logits of +-100 next to one another
+    W[100] *= 60
+    y = _tokens(gen, cuda_device, T, V, 3)
+    g, ge = torch.randn((T, 3), generator=gen, device=cuda_device), torch.randn((T,), generator=gen, device=cuda_device)
+    W.requires_grad_(True), H.requires_grad_(True)
+    logps, entropy = token_logps_and_entropy(W, H, y, softcap=None, keep_logits=True)
+    got_H, got_W = torch.autograd.grad([logps, entropy], [H, W], [g, ge])
+    dH, dW, bH, bW = Reference(W.detach(), H.detach(), None, kept=True).grads(y, g, ge)
+    within(got_H, dH, bH, "d hidden")
+    within(got_W, dW, bW, "d embedding")
 
 
 def test_shapes_strides_and_empty_batches(cuda_device):
@@ -478,7 +504,7 @@ def test_distillation_and_rollout_together(cuda_device):
     logps, entropy = token_logps_and_entropy(W, H, alternatives.ids, softcap=30.0)
     loss = (weight * (alternatives.logps - logps)).sum() - 0.1 * entropy.sum()
     dH, dW = torch.autograd.grad(loss, [H, W])
-    ref = Reference(W.detach(), H.detach(), 30.0)
+    ref = Reference(W.detach(), H.detach(), 30.0, kept=True)
     rH, rW, bH, bW = ref.grads(alternatives.ids.long(), -weight, torch.full((T,), -0.1, device=cuda_device))
     within(dH, rH, bH, "d hidden")
     within(dW, rW, bW, "d embedding")
