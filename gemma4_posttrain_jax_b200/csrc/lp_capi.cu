@@ -222,7 +222,11 @@ int current_device_info(DeviceInfo** out) {
   if (dev < 0 || dev >= kMaxDevices) return fail(LP_EINVAL, "device ordinal %d out of range", dev);
   // a thread that has made no runtime call yet (one of autograd's, say) has a current device but no
   // context, which the driver's tensor-map encoder needs
-  LP_CUDA_TRY(cudaSetDevice(dev));
+  static thread_local int bound = -1;
+  if (bound != dev) {
+    LP_CUDA_TRY(cudaSetDevice(dev));
+    bound = dev;
+  }
   std::lock_guard<std::mutex> lk(g_dev_mu);
   DeviceInfo& d = g_dev[dev];
   if (!d.ready) {
@@ -1024,6 +1028,10 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
       z.cap = softcap;
       z.dz = dz;
       z.ldz = L.ldz;
+      // enough blocks for every SM, a row each where there are rows enough
+      const int64_t row_steps = cdiv(Vs, kDzStep);
+      const int64_t per_row = std::max<int64_t>(1, std::min<int64_t>(cdiv(row_steps, 2), cdiv(16 * di->sms, tcur)));
+      z.steps = (int)cdiv(row_steps, per_row);
       ProfScope prof(st, "dist_dz");
       for (int64_t r = 0; r < tcur; r += 32768) {  // a grid has at most 65535 rows
         const int64_t rows = std::min<int64_t>(32768, tcur - r);
@@ -1042,7 +1050,7 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
           zr.entropy = z.entropy + r;
         }
         zr.dz = z.dz + r * L.ldz;
-        dist_dz_kernel<<<dim3((unsigned)cdiv(Vs, kDzCols), (unsigned)rows), 256, 0, st>>>(zr);
+        dist_dz_kernel<<<dim3((unsigned)cdiv(row_steps, z.steps), (unsigned)rows), 256, 0, st>>>(zr);
         LP_LAUNCH_CHECK("dist_dz_kernel");
       }
     }

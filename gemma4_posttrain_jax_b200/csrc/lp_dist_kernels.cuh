@@ -273,10 +273,11 @@ struct DistDzParams {
   float cap;
   __nv_bfloat16* dz;
   long long ldz;
+  int steps;  // per block
 };
-constexpr int kDzCols = 8192;
+constexpr int kDzStep = 2048;  // columns of a block's step
 
-__global__ void __launch_bounds__(256) dist_dz_kernel(const DistDzParams P) {
+__global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
   const int t = blockIdx.y;
   float a, b, l2, gv = 0.f;
   long long yl = -1;
@@ -299,42 +300,55 @@ __global__ void __launch_bounds__(256) dist_dz_kernel(const DistDzParams P) {
   const uint16_t* kept = P.kept + from * P.ldk;
   const float* kept_max = P.kept_max + from * P.ld_max;
   __nv_bfloat16* dz = P.dz + (size_t)t * P.ldz;
-  const float ucap = P.cap > 0.f ? kLn2 / P.cap : 0.f;  // z2 -> tanh(x / c)
-  const long long c0 = (long long)blockIdx.x * kDzCols + threadIdx.x * 8;
-  uint4 q[kDzCols / 2048];
-  float mx[kDzCols / 2048];
-#pragma unroll
-  for (int i = 0; i < kDzCols / 2048; ++i) {
-    const long long col = c0 + i * 2048;
-    if (col < P.Vs) {
-      q[i] = __ldcs(reinterpret_cast<const uint4*>(kept + col));
-      mx[i] = __ldg(kept_max + col / 32);
-    }
+  const float ucap = P.cap > 0.f ? kLn2 / P.cap : 0.f;  // z2 -> tanh(x / c), without softcap 0
+  const int c0 = (int)blockIdx.x * P.steps * kDzStep + (int)threadIdx.x * 8;
+  const int end = min((int)P.Vs, (int)(blockIdx.x + 1) * P.steps * kDzStep);
+  uint4 q = make_uint4(0, 0, 0, 0);
+  float mx = 0.f;
+  if (c0 < end) {
+    q = __ldcs(reinterpret_cast<const uint4*>(kept + c0));
+    mx = __ldg(kept_max + c0 / 32);
   }
-#pragma unroll
-  for (int i = 0; i < kDzCols / 2048; ++i) {
-    const long long col = c0 + i * 2048;
-    if (col >= P.Vs) break;
-    const float top = mx[i] - l2;  // log2 p of the largest of the 32
-    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+  constexpr float step = kKeepRange / 65535.f;
+  auto two = [](float x) { return pack_f32x2(x, x); };
+  const f32x2 a2 = two(a), b2 = two(b), ml2 = two(-l2), ucap2 = two(ucap), mstep2 = two(-step), m23 = two(-8388608.f),
+              mone = two(-1.f);
+  const int yc = yl >= 0 && yl < P.Vs ? (int)yl : -8;  // the row's token among this shard's columns
+#pragma unroll 1
+  for (int col = c0; col < end; col += kDzStep) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    const float m = mx;
+    if (col + kDzStep < end) {
+      q = __ldcs(reinterpret_cast<const uint4*>(kept + col + kDzStep));
+      mx = __ldg(kept_max + (col + kDzStep) / 32);
+    }
+    const f32x2 top = two(m);
     uint32_t out[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float v[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        // 2^23 + n, whose low bits are n, less 2^23
-        const float n = __uint_as_float(k == 0 ? (w[j] & 0xffffu) | 0x4b000000u : (w[j] >> 16) | 0x4b000000u) - 8388608.f;
-        const float lp = fmaf(n, -kKeepRange / 65535.f, top);
-        const float u = (lp + l2) * ucap;
-        float x = -fast_ex2(lp) * fmaf(b, lp, a);
-        if (col + 2 * j + k == yl) x += gv;
-        v[k] = fmaf(-u, u, 1.f) * x;
-      }
-      out[j] = pack_bf16x2(v[0], v[1]);
+      // 2^23 + n, whose low bits are n, less 2^23
+      const f32x2 n = add_f32x2(pack_f32x2(__uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7610)),
+                                           __uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7632))),
+                                m23);
+      const f32x2 z = fma_f32x2(n, mstep2, top);
+      const f32x2 lp = add_f32x2(z, ml2);
+      const f32x2 u = mul_f32x2(z, ucap2);
+      float l0, l1, v0, v1;
+      unpack_f32x2(lp, l0, l1);
+      // p (a + b log2 p) (u^2 - 1)
+      const f32x2 v = mul_f32x2(mul_f32x2(pack_f32x2(fast_ex2(l0), fast_ex2(l1)), fma_f32x2(b2, lp, a2)),
+                                fma_f32x2(u, u, mone));
+      unpack_f32x2(v, v0, v1);
+      out[j] = pack_bf16x2(v0, v1);
     }
     // rows of dZ are padded to 16 bytes
     *reinterpret_cast<uint4*>(dz + col) = make_uint4(out[0], out[1], out[2], out[3]);
+    if ((unsigned)(yc - col) < 8u) {
+      // the row's token: its entry again, with its gradient
+      const float z = fmaf((float)kept[yc], -step, m);
+      const float lp = z - l2, u = z * ucap;
+      dz[yc] = __float2bfloat16_rn((fmaf(b, lp, a) * fast_ex2(lp) - gv) * fmaf(u, u, -1.f));
+    }
   }
 }
 
