@@ -154,11 +154,9 @@ __global__ void __launch_bounds__(kDistThreads)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows = min(R, T - t0);
   // the tokens' rows of W come from all over it: ask for them before the partials are merged
-  for (int i = warp; i < rows * K; i += kDistThreads / 32) {
+  for (int i = threadIdx.x; i < rows * K; i += kDistThreads) {
     const long long v = (long long)y[(size_t)(t0 + i / K) * K + i % K] - v_off;
-    if (v >= 0 && v < Vs)
-      for (int l = lane * 128; l < (int)d * 2; l += 32 * 128)
-        prefetch_l2(reinterpret_cast<const char*>(W + (size_t)v * d) + l);
+    if (v >= 0 && v < Vs) prefetch_l2_bulk(W + (size_t)v * d, (uint32_t)d * 2);
   }
   DistAcc acc{-INFINITY, 0.f, 0.f};
   if (t < T) {
@@ -469,7 +467,7 @@ __device__ __forceinline__ double ordered_f64(long long b) {
 
 // G: columns per key (1: the keys are the accumulators).
 template <bool SAMPLE, int G>
-__global__ void __launch_bounds__(kTopThreads, 3) top_select_kernel(const TopParams P) {
+__global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopParams P) {
   constexpr bool GROUPS = G > 1;
   // keys while selecting, then the candidates' scores and ids
   extern __shared__ __align__(16) uint8_t dyn_s[];
@@ -500,6 +498,8 @@ __global__ void __launch_bounds__(kTopThreads, 3) top_select_kernel(const TopPar
   auto key = [&](int i) -> uint32_t { return P.keys_in_smem ? keys_s[i] : load_key(i); };
 
   // ---- loads: the row's partials (up to four per thread at once), hidden state and keys
+  const long long token = !SAMPLE && P.tokens != nullptr ? P.tokens[t] : -1;
+  if (tid == 0 && token >= 0 && token < P.V) prefetch_l2_bulk(P.W + (size_t)token * P.d, (uint32_t)P.d * 2);
   constexpr int PN = 4;
   float2 pv[PN];
   float pa[PN];
@@ -757,9 +757,8 @@ __global__ void __launch_bounds__(kTopThreads, 3) top_select_kernel(const TopPar
     __syncthreads();
     // The candidates' rows of W come from all over it: ask for all of them at once, so that their
     // latencies (HBM and address translation) pass together and not once per round of the warps.
-    for (int i = have + warp; i < count; i += kWarps)
-      for (int l = lane * 128; l < (int)P.d * 2; l += 32 * 128)
-        prefetch_l2(reinterpret_cast<const char*>(P.W + (size_t)cand_id[i] * P.d) + l);
+    for (int i = have + tid; i < count; i += kTopThreads)
+      prefetch_l2_bulk(P.W + (size_t)cand_id[i] * P.d, (uint32_t)P.d * 2);
 #pragma unroll 1
     for (int i = have + warp; i < count; i += kWarps) {
       const double z = warp_dot_exact(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);
@@ -800,7 +799,7 @@ __global__ void __launch_bounds__(kTopThreads, 3) top_select_kernel(const TopPar
     }
     if (tid == 0) P.entropy[t] = dist_entropy(acc);
     if (P.tokens != nullptr && warp == kTopThreads / 32 - 1) {
-      const long long v = P.tokens[t];
+      const long long v = token;
       float lp = 0.f;
       if (v >= 0 && v < P.V) lp = dist_logp(softcap_exact(warp_dot(h, P.W + (size_t)v * P.d, P.d, lane), P.cap), lse);
       if (lane == 0) P.token_logps[t] = lp;
