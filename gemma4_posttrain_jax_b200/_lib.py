@@ -87,6 +87,8 @@ _SIG = {
         [_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, _P, _P, _P, _P, _P, _P, _I64, _P, _P,
          _I64, _P, ctypes.c_int, _I64, _P, ctypes.c_size_t],
     ),
+    "lp_dist_rows_workspace_bytes": (ctypes.c_size_t, [_I64]),
+    "lp_dist_rows": (ctypes.c_int, [_P, _P, _I64, _I64, _I64, _P, _I64] + [_P] * 16 + [ctypes.c_size_t]),
     "lp_top_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, ctypes.c_int]),
     "lp_top": (
         ctypes.c_int,

@@ -1625,6 +1625,49 @@ int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, 
                   token_chunk, workspace, workspace_bytes, nullptr, &dg);
 }
 
+size_t lp_dist_rows_workspace_bytes(int64_t T) {
+  return align_up((size_t)std::max<int64_t>(T, 1), 256) + lp_compact_workspace_bytes(1, T);
+}
+
+int lp_dist_rows(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const int32_t* y, int64_t K,
+                 const float* zt, const float* lse, const float* entropy, const float* g_logp, const float* g_entropy,
+                 void* H_out, int32_t* y_out, float* zt_out, float* lse_out, float* entropy_out, float* g_logp_out,
+                 float* g_entropy_out, int32_t* idx, int32_t* pos, int32_t* count, void* workspace,
+                 size_t workspace_bytes) {
+  if (T <= 0 || T > (int64_t)1 << 30 || d <= 0 || d % 8 != 0 || ldh < d || ldh % 8 != 0)
+    return fail(LP_EINVAL, "bad sizes T=%lld d=%lld ldh=%lld", (long long)T, (long long)d, (long long)ldh);
+  if (K < 0 || K > LP_DIST_MAX_TOKENS) return fail(LP_EINVAL, "K=%lld tokens per row, at most %d", (long long)K,
+                                                    LP_DIST_MAX_TOKENS);
+  if (H == nullptr || lse == nullptr || entropy == nullptr || H_out == nullptr || lse_out == nullptr ||
+      entropy_out == nullptr || (K > 0 && (y == nullptr || zt == nullptr || y_out == nullptr || zt_out == nullptr)) ||
+      (g_logp != nullptr && g_logp_out == nullptr) || (g_entropy != nullptr && g_entropy_out == nullptr))
+    return fail(LP_EINVAL, "null input or output");
+  if (((reinterpret_cast<uintptr_t>(H) | reinterpret_cast<uintptr_t>(H_out)) & 15) != 0)
+    return fail(LP_EINVAL, "hidden rows must be 16-byte aligned");
+  const size_t need = lp_dist_rows_workspace_bytes(T);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(LP_EWORKSPACE, "lp_dist_rows needs %zu workspace bytes, got %zu", need, workspace_bytes);
+  DeviceInfo* di = nullptr;
+  int rc = current_device_info(&di);
+  if (rc) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  uint8_t* mask = reinterpret_cast<uint8_t*>(workspace);
+  char* rest = reinterpret_cast<char*>(workspace) + align_up((size_t)T, 256);
+  ProfScope prof(st, "dist_rows");
+  dist_row_mask_kernel<<<(unsigned)cdiv(T, 256), 256, 0, st>>>(K > 0 ? g_logp : nullptr, g_entropy, (int)T, (int)K, mask);
+  LP_LAUNCH_CHECK("dist_row_mask_kernel");
+  if ((rc = lp_compact(stream, mask, 1, T, nullptr, 0, 0, 0, 0, nullptr, nullptr, nullptr, idx, pos, count, rest,
+                       lp_compact_workspace_bytes(1, T))))
+    return rc;
+  const DistRows from{reinterpret_cast<const __nv_bfloat16*>(H), ldh, y, zt, lse, entropy, g_logp, g_entropy};
+  const DistRowsOut to{reinterpret_cast<__nv_bfloat16*>(H_out), y_out, zt_out, lse_out, entropy_out, g_logp_out,
+                       g_entropy_out};
+  const int64_t warps = std::min<int64_t>(T, (int64_t)di->sms * 32);
+  dist_gather_kernel<<<(unsigned)cdiv(warps * 32, 256), 256, 0, st>>>(idx, count, from, to, d, (int)K);
+  LP_LAUNCH_CHECK("dist_gather_kernel");
+  return LP_OK;
+}
+
 size_t lp_top_workspace_bytes(int64_t T, int64_t V, int k) {
   DeviceInfo* di = nullptr;
   const bool have = current_device_info(&di) == LP_OK;

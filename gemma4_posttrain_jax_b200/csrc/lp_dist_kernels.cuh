@@ -254,6 +254,55 @@ __global__ void dist_row_const_kernel(const float* __restrict__ lse, const float
   row_const[(size_t)2 * T + t] = lse[t] * kLog2e;
 }
 
+// mask[t] = whether row t sends any gradient: one of its g [T, K] or its ge [T] is not zero (either
+// may be null).
+__global__ void dist_row_mask_kernel(const float* __restrict__ g, const float* __restrict__ ge, int T, int K,
+                                     uint8_t* __restrict__ mask) {
+  const int t = blockIdx.x * blockDim.x + threadIdx.x;
+  if (t >= T) return;
+  bool sent = ge != nullptr && ge[t] != 0.f;
+  if (g != nullptr)
+    for (int k = 0; k < K; ++k) sent |= g[(size_t)t * K + k] != 0.f;
+  mask[t] = sent ? 1 : 0;
+}
+
+// Everything the backward reads of the rows that do, one warp per row: the hidden state, the tokens
+// with their logits and gradients, and the row's scalars.
+struct DistRows {
+  const __nv_bfloat16* H;
+  long long ldh;
+  const int32_t* y;
+  const float *zt, *lse, *entropy, *g, *ge;
+};
+struct DistRowsOut {
+  __nv_bfloat16* H;
+  int32_t* y;
+  float *zt, *lse, *entropy, *g, *ge;
+};
+__global__ void dist_gather_kernel(const int32_t* __restrict__ idx, const int* __restrict__ count, const DistRows from,
+                                   const DistRowsOut to, long long d, int K) {
+  const int lane = threadIdx.x & 31;
+  const int n = *count;
+  const int stride = (int)((gridDim.x * blockDim.x) >> 5);
+  for (int i = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5); i < n; i += stride) {
+    const int t = idx[i];
+    const uint4* src = reinterpret_cast<const uint4*>(from.H + (size_t)t * from.ldh);
+    uint4* dst = reinterpret_cast<uint4*>(to.H + (size_t)i * d);
+    for (int v = lane; v < (int)(d / 8); v += 32) dst[v] = src[v];
+    for (int k = lane; k < K; k += 32) {
+      const size_t a = (size_t)t * K + k, b = (size_t)i * K + k;
+      to.y[b] = from.y[a];
+      to.zt[b] = from.zt[a];
+      if (from.g != nullptr) to.g[b] = from.g[a];
+    }
+    if (lane == 0) {
+      to.lse[i] = from.lse[t];
+      to.entropy[i] = from.entropy[t];
+      if (from.ge != nullptr) to.ge[i] = from.ge[t];
+    }
+  }
+}
+
 // dZ of a chunk from kept logits (EPI_DIST_KEEP) instead of a recomputed product: reads 2 bytes and
 // writes 2 per entry, where the recompute costs 2 d flops. The same formula as EPI_DIST_DZ's; with one
 // token per row its entry is in it, too. One block per row and 8192 columns, eight columns (16 bytes)

@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .losses import _gather_rows, _nonzero_grad_rows, _validate_softcap
+from .losses import _SKIP_ZERO_GRAD_MIN_FRACTION, _check_device, _validate_softcap
 from .phase_timer import phase
 from .sharding import VocabMesh, all_gather_stats, all_reduce_sum, vocab_offset
 
@@ -45,11 +45,6 @@ def _as_int32(tokens: torch.Tensor) -> torch.Tensor:
     if tokens.dtype in (torch.int64, torch.uint64, torch.uint32):
         tokens = tokens.to(torch.int64).clamp(-1, 2**31 - 1)
     return tokens.to(torch.int32).contiguous()
-
-
-def _gather(rows: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
-    """``rows`` [n] or [n, w] (f32 or int32) at ``idx``."""
-    return _gather_rows(rows.view(torch.float32), idx).view(rows.dtype) if rows.numel() else rows[: idx.numel()]
 
 
 class _TokenLogpsAndEntropy(torch.autograd.Function):
@@ -100,33 +95,26 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
             return (torch.zeros_like(embed) if need_dw else None), (torch.zeros_like(hidden) if need_dh else None), *none
         g = None if g is None else g.contiguous()
         ge = None if ge is None else ge.contiguous()
-        rows = hidden.reshape(T, d)
-        pos = row_of = None
+        args = (hidden.reshape(T, d), tokens, saved, entropy, g, ge)
+        rows = pos = row_of = None
         if (
             skip_zero_grad
             and 6.0 * T * d * embed.shape[0] >= _SKIP_MIN_FLOPS
             and not torch.cuda.is_current_stream_capturing()
         ):
-            sent = torch.zeros((T,), dtype=torch.bool, device=hidden.device) if ge is None else ge.reshape(T) != 0
-            if g is not None and K > 0:
-                sent = sent | (g.reshape(T, K) != 0).any(dim=1)
-            sel = _nonzero_grad_rows(sent)
-            if sel is not None:
-                idx, pos, m = sel
-                if m == 0:
-                    return (
-                        (torch.zeros_like(embed) if need_dw else None), (torch.zeros_like(hidden) if need_dh else None), *none
-                    )
-                row_of = idx
-                rows, entropy = _gather_rows(rows, idx), _gather(entropy.reshape(T), idx)
-                tokens = _gather(tokens, idx)
-                saved = torch.cat([_gather(saved[: T * K].view(T, K), idx).reshape(-1), _gather(saved[T * K :], idx)])
-                g = None if g is None else _gather(g.reshape(T, K), idx)
-                ge = None if ge is None else _gather(ge.reshape(T), idx)
+            idx, where, count, gathered = ops.dist_rows(*args)
+            m = int(count.item())
+            _check_device(hidden.device, "token_logps_and_entropy backward")  # the host has waited anyway
+            if m == 0:
+                return (
+                    (torch.zeros_like(embed) if need_dw else None), (torch.zeros_like(hidden) if need_dh else None), *none
+                )
+            if T - m >= _SKIP_ZERO_GRAD_MIN_FRACTION * T:
+                args, rows, pos, row_of = gathered, m, where, idx
         dh_dtype = torch.float32 if P > 1 and dh_reduce_f32 else torch.bfloat16
         dH, dW = ops.dist_backward(
-            embed, rows, tokens, softcap, saved, entropy, g, ge, kept=kept, kept_rows=T, row_of=row_of, vocab_offset=off,
-            vocab=embed.shape[0] * P, need_dh=need_dh, need_dw=need_dw, dh_dtype=dh_dtype, token_chunk=token_chunk,
+            embed, softcap, *args, rows=rows, kept=kept, row_of=row_of, vocab_offset=off, vocab=embed.shape[0] * P,
+            need_dh=need_dh, need_dw=need_dw, dh_dtype=dh_dtype, token_chunk=token_chunk,
         )
         if dH is not None:
             if P > 1:
@@ -149,8 +137,8 @@ _eager_graphs: weakref.WeakSet = weakref.WeakSet()
 _KEPT_MAX_BYTES = 4 << 30
 
 # Rows without a gradient add nothing, and a backward of at least this much work (about 6 ms)
-# leaves them out. Below it, finding them on the host and gathering the others (0.15 ms) costs what a
-# tenth of the rows would; so do whole tiles of 256 rows that a few rows fewer do not save.
+# leaves them out. Below it, the wait for their number and whole tiles of 256 rows that a few rows
+# fewer do not save cost what a tenth of the rows would.
 _SKIP_MIN_FLOPS = 1e13
 
 

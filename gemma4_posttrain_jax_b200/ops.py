@@ -304,18 +304,55 @@ def dist_combine(
     return saved
 
 
-def dist_backward(
-    embed: torch.Tensor,
+def dist_rows(
     hidden: torch.Tensor,
     tokens: torch.Tensor,
+    saved: torch.Tensor,
+    entropy: torch.Tensor,
+    grad_logp: torch.Tensor | None,
+    grad_entropy: torch.Tensor | None,
+):
+    """``lp_dist_rows``: (idx [T], pos [T], count [1], rows), where ``rows`` are the arguments of
+    ``dist_backward`` from ``hidden`` on (without softcap), holding the ``count`` rows that send a
+    gradient first."""
+    dev = _require_cuda(hidden, tokens, saved, entropy, grad_logp, grad_entropy)
+    lib = _lib.load()
+    T, K = tokens.shape
+    h, ldh = _dense_rows(hidden)
+    d = h.shape[1]
+    h_out = torch.empty((T, d), dtype=h.dtype, device=dev)
+    y_out = torch.empty_like(tokens)
+    saved_out, entropy_out = torch.empty_like(saved), torch.empty((T,), dtype=torch.float32, device=dev)
+    g_out = None if grad_logp is None else torch.empty((T, K), dtype=torch.float32, device=dev)
+    ge_out = None if grad_entropy is None else torch.empty((T,), dtype=torch.float32, device=dev)
+    index = torch.empty((2 * T + 1,), dtype=torch.int32, device=dev)
+    lse = 4 * T * K
+
+    def call(stream):
+        ws, wsp, wsn = _workspace(lib.lp_dist_rows_workspace_bytes(T), dev)
+        zt, zt_out, at = saved.data_ptr(), saved_out.data_ptr(), index.data_ptr()
+        return lib.lp_dist_rows(
+            stream, h.data_ptr(), T, d, ldh, tokens.data_ptr(), K, zt, zt + lse, entropy.data_ptr(), _addr(grad_logp),
+            _addr(grad_entropy), h_out.data_ptr(), y_out.data_ptr(), zt_out, zt_out + lse, entropy_out.data_ptr(),
+            _addr(g_out), _addr(ge_out), at, at + 4 * T, at + 8 * T, wsp, wsn,
+        )
+
+    _on_device(dev, "lp_dist_rows", call)
+    return index[:T], index[T : 2 * T], index[2 * T :], (h_out, y_out, saved_out, entropy_out, g_out, ge_out)
+
+
+def dist_backward(
+    embed: torch.Tensor,
     softcap: float | None,
+    hidden: torch.Tensor,
+    tokens: torch.Tensor,
     saved: torch.Tensor,
     entropy: torch.Tensor,
     grad_logp: torch.Tensor | None,
     grad_entropy: torch.Tensor | None,
     *,
+    rows: int | None = None,
     kept: torch.Tensor | None = None,
-    kept_rows: int = 0,
     row_of: torch.Tensor | None = None,
     vocab_offset: int = 0,
     vocab: int | None = None,
@@ -327,11 +364,13 @@ def dist_backward(
 ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """``lp_dist_bwd``: (dH [T, d], partial over this shard; dW [Vs, d]) of contiguous f32 ``grad_logp``
     (T * K) and ``grad_entropy`` (T), either of which may be None. ``saved`` is the forward's;
-    ``vocab`` is the whole vocabulary's size. ``kept`` are the forward's kept logits of ``kept_rows``
-    rows, of which row t's are at ``row_of[t]`` (int32; None: t)."""
+    ``vocab`` is the whole vocabulary's size. ``rows`` takes the first that many rows only (of
+    ``dist_rows``). ``kept`` are the forward's kept logits of as many rows as ``tokens`` has, of which
+    row t's are at ``row_of[t]`` (int32; None: t)."""
     dev = _check_head(embed, hidden, tokens, saved, entropy, grad_logp, grad_entropy)
     lib = _lib.load()
-    T, K = tokens.shape
+    all_rows, K = tokens.shape
+    T = all_rows if rows is None else rows
     Vs, d = embed.shape
     flags = 0
     dH = dW = None
@@ -354,8 +393,8 @@ def dist_backward(
         zt = saved.data_ptr()
         return lib.lp_dist_bwd(
             stream, h.data_ptr(), T, d, ldh, w.data_ptr(), Vs, int(vocab_offset), int(vocab) if vocab else Vs,
-            tokens.data_ptr(), K, softcap or 0.0, zt, zt + 4 * T * K, entropy.data_ptr(), _addr(grad_logp),
-            _addr(grad_entropy), _addr(kept), kept_rows, _addr(row_of), _addr(dH), d, _addr(dW), flags, chunk, wsp, wsn,
+            tokens.data_ptr(), K, softcap or 0.0, zt, zt + 4 * all_rows * K, entropy.data_ptr(), _addr(grad_logp),
+            _addr(grad_entropy), _addr(kept), all_rows, _addr(row_of), _addr(dH), d, _addr(dW), flags, chunk, wsp, wsn,
         )
 
     _on_device(dev, "lp_dist_bwd", call)

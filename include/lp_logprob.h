@@ -324,6 +324,21 @@ LP_API int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_
                        const void* kept, int64_t kept_rows, const int32_t* row_of, void* dH, int64_t ld_dh, void* dW,
                        int flags, int64_t token_chunk, void* workspace, size_t workspace_bytes);
 
+/*
+ * The rows of a backward that send a gradient (one of g_logp[t, :], g_entropy[t] is not zero),
+ * gathered in order; the others add nothing to dH or dW. Inputs as lp_dist_bwd's; every *_out has
+ * the input's shape (H_out rows are packed: ld = d), of which the first *count rows are written.
+ *   idx  int32 [T]: row of each gathered row (lp_dist_bwd's row_of); pos  int32 [T]: gathered row of
+ *   each row, or -1; count  int32 [1]
+ * The workspace is lp_dist_rows_workspace_bytes(T).
+ */
+LP_API size_t lp_dist_rows_workspace_bytes(int64_t T);
+LP_API int lp_dist_rows(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const int32_t* y, int64_t K,
+                        const float* zt, const float* lse, const float* entropy, const float* g_logp,
+                        const float* g_entropy, void* H_out, int32_t* y_out, float* zt_out, float* lse_out,
+                        float* entropy_out, float* g_logp_out, float* g_entropy_out, int32_t* idx, int32_t* pos,
+                        int32_t* count, void* workspace, size_t workspace_bytes);
+
 /* Scratch bytes lp_top and lp_sample_top_k need for k tokens of T rows against V vocabulary rows. */
 LP_API size_t lp_top_workspace_bytes(int64_t T, int64_t V, int k);
 

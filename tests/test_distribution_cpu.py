@@ -114,6 +114,17 @@ def test_c_entries_refuse_before_the_device(lib):
     refused(bwd(kept=fake, kept_rows=3), "kept logits")
     assert lib.lp_dist_kept_bytes(3, 300) == 3 * 304 * 2 + 224 + 3 * 16 * 4  # 16-bit rows, 256-byte step, f32 maxima
     assert lib.lp_dist_kept_bytes(0, 300) == 0
+
+    def rows(T=4, d=8, H=fake, y_out=fake, g_out=fake, ws=1 << 20):
+        return lib.lp_dist_rows(None, H, T, d, 8, fake, 2, fake, fake, fake, fake, fake, fake, y_out, fake, fake, fake, g_out,
+                                fake, fake, fake, fake, fake, ws)
+
+    refused(rows(T=0), "bad sizes")
+    refused(rows(d=12), "bad sizes")
+    refused(rows(y_out=None), "null input")
+    refused(rows(g_out=None), "null input")
+    refused(rows(H=P(4104)), "aligned")
+    assert rows(ws=1) == _lib.LP_EWORKSPACE
     for k in (0, 11, 129):
         refused(lib.lp_top(None, fake, 4, 8, 8, fake, 10, 0.0, k, None, fake, fake, fake, None, fake, 1 << 20), "k=")
     refused(lib.lp_top(None, fake, 4, 8, 8, fake, 10, 0.0, 2, fake, fake, fake, fake, None, fake, 1 << 20), "token_logps")

@@ -132,7 +132,8 @@ def test_gradient_against_differences(cuda_device):
 
 
 @pytest.mark.parametrize("keep", [True, False])
-def test_rows_without_gradient_are_left_out(cuda_device, monkeypatch, keep):
+@pytest.mark.parametrize("send", ["both", "logps", "entropy"])
+def test_rows_without_gradient_are_left_out(cuda_device, monkeypatch, keep, send):
     from gemma4_posttrain_jax_b200 import distribution, token_logps_and_entropy
 
     T, V, d = 300, 1036, 64
@@ -142,12 +143,17 @@ def test_rows_without_gradient_are_left_out(cuda_device, monkeypatch, keep):
     off = torch.rand((T,), generator=gen, device=cuda_device) < 0.4
     g[off], ge[off] = 0.0, 0.0
     ge[3], g[3] = 0.0, torch.tensor([0.0, 1.0], device=cuda_device)  # one of several gradients is enough
+    if send == "logps":
+        ge.zero_()
+    elif send == "entropy":
+        g.zero_()
     W.requires_grad_(True), H.requires_grad_(True)
     results = []
     for least in (float("inf"), 0.0):
         monkeypatch.setattr(distribution, "_SKIP_MIN_FLOPS", least)
         logps, entropy = token_logps_and_entropy(W, H, y, softcap=30.0, keep_logits=keep)
-        results.append(torch.autograd.grad([logps, entropy], [H, W], [g, ge]))
+        sent = {"both": ([logps, entropy], [g, ge]), "logps": ([logps], [g]), "entropy": ([entropy], [ge])}[send]
+        results.append(torch.autograd.grad(sent[0], [H, W], sent[1]))
     dH, dW, bH, bW = Reference(W.detach(), H.detach(), 30.0, kept=keep).grads(y, g, ge)
     for got_H, got_W in results:
         within(got_H, dH, bH, "d hidden")
@@ -184,8 +190,8 @@ def test_shards_merge_to_the_whole(cuda_device, V, P, keep):
     within(logp, picked, ref.logp_bound(picked), "logps")
     within(entropy, ref.entropy, ref.entropy_bound(), "entropy")
     grads = [
-        ops.dist_backward(w, H, y, 30.0, saved, entropy, g, ge, vocab_offset=p * vs, vocab=V, dh_dtype=torch.float32, kept=kept[p],
-                          kept_rows=T)
+        ops.dist_backward(w, 30.0, H, y, saved, entropy, g, ge, vocab_offset=p * vs, vocab=V, dh_dtype=torch.float32,
+                          kept=kept[p])
         for p, w in enumerate(shards)
     ]
     dH, dW, bH, bW = ref.grads(y, g, ge)
