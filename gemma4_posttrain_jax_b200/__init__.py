@@ -9,7 +9,12 @@ with the entropy and the most likely tokens (``distribution.py``). The kernels l
 ``liblp_b200.so`` (C ABI: ``include/lp_logprob.h``); this package is the host side.
 """
 
-from .distribution import TopTokenLogps, token_logps_and_entropy, top_token_logps  # noqa: F401
+from .distribution import (  # noqa: F401
+    TopTokenLogps,
+    completion_logps_and_entropy,
+    token_logps_and_entropy,
+    top_token_logps,
+)
 from .logprob_protocol import CUDA_LOGPROB_PROTOCOL, logprob_run_metadata, validate_logprob_resume  # noqa: F401
 from .losses import completion_logps, per_token_logps, sft_token_logps  # noqa: F401
 from .sampler import lm_head_logits, sample_token, sample_top_k  # noqa: F401
@@ -20,6 +25,7 @@ __all__ = [
     "TopTokenLogps",
     "VocabMesh",
     "completion_logps",
+    "completion_logps_and_entropy",
     "lm_head_logits",
     "logprob_run_metadata",
     "make_mesh",

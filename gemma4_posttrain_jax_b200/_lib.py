@@ -96,7 +96,7 @@ _SIG = {
     ),
     "lp_sample_top_k": (
         ctypes.c_int,
-        [_P, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, ctypes.c_int, _P, ctypes.c_float, ctypes.c_float, _P, _P, _P,
+        [_P, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_float, ctypes.c_int, _P, ctypes.c_double, ctypes.c_double, _P, _P, _P,
          ctypes.c_size_t],
     ),
     "lp_compact_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),

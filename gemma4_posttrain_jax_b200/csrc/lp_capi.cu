@@ -1693,11 +1693,11 @@ int lp_top(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const
 }
 
 int lp_sample_top_k(void* stream, const void* H, int64_t B, int64_t d, int64_t ldh, const void* W, int64_t V,
-                    float softcap, int k, const float* uniform, float temperature, float top_p, int32_t* token,
+                    float softcap, int k, const float* uniform, double temperature, double top_p, int32_t* token,
                     float* logp, void* workspace, size_t workspace_bytes) {
   if (int rc = check_top(H, B, d, ldh, W, V, k)) return rc;
-  if (!(temperature > 0.f) || temperature > 3.4e38f) return fail(LP_EINVAL, "temperature must be finite and positive");
-  if (!(top_p > 0.f && top_p <= 1.f)) return fail(LP_EINVAL, "top_p must be in (0, 1]");
+  if (!(temperature > 0.) || temperature > 1.7e308) return fail(LP_EINVAL, "temperature must be finite and positive");
+  if (!(top_p > 0. && top_p <= 1.)) return fail(LP_EINVAL, "top_p must be in (0, 1]");
   if (B == 0) return LP_OK;
   if (uniform == nullptr || token == nullptr || logp == nullptr) return fail(LP_EINVAL, "null uniform, token or logp");
   TopParams P{};

@@ -489,7 +489,7 @@ struct TopParams {
   float* entropy;         // top: [T]
   float* token_logps;     // top: [T] (with tokens)
   const float* uniform;   // sample: [T] in [0, 1)
-  float temperature, top_p;
+  double temperature, top_p;
   int32_t* sampled;  // sample: [T]
 };
 
@@ -855,7 +855,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
     }
   } else {
     __shared__ double weight_s[kTopMax];
-    if (tid < P.k) weight_s[tid] = exp((best_z[tid] - best_z[0]) / (double)P.temperature);
+    if (tid < P.k) weight_s[tid] = exp((best_z[tid] - best_z[0]) / P.temperature);
     __syncthreads();
     if (warp != 0) return;
     // Inverse of the cumulative distribution of the kept prefix, in f64: kTopMax / 32 consecutive
@@ -878,7 +878,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
     }
     const double before = incl - run;
     const double total = __shfl_sync(0xffffffffu, incl, 31);
-    const double limit = (double)P.top_p * total;
+    const double limit = P.top_p * total;
     int kept = 0;
     double mass = 0.;  // of the kept prefix: the largest kept cumulative sum
 #pragma unroll

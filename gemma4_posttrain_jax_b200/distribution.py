@@ -3,13 +3,15 @@
 ``token_logps_and_entropy`` is ``per_token_logps`` for what a loss takes besides the sampled token's
 log-probability: any number of given tokens per position (a distillation or KL term over a
 teacher's alternatives) and the entropy of the policy (an entropy bonus), with the gradients of
-both. ``top_token_logps`` gives such alternatives: the k most likely tokens of each position.
+both; ``completion_logps_and_entropy`` is its caller for completions, as ``completion_logps`` is
+``per_token_logps``'. ``top_token_logps`` gives such alternatives: the k most likely tokens of each position.
 Neither writes a ``[..., vocab]`` array of probabilities. The reference has no counterpart.
 """
 
 from __future__ import annotations
 
 import math
+import operator
 import weakref
 from typing import NamedTuple
 
@@ -17,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .losses import _SKIP_ZERO_GRAD_MIN_FRACTION, _check_device, _validate_softcap
+from .losses import _SKIP_ZERO_GRAD_MIN_FRACTION, _check_device, _check_num_valid, _debug_checks, _validate_softcap
 from .phase_timer import phase
 from .sharding import VocabMesh, all_gather_stats, all_reduce_sum, vocab_offset
 
@@ -136,10 +138,10 @@ _eager_graphs: weakref.WeakSet = weakref.WeakSet()
 # size of the backward's own dZ scratch.
 _KEPT_MAX_BYTES = 4 << 30
 
-# Rows without a gradient add nothing, and a backward of at least this much work (about 6 ms)
+# Rows without a gradient add nothing, and a backward of at least this much work (about 3 ms)
 # leaves them out. Below it, the wait for their number and whole tiles of 256 rows that a few rows
 # fewer do not save cost what a tenth of the rows would.
-_SKIP_MIN_FLOPS = 1e13
+_SKIP_MIN_FLOPS = 5e12
 
 
 def token_logps_and_entropy(
@@ -206,6 +208,70 @@ def token_logps_and_entropy(
     return logps, entropy
 
 
+class _ValidSlots(torch.autograd.Function):
+    """The rows of hidden [B, S, d] and ids [B, N] at the valid slots of mask [B, N], in slot order."""
+
+    @staticmethod
+    def forward(ctx, hidden, ids, mask, first, num_valid):
+        rows, tokens, idx, pos, count = ops.compact(mask, hidden, ids, row_offset=first)
+        n = int(count.item()) if num_valid is None else int(num_valid)
+        if num_valid is None:
+            _check_device(hidden.device, "completion_logps_and_entropy")
+        elif _debug_checks():
+            _check_num_valid(count, n)
+        ctx.save_for_backward(pos)
+        ctx.meta = (tuple(hidden.shape), hidden.dtype, first, mask.shape[1])
+        tokens, idx = tokens[:n], idx[:n]
+        ctx.mark_non_differentiable(tokens, idx)
+        return rows[:n], tokens, idx
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _tokens, _idx):
+        (pos,) = ctx.saved_tensors
+        shape, dtype, first, width = ctx.meta
+        out = torch.zeros(shape, dtype=dtype, device=g.device)
+        ops.scatter_rows(g.contiguous(), pos, out[:, first : first + width])
+        return out, None, None, None, None
+
+
+def completion_logps_and_entropy(
+    embed_tokens: torch.Tensor,
+    hidden: torch.Tensor,
+    completion_ids: torch.Tensor,
+    completion_mask: torch.Tensor,
+    *,
+    prompt_width: int,
+    softcap: float | None,
+    num_valid: int | None = None,
+    **options,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``completion_logps`` with the entropy: (logps [B, N], entropy [B, N]) of the completion tokens of
+    hidden [B, P + N, d], differentiable, computed at the valid slots only and 0 elsewhere. ``num_valid``
+    is ``completion_logps``'; ``options`` are those of ``token_logps_and_entropy``.
+    """
+    if hidden.ndim != 3 or completion_ids.ndim != 2 or completion_mask.shape != completion_ids.shape:
+        raise ValueError("hidden must be [B, S, d] and completion ids / mask [B, N]")
+    if completion_ids.shape[0] != hidden.shape[0]:
+        raise ValueError(f"hidden has {hidden.shape[0]} sequences, completion ids {completion_ids.shape[0]}")
+    if prompt_width < 1 or prompt_width - 1 + completion_ids.shape[1] > hidden.shape[1]:
+        raise ValueError("prompt_width and completion width do not fit the hidden sequence")
+    _check_embed(embed_tokens, hidden)
+    _validate_softcap(softcap)
+    rows = hidden
+    if hidden.stride(-1) != 1 or hidden.stride(0) % 8 or hidden.stride(1) % 8 or hidden.data_ptr() % 16:
+        rows = hidden.contiguous()
+    rows, tokens, idx = _ValidSlots.apply(rows, _as_int32(completion_ids), completion_mask, prompt_width - 1, num_valid)
+    logps, entropy = token_logps_and_entropy(embed_tokens, rows, tokens, softcap=softcap, **options)
+    slots = idx.long()
+
+    def scattered(values):
+        out = torch.zeros(completion_ids.numel(), dtype=values.dtype, device=values.device)
+        return out.index_put((slots,), values).view(completion_ids.shape)
+
+    return scattered(logps), scattered(entropy)
+
+
 def top_token_logps(
     embed_tokens: torch.Tensor,
     hidden: torch.Tensor,
@@ -223,6 +289,7 @@ def top_token_logps(
     """
     _check_embed(embed_tokens, hidden)
     _validate_softcap(softcap)
+    k = operator.index(k)
     if not 1 <= k <= min(_lib.LP_TOP_MAX, embed_tokens.shape[0]):
         raise ValueError(f"k must be between 1 and min({_lib.LP_TOP_MAX}, {embed_tokens.shape[0]}), got {k}")
     prefix = tuple(hidden.shape[:-1])
@@ -232,7 +299,6 @@ def top_token_logps(
             raise ValueError(f"hidden prefix {prefix} does not match tokens {tuple(tokens.shape)}")
         tokens = _as_int32(tokens)
         token_logps = torch.empty(prefix, dtype=torch.float32, device=hidden.device)
-    k = int(k)
     ids = torch.empty((*prefix, k), dtype=torch.int32, device=hidden.device)
     logps = torch.empty((*prefix, k), dtype=torch.float32, device=hidden.device)
     entropy = torch.empty(prefix, dtype=torch.float32, device=hidden.device)

@@ -15,6 +15,7 @@ same).
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 
@@ -119,6 +120,7 @@ def sample_top_k(
     _validate_softcap(softcap)
     if not (math.isfinite(temperature) and temperature > 0):
         raise ValueError("temperature must be finite and positive (sample_token decodes greedily)")
+    top_k = operator.index(top_k)
     if not 1 <= top_k <= min(_lib.LP_TOP_MAX, embed_tokens.shape[0]):
         raise ValueError(f"top_k must be between 1 and min({_lib.LP_TOP_MAX}, {embed_tokens.shape[0]}), got {top_k}")
     if not 0.0 < top_p <= 1.0:
@@ -127,6 +129,6 @@ def sample_top_k(
         raise ValueError(f"uniform must be float32 [{hidden.shape[0]}], got {uniform.dtype} {tuple(uniform.shape)}")
     with torch.no_grad():
         return ops.sample_top_k(
-            embed_tokens, hidden, softcap, uniform.contiguous(), temperature=float(temperature), top_k=int(top_k),
+            embed_tokens, hidden, softcap, uniform.contiguous(), temperature=float(temperature), top_k=top_k,
             top_p=float(top_p),
         )

@@ -361,11 +361,12 @@ LP_API int lp_top(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh
  * its cumulative distribution in descending order: with w_j = exp((z_j - z_0) / temperature) over
  * lp_top's k tokens, token j is kept while w_0 + .. + w_(j-1) < top_p * sum w (the first always),
  * and the drawn one is the first whose kept cumulative weight exceeds uniform * kept weight.
- *   uniform  f32 [B] in [0, 1)          temperature > 0, 0 < top_p <= 1
+ *   uniform  f32 [B] in [0, 1) (what lies outside draws the first or the last kept token)
+ *   temperature finite and > 0, 0 < top_p <= 1
  *   token    int32 [B]; logp f32 [B]: its log-probability under the unfiltered, untempered policy
  */
 LP_API int lp_sample_top_k(void* stream, const void* H, int64_t B, int64_t d, int64_t ldh, const void* W, int64_t V,
-                           float softcap, int k, const float* uniform, float temperature, float top_p, int32_t* token,
+                           float softcap, int k, const float* uniform, double temperature, double top_p, int32_t* token,
                            float* logp, void* workspace, size_t workspace_bytes);
 
 /* Scratch bytes lp_compact needs for B * N response slots. */

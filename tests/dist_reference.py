@@ -91,7 +91,7 @@ class Reference:
         best = self.z.gather(1, ids)
         w = ((best - best[:, :1]) / temperature).exp()
         upto = w.cumsum(-1)
-        keep = upto - w < float(torch.tensor(top_p, dtype=torch.float32)) * upto[:, -1:]
+        keep = upto - w < top_p * upto[:, -1:]
         keep[:, 0] = True
         kept = torch.where(keep, w, 0.0).cumsum(-1)
         place = (kept <= uniform.double()[:, None] * kept[:, -1:]).sum(-1)

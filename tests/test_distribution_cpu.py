@@ -7,7 +7,14 @@ import ctypes
 import pytest
 import torch
 
-from gemma4_posttrain_jax_b200 import _lib, build, sample_top_k, token_logps_and_entropy, top_token_logps
+from gemma4_posttrain_jax_b200 import (
+    _lib,
+    build,
+    completion_logps_and_entropy,
+    sample_top_k,
+    token_logps_and_entropy,
+    top_token_logps,
+)
 
 
 @pytest.fixture(scope="module")
@@ -43,6 +50,25 @@ def test_logps_refusals(change, message):
     embed, hidden, tokens = (args.pop(name) for name in ("embed_tokens", "hidden", "tokens"))
     with pytest.raises(ValueError, match=message):
         token_logps_and_entropy(embed, hidden, tokens, **args)
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"hidden": H[0]}, r"\[B, S, d\]"),
+    ({"ids": torch.zeros((2, 1), dtype=torch.int64)}, "completion ids"),
+    ({"hidden": torch.zeros((3, 3, 16), dtype=torch.bfloat16)}, "sequences"),
+    ({"prompt_width": 0}, "prompt_width"),
+    ({"prompt_width": 3}, "prompt_width"),
+    ({"softcap": -1.0}, "softcap"),
+    ({"embed_tokens": W[:, :8]}, "incompatible"),
+    ({"ids": torch.zeros((2, 2))}, "integers"),
+    ({}, "CUDA tensors"),
+])  # fmt: skip
+def test_completion_refusals(change, message):
+    args = {"embed_tokens": W, "hidden": H, "ids": torch.zeros((2, 2), dtype=torch.int64),
+            "mask": torch.ones((2, 2), dtype=torch.bool), "prompt_width": 2, "softcap": 30.0} | change
+    first = [args.pop(name) for name in ("embed_tokens", "hidden", "ids", "mask")]
+    with pytest.raises(ValueError, match=message):
+        completion_logps_and_entropy(*first, **args)
 
 
 @pytest.mark.parametrize("args,tokens,message", [

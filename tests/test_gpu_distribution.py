@@ -98,6 +98,138 @@ def test_one_gradient_alone_and_row_chunks(cuda_device, frozen, K, keep):
     within(got, dH if frozen == "embed" else dW, bH if frozen == "embed" else bW, "gradient")
 
 
+def test_entropy_alone_and_a_graph_used_twice(cuda_device):
+    from gemma4_posttrain_jax_b200 import token_logps_and_entropy
+
+    T, V, d = 45, 1036, 64
+    W, H, gen = _inputs(cuda_device, T, V, d)
+    ge = torch.randn((T,), generator=gen, device=cuda_device)
+    none = torch.empty((T, 0), dtype=torch.int64, device=cuda_device)
+    W.requires_grad_(True), H.requires_grad_(True)
+    _, entropy = token_logps_and_entropy(W, H, none, softcap=30.0)
+    first = torch.autograd.grad([entropy], [H, W], [ge], retain_graph=True)
+    dH, dW, bH, bW = Reference(W.detach(), H.detach(), 30.0, kept=True).grads(none, None, ge)
+    within(first[0], dH, bH, "d hidden")
+    within(first[1], dW, bW, "d embedding")
+    again = torch.autograd.grad([entropy], [H, W], [ge], retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    with torch.no_grad():
+        W.mul_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad([entropy], [H, W], [ge])
+
+
+@pytest.mark.parametrize("group", [1, 2])
+def test_either_cta_group(cuda_device, group):
+    """Every product as single CTAs and as pairs, whatever the sizes would choose."""
+    from gemma4_posttrain_jax_b200 import _lib, token_logps_and_entropy, top_token_logps
+
+    try:
+        _lib.set_cta_group(group)
+        for T, V in ((5, 300), (130, 4099), (257, 9001)):
+            for keep in (True, False):
+                W, H, gen = _inputs(cuda_device, T, V, 72)
+                y = _tokens(gen, cuda_device, T, V, 2)
+                g, ge = torch.randn((T, 2), generator=gen, device=cuda_device), torch.randn((T,), generator=gen, device=cuda_device)
+                W.requires_grad_(True), H.requires_grad_(True)
+                logps, entropy = token_logps_and_entropy(W, H, y, softcap=30.0, keep_logits=keep)
+                got = torch.autograd.grad([logps, entropy], [H, W], [g, ge])
+                ref = Reference(W.detach(), H.detach(), 30.0, kept=keep)
+                dH, dW, bH, bW = ref.grads(y, g, ge)
+                within(got[0], dH, bH, "d hidden")
+                within(got[1], dW, bW, "d embedding")
+            top = top_token_logps(W, H, 30.0, 6)
+            assert torch.equal(top.ids.long(), ref.order(6))
+            within(top.entropy, ref.entropy, ref.entropy_bound(), "entropy")
+    finally:
+        _lib.set_cta_group(0)
+
+
+class _OneOfMany:
+    """A vocabulary mesh of ``size`` ranks, this one ``rank``; the test plays the collectives."""
+
+    axis_names = ("d",)
+
+    def __init__(self, size, rank):
+        self.size, self.rank = size, rank
+
+
+def test_vocabulary_mesh(cuda_device, monkeypatch):
+    """Every rank's call in turn, with the all-gather played from all shards' statistics: each rank has
+    the whole vocabulary's results and its own rows of dW, and the ranks' dH add up."""
+    from gemma4_posttrain_jax_b200 import distribution, ops, token_logps_and_entropy
+
+    T, V, d, K, P = 67, 1040, 128, 4, 4
+    W, H, gen = _inputs(cuda_device, T, V, d)
+    y = _tokens(gen, cuda_device, T, V, K)
+    g, ge = torch.randn((T, K), generator=gen, device=cuda_device), torch.randn((T,), generator=gen, device=cuda_device)
+    vs = V // P
+    tokens = y.to(torch.int32).contiguous()
+
+    def gathered(own, mesh):
+        parts = [ops.dist_forward_shard(W[p * vs : (p + 1) * vs], H, tokens, 30.0, p * vs) for p in range(P)]
+        parts = torch.stack([torch.cat([s.reshape(-1), z.reshape(-1)]) for s, z in parts])
+        assert torch.equal(parts[mesh.rank], own)
+        return parts
+
+    monkeypatch.setattr(distribution, "all_gather_stats", gathered)
+    monkeypatch.setattr(distribution, "all_reduce_sum", lambda t, mesh: t)  # leaves the rank's partial sum
+    monkeypatch.setattr(distribution, "_SKIP_MIN_FLOPS", 0.0)
+    off = torch.arange(T, device=cuda_device) % 3 == 0
+    g[off], ge[off] = 0.0, 0.0
+    ref = Reference(W, H, 30.0, kept=True)
+    dH, dW, bH, bW = ref.grads(y, g, ge)
+    total = torch.zeros_like(dH)
+    for rank in range(P):
+        shard = W[rank * vs : (rank + 1) * vs].clone().requires_grad_(True)
+        leaf = H.clone().requires_grad_(True)
+        logps, entropy = token_logps_and_entropy(shard, leaf, y, softcap=30.0, mesh=_OneOfMany(P, rank), dh_reduce_f32=True)
+        picked = ref.picked(y)
+        within(logps, picked, ref.logp_bound(picked), "logps")
+        within(entropy, ref.entropy, ref.entropy_bound(), "entropy")
+        got_H, got_W = torch.autograd.grad([logps, entropy], [leaf, shard], [g, ge])
+        within(got_W, dW[rank * vs : (rank + 1) * vs], bW[rank * vs : (rank + 1) * vs], "d embedding")
+        total += got_H.double()
+    # each rank rounded its partial sum to bf16 once: 2^-8 of sizes that the bound's first term covers
+    within(total, dH, P * bH, "d hidden")
+
+
+def test_completions(cuda_device):
+    from gemma4_posttrain_jax_b200 import completion_logps_and_entropy
+
+    B, S, N, V, d, prompt = 5, 40, 23, 1036, 64, 12
+    W, H, gen = _inputs(cuda_device, B * S, V, d)
+    H = H.reshape(B, S, d)
+    ids = torch.randint(V, (B, N), generator=gen, device=cuda_device)
+    mask = torch.arange(N, device=cuda_device) < torch.tensor([23, 7, 0, 1, 15], device=cuda_device)[:, None]
+    g, ge = torch.randn((B, N), generator=gen, device=cuda_device), torch.randn((B, N), generator=gen, device=cuda_device)
+    W.requires_grad_(True)
+    flat = H[:, prompt - 1 : prompt - 1 + N].reshape(-1, d)
+    on = mask.reshape(-1)
+    ref = Reference(W.detach(), flat[on], 30.0, kept=True)
+    y = ids.reshape(-1)[on][:, None]
+    dH, dW, bH, bW = ref.grads(y, g.reshape(-1)[on][:, None], ge.reshape(-1)[on])
+    wide = torch.nn.functional.pad(H, (0, 4))[..., :d]  # rows that have to be copied first
+    for hidden, count in ((H.clone(), None), (H.clone(), int(mask.sum())), (wide.detach(), None)):
+        hidden.requires_grad_(True)
+        logps, entropy = completion_logps_and_entropy(W, hidden, ids, mask, prompt_width=prompt, softcap=30.0, num_valid=count)
+        assert logps.shape == entropy.shape == (B, N)
+        assert (logps[~mask] == 0).all() and (entropy[~mask] == 0).all()
+        picked = ref.picked(y)
+        within(logps[mask][:, None], picked, ref.logp_bound(picked), "logps")
+        within(entropy[mask], ref.entropy, ref.entropy_bound(), "entropy")
+        got_H, got_W = torch.autograd.grad([logps, entropy], [hidden, W], [g, ge])
+        rows = got_H[:, prompt - 1 : prompt - 1 + N].reshape(-1, d)
+        within(rows[on], dH, bH, "d hidden")
+        assert (rows[~on] == 0).all() and got_H.abs().sum() == rows.abs().sum()
+        within(got_W, dW, bW, "d embedding")
+    # no completion token at all
+    logps, entropy = completion_logps_and_entropy(W, H, ids, torch.zeros_like(mask), prompt_width=prompt, softcap=30.0)
+    assert (logps == 0).all() and (entropy == 0).all()
+    (got_W,) = torch.autograd.grad([logps.sum() + entropy.sum()], [W])
+    assert (got_W == 0).all()
+
+
 def test_gradient_against_differences(cuda_device):
     """Central differences of the operator itself, along directions that bf16 holds exactly: hidden
     entries are multiples of 2^-2 below 4 and the step is 2^-6, so h +- step needs 8 bits."""
@@ -269,6 +401,8 @@ TOP_SHAPES = [
     (129, 70001, 64, 64, 50.0),
     (3, 262144, 256, 40, 30.0),
     (140, 33000, 72, 100, None),
+    (2, 1600000, 8, 3, None),  # more keys than shared memory holds
+    (3, 5000, 6000, 7, 30.0),  # wide rows
 ]
 
 
