@@ -13,20 +13,8 @@
 namespace lpk {
 
 struct DistAcc {
-  float m, s, a;  // base 2: max, sum 2^(z-m), sum 2^(z-m) (z-m); s == 0: nothing yet
+  float m, s, a;  // base 2: max, sum 2^(z-m), sum 2^(z-m) (z-m)
 };
-
-__device__ __forceinline__ DistAcc dist_merge(const DistAcc& x, const DistAcc& y) {
-  if (y.s == 0.f) return x;
-  if (x.s == 0.f) return y;
-  DistAcc r;
-  r.m = fmaxf(x.m, y.m);
-  const float dx = x.m - r.m, dy = y.m - r.m;
-  const float ex = exp2f(dx), ey = exp2f(dy);
-  r.s = x.s * ex + y.s * ey;
-  r.a = fmaf(x.s, dx, x.a) * ex + fmaf(y.s, dy, y.a) * ey;
-  return r;
-}
 
 __device__ __forceinline__ float dist_lse(const DistAcc& x) { return x.m * kLn2 + logf(x.s); }
 __device__ __forceinline__ float dist_entropy(const DistAcc& x) { return logf(x.s) - kLn2 * (x.a / x.s); }
@@ -45,7 +33,9 @@ __device__ __forceinline__ float softcap_exact(float x, float cap) { return cap 
 __device__ __forceinline__ float warp_dot(const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w,
                                           long long d, int lane) {
   float acc0 = 0.f, acc1 = 0.f;
-  for (long long i = lane; i < d / 8; i += 32) {
+  const int n = (int)(d / 8);
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) {
     const uint4 a = __ldg(reinterpret_cast<const uint4*>(h) + i);
     const uint4 b = __ldg(reinterpret_cast<const uint4*>(w) + i);
     const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
@@ -140,42 +130,60 @@ __device__ __forceinline__ double warp_dot_exact(const __nv_bfloat16* __restrict
 constexpr int kDistThreads = 256;
 
 template <int R>
-__global__ void __launch_bounds__(kDistThreads)
+__global__ void __launch_bounds__(kDistThreads, 4)
     dist_finalize_kernel(const float2* __restrict__ part, const float* __restrict__ part_a, int n_parts, int T,
                          const __nv_bfloat16* __restrict__ H, long long ldh, const __nv_bfloat16* __restrict__ W,
                          long long d, long long Vs, long long v_off, const int32_t* __restrict__ y, int K, float cap,
                          float* __restrict__ stats, float* __restrict__ zt, float* __restrict__ lse,
                          float* __restrict__ entropy, float* __restrict__ logp) {
-  __shared__ DistAcc acc_s[kDistThreads];
+  constexpr int kWarps = kDistThreads / 32;
+  __shared__ float m_s[kWarps][R], s_s[kWarps][R], a_s[kWarps][R];
   __shared__ float lse_s[R];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = blockIdx.x * R;
   const int r = threadIdx.x % R;
-  const int t = t0 + r;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = min(t0 + r, T - 1);
   const int rows = min(R, T - t0);
-  // the tokens' rows of W come from all over it: ask for them before the partials are merged
-  for (int i = threadIdx.x; i < rows * K; i += kDistThreads) {
-    const long long v = (long long)y[(size_t)(t0 + i / K) * K + i % K] - v_off;
-    if (v >= 0 && v < Vs) prefetch_l2_bulk(W + (size_t)v * d, (uint32_t)d * 2);
-  }
-  DistAcc acc{-INFINITY, 0.f, 0.f};
-  if (t < T) {
-    for (int g = threadIdx.x / R; g < n_parts; g += kDistThreads / R) {
-      const float2 p = part[(size_t)g * T + t];
-      acc = dist_merge(acc, DistAcc{p.x, p.y, part_a[(size_t)g * T + t]});
-    }
-  }
-  acc_s[threadIdx.x] = acc;
+  // the row's maximum, then the sums at it: no chain of rescaled pairs, so the loads pass together
+  float m = -INFINITY;
+#pragma unroll 8
+  for (int g = threadIdx.x / R; g < n_parts; g += kDistThreads / R) m = fmaxf(m, part[(size_t)g * T + t].x);
+#pragma unroll
+  for (int o = R; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane < R) m_s[warp][lane] = m;
   __syncthreads();
 #pragma unroll
-  for (int o = kDistThreads / 2; o >= R; o >>= 1) {
-    if ((int)threadIdx.x < o) acc_s[threadIdx.x] = dist_merge(acc_s[threadIdx.x], acc_s[threadIdx.x + o]);
-    __syncthreads();
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, m_s[w][r]);
+  float s = 0.f, a = 0.f;
+#pragma unroll 8
+  for (int g = threadIdx.x / R; g < n_parts; g += kDistThreads / R) {
+    const float2 p = part[(size_t)g * T + t];
+    const float pa = part_a[(size_t)g * T + t];
+    if (p.y != 0.f) {  // 0: a partial that saw padding only
+      const float dm = p.x - m, e = exp2f(dm);
+      s = fmaf(p.y, e, s);
+      a = fmaf(fmaf(p.y, dm, pa), e, a);
+    }
   }
-  if (threadIdx.x < R && t < T) {
-    acc = acc_s[threadIdx.x];
+#pragma unroll
+  for (int o = R; o < 32; o <<= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+  }
+  if (lane < R) {
+    s_s[warp][lane] = s;
+    a_s[warp][lane] = a;
+  }
+  __syncthreads();
+  if (threadIdx.x < rows) {
+    DistAcc acc{m, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      acc.s += s_s[w][r];
+      acc.a += a_s[w][r];
+    }
     const float l = dist_lse(acc);
-    lse_s[threadIdx.x] = l;
+    lse_s[r] = l;
     if (stats != nullptr) {
       stats[t] = acc.m * kLn2;
       stats[(size_t)T + t] = acc.s;
@@ -548,7 +556,6 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
 
   // ---- loads: the row's partials (up to four per thread at once), hidden state and keys
   const long long token = !SAMPLE && P.tokens != nullptr ? P.tokens[t] : -1;
-  if (tid == 0 && token >= 0 && token < P.V) prefetch_l2_bulk(P.W + (size_t)token * P.d, (uint32_t)P.d * 2);
   constexpr int PN = 4;
   float2 pv[PN];
   float pa[PN];
@@ -804,10 +811,6 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
     }
     for (int c = max(0, b0 - my_at); c < min(cols, b0 + kTopBatch - my_at); ++c) cand_id[have + my_at + c - b0] = first + c;
     __syncthreads();
-    // The candidates' rows of W come from all over it: ask for all of them at once, so that their
-    // latencies (HBM and address translation) pass together and not once per round of the warps.
-    for (int i = have + tid; i < count; i += kTopThreads)
-      prefetch_l2_bulk(P.W + (size_t)cand_id[i] * P.d, (uint32_t)P.d * 2);
 #pragma unroll 1
     for (int i = have + warp; i < count; i += kWarps) {
       const double z = warp_dot_exact(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);
