@@ -56,14 +56,14 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, embed, hidden, tokens, shape, softcap, mesh, token_chunk, dh_reduce_f32, skip_zero_grad, keep_logits):
         T, K = tokens.shape
-        h = hidden.reshape(T, hidden.shape[-1])
-        logp = torch.empty(shape, dtype=torch.float32, device=hidden.device)
-        entropy = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=hidden.device)
-        kept = None
-        if (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]) and keep_logits is not False:
-            nbytes = ops.dist_kept_bytes(T, embed.shape[0])
-            if keep_logits or nbytes <= _KEPT_MAX_BYTES:
-                kept = torch.empty((nbytes,), dtype=torch.uint8, device=hidden.device)
+        dev = hidden.device
+        h = hidden if hidden.ndim == 2 else hidden.reshape(T, hidden.shape[-1])
+        logp = torch.empty(shape, dtype=torch.float32, device=dev)
+        entropy = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
+        most = 0  # bytes of kept logits
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            most = _KEPT_MAX_BYTES if keep_logits is None else (math.inf if keep_logits else 0)
+        saved, kept = ops.dist_saved(T, K, embed.shape[0], most, dev)
         P = mesh.size if mesh is not None else 1
         off = 0
         if P > 1:
@@ -71,64 +71,72 @@ class _TokenLogpsAndEntropy(torch.autograd.Function):
             stats, zt = ops.dist_forward_shard(embed, h, tokens, softcap, off, kept)
             with phase("stats_all_gather"):
                 both = all_gather_stats(torch.cat([stats.reshape(-1), zt.reshape(-1)]), mesh)
-            saved = ops.dist_combine(
+            ops.dist_combine(
                 both[:, : 3 * T].reshape(P, 3, T), both[:, 3 * T :].reshape(P, T, K), tokens, embed.shape[0] * P, logp,
-                entropy,
+                entropy, saved,
             )
         else:
-            saved = ops.dist_forward(embed, h, tokens, softcap, logp, entropy, kept)
-        ctx.save_for_backward(embed, hidden, tokens, saved, entropy, kept)
+            ops.dist_forward(embed, h, tokens, softcap, logp, entropy, saved, kept)
+        ctx.save_for_backward(embed, hidden, tokens, saved, entropy)
         ctx.meta = (softcap, mesh, P, off, token_chunk, dh_reduce_f32, skip_zero_grad)
         ctx.set_materialize_grads(False)
         return logp, entropy
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g, ge):
-        need_dw, need_dh = ctx.needs_input_grad[:2]
-        none = (None,) * 8
-        if (g is None and ge is None) or not (need_dw or need_dh):
-            return None, None, *none
-        embed, hidden, tokens, saved, entropy, kept = ctx.saved_tensors
-        softcap, mesh, P, off, token_chunk, dh_reduce_f32, skip_zero_grad = ctx.meta
-        T, K = tokens.shape
-        d = hidden.shape[-1]
-        if T == 0:
+        if not torch.is_grad_enabled():
+            return _dist_gradients(ctx, g, ge)
+        # A graph of the backward itself is asked for. once_differentiable lets its results refuse a
+        # second derivative, if an incoming gradient takes part in the graph: these do, here.
+        return _once(ctx, *(None if x is None else x.detach().requires_grad_() for x in (g, ge)))
+
+
+def _dist_gradients(ctx, g, ge):
+    need_dw, need_dh = ctx.needs_input_grad[:2]
+    none = (None,) * 8
+    if (g is None and ge is None) or not (need_dw or need_dh):
+        return None, None, *none
+    embed, hidden, tokens, saved, entropy = ctx.saved_tensors
+    softcap, mesh, P, off, token_chunk, dh_reduce_f32, skip_zero_grad = ctx.meta
+    T, K = tokens.shape
+    d = hidden.shape[-1]
+    if T == 0:
+        return (torch.zeros_like(embed) if need_dw else None), (torch.zeros_like(hidden) if need_dh else None), *none
+    g = None if g is None else g.contiguous()
+    ge = None if ge is None else ge.contiguous()
+    args = (hidden if hidden.ndim == 2 else hidden.reshape(T, d), tokens, saved, entropy, g, ge)
+    rows = pos = row_of = None
+    if (
+        skip_zero_grad
+        and 6.0 * T * d * embed.shape[0] >= _SKIP_MIN_FLOPS
+        and not torch.cuda.is_current_stream_capturing()
+    ):
+        idx, where, count, gathered = ops.dist_rows(*args)
+        m = int(count.item())
+        _check_device(hidden.device, "token_logps_and_entropy backward")  # the host has waited anyway
+        if m == 0:
             return (torch.zeros_like(embed) if need_dw else None), (torch.zeros_like(hidden) if need_dh else None), *none
-        g = None if g is None else g.contiguous()
-        ge = None if ge is None else ge.contiguous()
-        args = (hidden.reshape(T, d), tokens, saved, entropy, g, ge)
-        rows = pos = row_of = None
-        if (
-            skip_zero_grad
-            and 6.0 * T * d * embed.shape[0] >= _SKIP_MIN_FLOPS
-            and not torch.cuda.is_current_stream_capturing()
-        ):
-            idx, where, count, gathered = ops.dist_rows(*args)
-            m = int(count.item())
-            _check_device(hidden.device, "token_logps_and_entropy backward")  # the host has waited anyway
-            if m == 0:
-                return (
-                    (torch.zeros_like(embed) if need_dw else None), (torch.zeros_like(hidden) if need_dh else None), *none
-                )
-            if T - m >= _SKIP_ZERO_GRAD_MIN_FRACTION * T:
-                args, rows, pos, row_of = gathered, m, where, idx
-        dh_dtype = torch.float32 if P > 1 and dh_reduce_f32 else torch.bfloat16
-        dH, dW = ops.dist_backward(
-            embed, softcap, *args, rows=rows, kept=kept, row_of=row_of, vocab_offset=off, vocab=embed.shape[0] * P,
-            need_dh=need_dh, need_dw=need_dw, dh_dtype=dh_dtype, token_chunk=token_chunk,
-        )
-        if dH is not None:
-            if P > 1:
-                with phase("dh_all_reduce"):
-                    all_reduce_sum(dH, mesh)
-            if pos is not None:
-                dH = ops.scatter_rows(dH, pos, torch.empty((T, d), dtype=hidden.dtype, device=hidden.device))
-            elif dH.dtype != hidden.dtype:
-                dH = dH.to(hidden.dtype)
-            if dH.shape != hidden.shape:
-                dH = dH.view(hidden.shape)
-        return dW, dH, *none
+        if T - m >= _SKIP_ZERO_GRAD_MIN_FRACTION * T:
+            args, rows, pos, row_of = gathered, m, where, idx
+    dH, dW = ops.dist_backward(
+        embed, softcap, *args, rows=rows, kept=ops.dist_kept(saved, T, K), row_of=row_of, vocab_offset=off,
+        vocab=embed.shape[0] * P, need_dh=need_dh, need_dw=need_dw,
+        dh_dtype=torch.float32 if P > 1 and dh_reduce_f32 else torch.bfloat16, token_chunk=token_chunk,
+    )
+    if dH is not None:
+        if P > 1:
+            with phase("dh_all_reduce"):
+                all_reduce_sum(dH, mesh)
+        if pos is not None:
+            dH = ops.scatter_rows(dH, pos, torch.empty((T, d), dtype=hidden.dtype, device=hidden.device))
+        elif dH.dtype != hidden.dtype:
+            dH = dH.to(hidden.dtype)
+        if hidden.ndim != 2:
+            dH = dH.view(hidden.shape)
+    return dW, dH, *none
+
+
+_once = once_differentiable(_dist_gradients)
 
 
 # Autograd nodes of this operator's eager calls that are still alive, each with its leaves.

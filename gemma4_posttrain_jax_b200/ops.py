@@ -180,10 +180,12 @@ def _dense_rows(h: torch.Tensor) -> tuple[torch.Tensor, int]:
     """``h`` [T, d] as the distribution kernels read it: unit column stride, 16-byte aligned rows
     that do not overlap (an expanded or oddly sliced ``h`` is copied); (view, row stride)."""
     T, d = h.shape
-    ok = h.stride(1) == 1 and h.data_ptr() % 16 == 0 and (T == 1 or (h.stride(0) % 8 == 0 and h.stride(0) >= d))
-    if not ok:
-        h = h.clone(memory_format=torch.contiguous_format)
-    return h, int(h.stride(0)) if T > 1 else d
+    ld, step = h.stride()
+    if T <= 1:
+        ld = d
+    if step != 1 or ld % 8 or ld < d or h.data_ptr() % 16:
+        return h.clone(memory_format=torch.contiguous_format), d
+    return h, ld
 
 
 def _dense_embed(w: torch.Tensor) -> torch.Tensor:
@@ -193,7 +195,9 @@ def _dense_embed(w: torch.Tensor) -> torch.Tensor:
 
 
 def _check_head(embed: torch.Tensor, hidden: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    dev = _require_cuda(embed, hidden, *others)
+    dev = embed.device
+    if not embed.is_cuda or hidden.device != dev or any(t is not None and t.device != dev for t in others):
+        _require_cuda(embed, hidden, *others)  # says what is wrong
     _check_bf16("embedding", embed)
     _check_bf16("hidden", hidden)
     return dev
@@ -203,15 +207,39 @@ def _addr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# Small calls take as long as the host takes to make them, so these look things up by the shortest way
+# (torch.cuda.current_stream builds a Stream object, torch.cuda.current_device checks its set-up).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _on_device(dev: torch.device, what: str, call) -> None:
     """``call(stream)`` with ``dev`` current, and its return code checked."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if dev.index == torch.cuda.current_device():
-        rc = call(stream)
+    if dev.index == _current_device():
+        rc = call(_raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = call(stream)
-    _lib.check(rc, what)
+            rc = call(_raw_stream(dev.index))
+    if rc != _lib.LP_OK:
+        _lib.check(rc, what)
+
+
+def dist_saved(T: int, K: int, vocab_rows: int, most: float, dev: torch.device) -> tuple[torch.Tensor, int | None]:
+    """What a forward leaves for its backward, as one f32 tensor: the tokens' logits [T, K], the rows'
+    log-normalisers [T] and, where they take at most ``most`` bytes, the logits in 16 bits;
+    (tensor, address of those or None)."""
+    n = T * K + T
+    at = -(-n // 64) * 64
+    nbytes = _lib.load().lp_dist_kept_bytes(T, vocab_rows) if most > 0 else 0
+    keep = 0 < nbytes <= most
+    saved = torch.empty((at + -(-nbytes // 4) if keep else n,), dtype=torch.float32, device=dev)
+    return saved, saved.data_ptr() + 4 * at if keep else None
+
+
+def dist_kept(saved: torch.Tensor, T: int, K: int) -> int | None:
+    """Address of the kept logits in ``dist_saved``'s tensor, if it has them."""
+    at = -(-(T * K + T) // 64) * 64
+    return saved.data_ptr() + 4 * at if saved.numel() > T * K + T else None
 
 
 def dist_forward(
@@ -221,35 +249,29 @@ def dist_forward(
     softcap: float | None,
     logp: torch.Tensor,
     entropy: torch.Tensor,
-    kept: torch.Tensor | None = None,
-) -> torch.Tensor:
-    """``lp_dist_fwd`` for int32 ``tokens`` [T, K] into f32 ``logp`` (T * K) and ``entropy`` (T). Returns
-    what the backward needs, f32 [T * K + T]: the tokens' logits, then the rows' log-normalisers.
-    ``kept`` (uint8, ``dist_kept_bytes``) receives the logits in 16 bits."""
+    saved: torch.Tensor,
+    kept: int | None = None,
+) -> None:
+    """``lp_dist_fwd`` for int32 ``tokens`` [T, K] into f32 ``logp`` (T * K), ``entropy`` (T) and
+    ``dist_saved``'s tensor."""
     dev = _check_head(embed, hidden, tokens)
     lib = _lib.load()
     T, K = tokens.shape
-    saved = torch.empty((T * K + T,), dtype=torch.float32, device=dev)
-    if T > 0:
-        h, ldh = _dense_rows(hidden)
-        w = _dense_embed(embed)
-        V, d = w.shape
+    if T == 0:
+        return
+    h, ldh = _dense_rows(hidden)
+    w = _dense_embed(embed)
+    V, d = w.shape
 
-        def call(stream):
-            ws, wsp, wsn = _workspace(lib.lp_dist_fwd_workspace_bytes(T, V), dev)
-            zt = saved.data_ptr()
-            return lib.lp_dist_fwd(
-                stream, h.data_ptr(), T, d, ldh, w.data_ptr(), V, 0, tokens.data_ptr(), K, softcap or 0.0, None, zt,
-                zt + 4 * T * K, entropy.data_ptr(), logp.data_ptr(), _addr(kept), wsp, wsn,
-            )
+    def call(stream):
+        ws, wsp, wsn = _workspace(lib.lp_dist_fwd_workspace_bytes(T, V), dev)
+        zt = saved.data_ptr()
+        return lib.lp_dist_fwd(
+            stream, h.data_ptr(), T, d, ldh, w.data_ptr(), V, 0, tokens.data_ptr(), K, softcap or 0.0, None, zt,
+            zt + 4 * T * K, entropy.data_ptr(), logp.data_ptr(), kept, wsp, wsn,
+        )
 
-        _on_device(dev, "lp_dist_fwd", call)
-    return saved
-
-
-def dist_kept_bytes(rows: int, vocab_rows: int) -> int:
-    """Bytes of the kept logits of ``rows`` rows over a (shard of the) vocabulary."""
-    return int(_lib.load().lp_dist_kept_bytes(rows, vocab_rows))
+    _on_device(dev, "lp_dist_fwd", call)
 
 
 def dist_forward_shard(
@@ -258,7 +280,7 @@ def dist_forward_shard(
     tokens: torch.Tensor,
     softcap: float | None,
     vocab_offset: int,
-    kept: torch.Tensor | None = None,
+    kept: int | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``lp_dist_fwd`` over one shard of the vocabulary: (stats [3, T], zt [T, K]) for ``dist_combine``."""
     dev = _check_head(embed, hidden, tokens)
@@ -274,7 +296,7 @@ def dist_forward_shard(
             ws, wsp, wsn = _workspace(lib.lp_dist_fwd_workspace_bytes(T, w.shape[0]), dev)
             return lib.lp_dist_fwd(
                 stream, h.data_ptr(), T, h.shape[1], ldh, w.data_ptr(), w.shape[0], int(vocab_offset),
-                tokens.data_ptr(), K, softcap or 0.0, stats.data_ptr(), zt.data_ptr(), None, None, None, _addr(kept), wsp, wsn,
+                tokens.data_ptr(), K, softcap or 0.0, stats.data_ptr(), zt.data_ptr(), None, None, None, kept, wsp, wsn,
             )
 
         _on_device(dev, "lp_dist_fwd", call)
@@ -288,20 +310,19 @@ def dist_combine(
     vocab: int,
     logp: torch.Tensor,
     entropy: torch.Tensor,
-) -> torch.Tensor:
-    """``lp_dist_combine``: [P, 3, T] and [P, T, K] into f32 ``logp`` (T * K) and ``entropy`` (T);
-    returns what ``dist_forward`` returns."""
+    saved: torch.Tensor,
+) -> None:
+    """``lp_dist_combine``: [P, 3, T] and [P, T, K] into f32 ``logp`` (T * K), ``entropy`` (T) and
+    ``dist_saved``'s tensor."""
     dev = _require_cuda(shard_stats, shard_zt, tokens)
     lib = _lib.load()
     T, K = tokens.shape
-    saved = torch.empty((T * K + T,), dtype=torch.float32, device=dev)
     stats, parts = shard_stats.contiguous(), shard_zt.contiguous()
     zt = saved.data_ptr()
     _on_device(dev, "lp_dist_combine", lambda stream: lib.lp_dist_combine(
         stream, stats.data_ptr(), parts.data_ptr(), stats.shape[0], T, K, int(vocab), tokens.data_ptr(), zt + 4 * T * K,
         entropy.data_ptr(), zt, logp.data_ptr(),
     ))
-    return saved
 
 
 def dist_rows(
@@ -322,7 +343,8 @@ def dist_rows(
     d = h.shape[1]
     h_out = torch.empty((T, d), dtype=h.dtype, device=dev)
     y_out = torch.empty_like(tokens)
-    saved_out, entropy_out = torch.empty_like(saved), torch.empty((T,), dtype=torch.float32, device=dev)
+    saved_out, _ = dist_saved(T, K, 0, 0, dev)
+    entropy_out = torch.empty((T,), dtype=torch.float32, device=dev)
     g_out = None if grad_logp is None else torch.empty((T, K), dtype=torch.float32, device=dev)
     ge_out = None if grad_entropy is None else torch.empty((T,), dtype=torch.float32, device=dev)
     index = torch.empty((2 * T + 1,), dtype=torch.int32, device=dev)
@@ -352,7 +374,7 @@ def dist_backward(
     grad_entropy: torch.Tensor | None,
     *,
     rows: int | None = None,
-    kept: torch.Tensor | None = None,
+    kept: int | None = None,
     row_of: torch.Tensor | None = None,
     vocab_offset: int = 0,
     vocab: int | None = None,
@@ -365,8 +387,8 @@ def dist_backward(
     """``lp_dist_bwd``: (dH [T, d], partial over this shard; dW [Vs, d]) of contiguous f32 ``grad_logp``
     (T * K) and ``grad_entropy`` (T), either of which may be None. ``saved`` is the forward's;
     ``vocab`` is the whole vocabulary's size. ``rows`` takes the first that many rows only (of
-    ``dist_rows``). ``kept`` are the forward's kept logits of as many rows as ``tokens`` has, of which
-    row t's are at ``row_of[t]`` (int32; None: t)."""
+    ``dist_rows``). ``kept`` is the address of the forward's kept logits of as many rows as ``tokens``
+    has, of which row t's are at ``row_of[t]`` (int32; None: t)."""
     dev = _check_head(embed, hidden, tokens, saved, entropy, grad_logp, grad_entropy)
     lib = _lib.load()
     all_rows, K = tokens.shape
@@ -394,7 +416,7 @@ def dist_backward(
         return lib.lp_dist_bwd(
             stream, h.data_ptr(), T, d, ldh, w.data_ptr(), Vs, int(vocab_offset), int(vocab) if vocab else Vs,
             tokens.data_ptr(), K, softcap or 0.0, zt, zt + 4 * all_rows * K, entropy.data_ptr(), _addr(grad_logp),
-            _addr(grad_entropy), _addr(kept), all_rows, _addr(row_of), _addr(dH), d, _addr(dW), flags, chunk, wsp, wsn,
+            _addr(grad_entropy), kept, all_rows, _addr(row_of), _addr(dH), d, _addr(dW), flags, chunk, wsp, wsn,
         )
 
     _on_device(dev, "lp_dist_bwd", call)

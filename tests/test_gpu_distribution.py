@@ -113,6 +113,11 @@ def test_entropy_alone_and_a_graph_used_twice(cuda_device):
     within(first[1], dW, bW, "d embedding")
     again = torch.autograd.grad([entropy], [H, W], [ge], retain_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+    # gradients of gradients are refused, where they are asked for
+    (once,) = torch.autograd.grad([entropy], [H], [ge], create_graph=True)
+    assert torch.equal(once, first[0])
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        once.float().sum().backward()
     with torch.no_grad():
         W.mul_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
@@ -311,18 +316,18 @@ def test_shards_merge_to_the_whole(cuda_device, V, P, keep):
     g, ge = torch.randn((T, K), generator=gen, device=cuda_device), torch.randn((T,), generator=gen, device=cuda_device)
     ref = Reference(W, H, 30.0, kept=keep)
     vs = V // P
-    kept = [torch.empty(ops.dist_kept_bytes(T, vs), dtype=torch.uint8, device=cuda_device) if keep else None for _ in range(P)]
     shards = [W[p * vs : (p + 1) * vs] for p in range(P)]
-    parts = [ops.dist_forward_shard(w, H, y, 30.0, p * vs, kept[p]) for p, w in enumerate(shards)]
     logp, entropy = torch.empty((T, K), device=cuda_device), torch.empty((T,), device=cuda_device)
-    saved = ops.dist_combine(
-        torch.stack([s for s, _ in parts]), torch.stack([z for _, z in parts]), y, V, logp, entropy
-    )
+    saved, kept = zip(*[ops.dist_saved(T, K, vs, 1e9 if keep else 0, cuda_device) for _ in range(P)])
+    assert all(k == ops.dist_kept(s, T, K) for s, k in zip(saved, kept))
+    parts = [ops.dist_forward_shard(w, H, y, 30.0, p * vs, kept[p]) for p, w in enumerate(shards)]
+    for one in saved:
+        ops.dist_combine(torch.stack([s for s, _ in parts]), torch.stack([z for _, z in parts]), y, V, logp, entropy, one)
     picked = ref.picked(y)
     within(logp, picked, ref.logp_bound(picked), "logps")
     within(entropy, ref.entropy, ref.entropy_bound(), "entropy")
     grads = [
-        ops.dist_backward(w, 30.0, H, y, saved, entropy, g, ge, vocab_offset=p * vs, vocab=V, dh_dtype=torch.float32,
+        ops.dist_backward(w, 30.0, H, y, saved[p], entropy, g, ge, vocab_offset=p * vs, vocab=V, dh_dtype=torch.float32,
                           kept=kept[p])
         for p, w in enumerate(shards)
     ]
