@@ -845,10 +845,13 @@ struct MeshSum {
 // 256-row tile takes 0.94 of the time of two 128-row tiles: 512 rows of the 262144 x 2048 head 434
 // against 462 us, 1024 rows 826 / 868), but a last half-empty pair tile or a last round that pairs
 // fill badly costs more (128 rows 215 / 179 us, 301 rows 403 / 381, 1100 rows 1110 / 1013). Rounds
-// of the persistent workers decide, single CTAs' against 0.94 of the pairs'.
-int cta_group_dist(int64_t M, int64_t N, const DeviceInfo* di, CgUse use) {
+// of the persistent workers decide, single CTAs' against 0.94 of the pairs'. Below K = 1024 a tile's
+// epilogue takes longer than its product, and single CTAs, whose epilogues wait for no other CTA, are
+// faster (2048 rows, 131072 columns, K = 256 / 512 / 768: 242 / 253 / 328 us against 273 / 291 / 334).
+int cta_group_dist(int64_t M, int64_t N, int64_t K, const DeviceInfo* di, CgUse use) {
   const int f = forced_cta_group();
   if (f) return f;
+  if (K <= 768) return 1;
   const int w1 = di != nullptr ? workers(di, 1) : 148, w2 = di != nullptr ? workers(di, 2) : 74;
   const int64_t tn = cdiv(N, BN);
   const double one = (double)cdiv(cdiv(M, 128) * tn, w1), two = 0.94 * (double)cdiv(cdiv(M, 256) * tn, w2);
@@ -893,7 +896,7 @@ struct DistBwdPlan {
 DistBwdPlan dist_bwd_plan(int64_t T, int64_t d, int64_t Vs, int64_t token_chunk, int flags, const DeviceInfo* di) {
   DistBwdPlan P;
   const int64_t tc = token_chunk > 0 ? std::min<int64_t>(token_chunk, T) : default_token_chunk(T, Vs, d);
-  P.cg_dz = cta_group_dist(tc, Vs, di, CG_DZ);
+  P.cg_dz = cta_group_dist(tc, Vs, d, di, CG_DZ);
   // rows of one M tile waste half of a pair whatever the split of K; and a reduce launch takes
   // about as long as 16 K blocks
   P.split_dh = cdiv(Vs, BK) > 32;
@@ -1340,17 +1343,25 @@ struct DistFwdLayout {
   size_t part_off, part_a_off, keys_off, total;
 };
 
-// Scratch of one launch over T rows: its work counter, the (max, S) and A partials, and (top) the
-// rows' selection keys.
-DistFwdLayout dist_fwd_layout(int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di, int sms, size_t key_row_bytes) {
+// Scratch of one launch over T rows as CTA group cg: its work counter, the (max, S) and A partials,
+// and (top) the rows' selection keys.
+DistFwdLayout dist_fwd_layout(int cg, int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di, size_t key_row_bytes) {
   DistFwdLayout L{};
-  L.cg = cta_group_dist(T, Vs, di, CG_FWD);
-  L.s = plan_fwd(T, Vs, d, di != nullptr ? workers(di, L.cg) : sms / L.cg, 128 * L.cg);
+  L.cg = cg;
+  L.s = plan_fwd(T, Vs, d, di != nullptr ? workers(di, cg) : 148 / cg, 128 * cg);
   L.part_off = 256;
   L.part_a_off = L.part_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float2), 256);
   L.keys_off = L.part_a_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float), 256);
   L.total = L.keys_off + align_up((size_t)T * key_row_bytes, 256);
   return L;
+}
+DistFwdLayout dist_fwd_layout(int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di, size_t key_row_bytes) {
+  return dist_fwd_layout(cta_group_dist(T, Vs, d, di, CG_FWD), T, Vs, d, di, key_row_bytes);
+}
+// Enough for any hidden size, whichever CTA group that leads to.
+size_t dist_fwd_bytes(int64_t T, int64_t Vs, const DeviceInfo* di, size_t key_row_bytes) {
+  return std::max(dist_fwd_layout(1, T, Vs, 64, di, key_row_bytes).total,
+                  dist_fwd_layout(2, T, Vs, 64, di, key_row_bytes).total);
 }
 
 // Rows of the hidden operand's box: of a single M tile only the rows there are (in eights, the
@@ -1402,10 +1413,10 @@ TopKeys top_keys(int64_t T, int64_t V, int k) {
   return K;
 }
 
-size_t top_workspace(int64_t T, int64_t V, int k, const DeviceInfo* di, int sms) {
+size_t top_workspace(int64_t T, int64_t V, int k, const DeviceInfo* di) {
   const TopKeys K = top_keys(T, V, k);
-  size_t need = dist_fwd_layout(K.rows, V, 64, di, sms, K.row_bytes).total;
-  if (T % K.rows != 0) need = std::max(need, dist_fwd_layout(T % K.rows, V, 64, di, sms, K.row_bytes).total);
+  size_t need = dist_fwd_bytes(K.rows, V, di, K.row_bytes);
+  if (T % K.rows != 0) need = std::max(need, dist_fwd_bytes(T % K.rows, V, di, K.row_bytes));
   return need;
 }
 
@@ -1441,7 +1452,7 @@ int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
   int rc = current_device_info(&di);
   if (rc) return rc;
   const TopKeys K = top_keys(T, V, all.k);
-  const size_t need = top_workspace(T, V, all.k, di, di->sms);
+  const size_t need = top_workspace(T, V, all.k, di);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(LP_EWORKSPACE, "%zu workspace bytes needed, got %zu", need, workspace_bytes);
   if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return fail(LP_EINVAL, "workspace must be 256-byte aligned");
@@ -1449,7 +1460,7 @@ int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
   char* ws = reinterpret_cast<char*>(workspace);
   for (int64_t t0 = 0; t0 < T; t0 += K.rows) {
     const int64_t n = std::min<int64_t>(K.rows, T - t0);
-    const DistFwdLayout L = dist_fwd_layout(n, V, d, di, di->sms, K.row_bytes);
+    const DistFwdLayout L = dist_fwd_layout(n, V, d, di, K.row_bytes);
     const __nv_bfloat16* Hc = reinterpret_cast<const __nv_bfloat16*>(H) + t0 * ldh;
     alignas(64) CUtensorMap ta, tb, to;
     if ((rc = map_bf16(&ta, Hc, d, n, ldh, BK, a_box_rows(L, n), "hidden"))) return rc;
@@ -1520,7 +1531,7 @@ size_t lp_dist_fwd_workspace_bytes(int64_t T, int64_t Vs) {
   DeviceInfo* di = nullptr;
   const bool have = current_device_info(&di) == LP_OK;
   if (T <= 0 || Vs <= 0) return 256;
-  return dist_fwd_layout(T, Vs, 64, have ? di : nullptr, 148, 0).total;
+  return dist_fwd_bytes(T, Vs, have ? di : nullptr, 0);
 }
 
 size_t lp_dist_kept_bytes(int64_t T, int64_t Vs) {
@@ -1535,7 +1546,7 @@ int lp_dist_fwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, 
   if (T == 0) return LP_OK;
   DeviceInfo* di = nullptr;
   if ((rc = current_device_info(&di))) return rc;
-  const DistFwdLayout L = dist_fwd_layout(T, Vs, d, di, di->sms, 0);
+  const DistFwdLayout L = dist_fwd_layout(T, Vs, d, di, 0);
   if (workspace == nullptr || workspace_bytes < L.total)
     return fail(LP_EWORKSPACE, "lp_dist_fwd needs %zu workspace bytes, got %zu", L.total, workspace_bytes);
   if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return fail(LP_EINVAL, "workspace must be 256-byte aligned");
@@ -1672,7 +1683,7 @@ size_t lp_top_workspace_bytes(int64_t T, int64_t V, int k) {
   DeviceInfo* di = nullptr;
   const bool have = current_device_info(&di) == LP_OK;
   if (T <= 0 || V <= 0 || k < 1) return 256;
-  return top_workspace(T, V, k, have ? di : nullptr, 148);
+  return top_workspace(T, V, k, have ? di : nullptr);
 }
 
 int lp_top(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, int64_t V, float softcap,
