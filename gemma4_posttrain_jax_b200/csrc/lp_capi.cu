@@ -393,13 +393,14 @@ int launch_gemm_cg(cudaStream_t st, const CUtensorMap& a, const CUtensorMap& b, 
   const int grid = CG * std::max(1, std::min(p.s.num_units, workers(di, CG)));
   GemmParams pp = p;
   pp.dbg = dbg_ptr(tag);
-  // a caller that keeps a counter of its own (in its workspace) passes it in; where every worker
-  // has one unit it needs no counter and no memset (the distribution operators' small calls)
+  // A caller that keeps a counter of its own (in its workspace) passes it in. A single M tile's units
+  // are alike and share no operand but its few rows, so workers take them in turn: no counter, and no
+  // memset before the launch (3 us of a decode step with its gap).
   if (pp.sched == nullptr) {
     if (int rc = sched_slot(st, &pp.sched)) return rc;
-  } else if (p.s.num_units * CG <= grid) {
+  } else if (p.s.num_units * CG <= grid || (p.s.tiles_m == 1 && p.s.k_splits == 1)) {
     pp.sched = nullptr;
-  } else if (!p.sched_zeroed) {
+  } else {
     LP_CUDA_TRY(cudaMemsetAsync(pp.sched, 0, sizeof(unsigned), st));
   }
   ProfScope prof(st, tag);

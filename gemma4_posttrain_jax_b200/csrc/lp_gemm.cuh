@@ -206,10 +206,9 @@ struct GemmParams {
   // issued, [6] epilogue-warp cycles from accumulator ready to hand-back (warp 2), [7] tiles.
   unsigned long long* dbg;
   // Dynamic work distribution: units are claimed in order with atomicAdd on this counter
-  // (zero at launch), so the units in flight always form a compact window of the unit order. Null
-  // where every worker of the grid has one unit.
+  // (zero at launch), so the units in flight always form a compact window of the unit order. Null:
+  // worker w takes units w, w + workers, ...
   unsigned int* sched;
-  int sched_zeroed;  // host side: sched is zero already
   // MN-major operands with 3-D tensor maps (64 columns, K, 64-column chunks): the CTA's
   // tile of that operand is one TMA instruction instead of one per 64-column chunk.
   int a_mn3d, b_mn3d;
@@ -542,9 +541,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                                      : mbar_wait_bounded_cluster(&sempty_bar[slot], sph ^ 1, abort_flag,
                                                                  DEV_TIMEOUT_PRODUCER);
           if (!free_slot) break;
-          // no counter: as many workers as units, one unit each
           const unsigned claimed =
-              P.sched != nullptr ? atomicAdd(P.sched, 1u) : (i == 0 ? blockIdx.x / CG : (unsigned)S.num_units);
+              P.sched != nullptr ? atomicAdd(P.sched, 1u) : blockIdx.x / CG + (unsigned)i * (gridDim.x / CG);
           u = claimed < (unsigned)S.num_units ? (int)claimed : -1;
           sched_u[slot] = u;
           if constexpr (CG == 2) {

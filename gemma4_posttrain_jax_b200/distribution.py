@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .losses import _SKIP_ZERO_GRAD_MIN_FRACTION, _check_device, _check_num_valid, _debug_checks, _validate_softcap
+from .losses import _SKIP_ZERO_GRAD_MIN_FRACTION, _check_device, _validate_softcap
 from .phase_timer import phase
 from .sharding import VocabMesh, all_gather_stats, all_reduce_sum, vocab_offset
 
@@ -220,13 +220,10 @@ class _ValidSlots(torch.autograd.Function):
     """The rows of hidden [B, S, d] and ids [B, N] at the valid slots of mask [B, N], in slot order."""
 
     @staticmethod
-    def forward(ctx, hidden, ids, mask, first, num_valid):
+    def forward(ctx, hidden, ids, mask, first):
         rows, tokens, idx, pos, count = ops.compact(mask, hidden, ids, row_offset=first)
-        n = int(count.item()) if num_valid is None else int(num_valid)
-        if num_valid is None:
-            _check_device(hidden.device, "completion_logps_and_entropy")
-        elif _debug_checks():
-            _check_num_valid(count, n)
+        n = int(count.item())
+        _check_device(hidden.device, "completion_logps_and_entropy")  # the host has waited anyway
         ctx.save_for_backward(pos)
         ctx.meta = (tuple(hidden.shape), hidden.dtype, first, mask.shape[1])
         tokens, idx = tokens[:n], idx[:n]
@@ -240,7 +237,7 @@ class _ValidSlots(torch.autograd.Function):
         shape, dtype, first, width = ctx.meta
         out = torch.zeros(shape, dtype=dtype, device=g.device)
         ops.scatter_rows(g.contiguous(), pos, out[:, first : first + width])
-        return out, None, None, None, None
+        return out, None, None, None
 
 
 def completion_logps_and_entropy(
@@ -251,12 +248,11 @@ def completion_logps_and_entropy(
     *,
     prompt_width: int,
     softcap: float | None,
-    num_valid: int | None = None,
     **options,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``completion_logps`` with the entropy: (logps [B, N], entropy [B, N]) of the completion tokens of
-    hidden [B, P + N, d], differentiable, computed at the valid slots only and 0 elsewhere. ``num_valid``
-    is ``completion_logps``'; ``options`` are those of ``token_logps_and_entropy``.
+    hidden [B, P + N, d], differentiable, computed at the valid slots only and 0 elsewhere. The host
+    waits once for the number of valid slots. ``options`` are those of ``token_logps_and_entropy``.
     """
     if hidden.ndim != 3 or completion_ids.ndim != 2 or completion_mask.shape != completion_ids.shape:
         raise ValueError("hidden must be [B, S, d] and completion ids / mask [B, N]")
@@ -269,7 +265,7 @@ def completion_logps_and_entropy(
     rows = hidden
     if hidden.stride(-1) != 1 or hidden.stride(0) % 8 or hidden.stride(1) % 8 or hidden.data_ptr() % 16:
         rows = hidden.contiguous()
-    rows, tokens, idx = _ValidSlots.apply(rows, _as_int32(completion_ids), completion_mask, prompt_width - 1, num_valid)
+    rows, tokens, idx = _ValidSlots.apply(rows, _as_int32(completion_ids), completion_mask, prompt_width - 1)
     logps, entropy = token_logps_and_entropy(embed_tokens, rows, tokens, softcap=softcap, **options)
     slots = idx.long()
 

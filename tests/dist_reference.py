@@ -100,6 +100,7 @@ class Reference:
 
 
 def within(got, ref, bound, what):
+    got = got.detach()
     off = (got.double() - ref).abs()
     assert torch.isfinite(got).all(), what
     worst = float((off / bound).max()) if off.numel() else 0.0

@@ -98,6 +98,24 @@ def test_one_gradient_alone_and_row_chunks(cuda_device, frozen, K, keep):
     within(got, dH if frozen == "embed" else dW, bH if frozen == "embed" else bW, "gradient")
 
 
+def test_many_tokens_per_position(cuda_device):
+    from gemma4_posttrain_jax_b200 import token_logps_and_entropy
+
+    T, V, d, K = 9, 300, 64, 256
+    W, H, gen = _inputs(cuda_device, T, V, d)
+    y = torch.randint(-40, V + 40, (T, K), generator=gen, device=cuda_device)  # many of them several times
+    g, ge = torch.randn((T, K), generator=gen, device=cuda_device), torch.randn((T,), generator=gen, device=cuda_device)
+    W.requires_grad_(True), H.requires_grad_(True)
+    logps, entropy = token_logps_and_entropy(W, H, y, softcap=30.0)
+    ref = Reference(W.detach(), H.detach(), 30.0, kept=True)
+    picked = ref.picked(y)
+    within(logps, picked, ref.logp_bound(picked), "logps")
+    dH, dW, bH, bW = ref.grads(y, g, ge)
+    got = torch.autograd.grad([logps, entropy], [H, W], [g, ge])
+    within(got[0], dH, bH, "d hidden")
+    within(got[1], dW, bW, "d embedding")
+
+
 def test_entropy_alone_and_a_graph_used_twice(cuda_device):
     from gemma4_posttrain_jax_b200 import token_logps_and_entropy
 
@@ -215,9 +233,9 @@ def test_completions(cuda_device):
     y = ids.reshape(-1)[on][:, None]
     dH, dW, bH, bW = ref.grads(y, g.reshape(-1)[on][:, None], ge.reshape(-1)[on])
     wide = torch.nn.functional.pad(H, (0, 4))[..., :d]  # rows that have to be copied first
-    for hidden, count in ((H.clone(), None), (H.clone(), int(mask.sum())), (wide.detach(), None)):
+    for hidden in (H.clone(), wide.detach()):
         hidden.requires_grad_(True)
-        logps, entropy = completion_logps_and_entropy(W, hidden, ids, mask, prompt_width=prompt, softcap=30.0, num_valid=count)
+        logps, entropy = completion_logps_and_entropy(W, hidden, ids, mask, prompt_width=prompt, softcap=30.0)
         assert logps.shape == entropy.shape == (B, N)
         assert (logps[~mask] == 0).all() and (entropy[~mask] == 0).all()
         picked = ref.picked(y)
