@@ -395,7 +395,7 @@ int launch_gemm_cg(cudaStream_t st, const CUtensorMap& a, const CUtensorMap& b, 
   pp.dbg = dbg_ptr(tag);
   // A caller that keeps a counter of its own (in its workspace) passes it in. A single M tile's units
   // are alike and share no operand but its few rows, so workers take them in turn: no counter, and no
-  // memset before the launch (3 us of a decode step with its gap).
+  // memset before the launch (1 row x 262144 x 2048, the whole top-20 call: 192.2 us, with a counter 193.8).
   if (pp.sched == nullptr) {
     if (int rc = sched_slot(st, &pp.sched)) return rc;
   } else if (p.s.num_units * CG <= grid || (p.s.tiles_m == 1 && p.s.k_splits == 1)) {
