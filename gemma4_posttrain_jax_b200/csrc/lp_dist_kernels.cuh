@@ -334,6 +334,27 @@ struct DistDzParams {
 };
 constexpr int kDzStep = 2048;  // columns of a block's step
 
+// Eight entries whose columns are kept by y = 2 x / c in base 2 (keep_raw), the one of place `at`
+// with gv. With e = 2^y, r = 1 / (1 + e): z = c (1 - 2 r) and softcap' = 4 e r^2, near 0 too. Out of
+// line: rare, and the common path has no registers to spare.
+__device__ __noinline__ uint4 dist_dz_raw(uint4 kept, float slot, float cap, float a, float b, float l2, float gv,
+                                          int at) {
+  const uint32_t w[4] = {kept.x, kept.y, kept.z, kept.w};
+  float y0, step;
+  keep_raw_range(slot, y0, step);
+  const float c2 = cap * kLog2e;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t n = (j & 1) ? w[j / 2] >> 16 : w[j / 2] & 0xffffu;
+    const float e = fast_ex2(fmaf((float)n, step, y0));
+    const float r = fast_rcp(1.f + e);
+    const float lp = fmaf(-2.f * c2, r, c2 - l2);
+    v[j] = 4.f * e * r * r * ((j == at ? gv : 0.f) - fast_ex2(lp) * fmaf(b, lp, a));
+  }
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
 __global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
   const int t = blockIdx.y;
   float a, b, l2, gv = 0.f;
@@ -366,7 +387,7 @@ __global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
     q = __ldcs(reinterpret_cast<const uint4*>(kept + c0));
     mx = __ldg(kept_max + c0 / 32);
   }
-  constexpr float step = kKeepRange / 65535.f;
+  const float step = keep_range(P.cap * kLog2e) / 65535.f;
   auto two = [](float x) { return pack_f32x2(x, x); };
   const f32x2 a2 = two(a), b2 = two(b), ml2 = two(-l2), ucap2 = two(ucap), mstep2 = two(-step), m23 = two(-8388608.f),
               mone = two(-1.f);
@@ -378,6 +399,11 @@ __global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
     if (col + kDzStep < end) {
       q = __ldcs(reinterpret_cast<const uint4*>(kept + col + kDzStep));
       mx = __ldg(kept_max + (col + kDzStep) / 32);
+    }
+    if (kept_raw(m)) {
+      *reinterpret_cast<uint4*>(dz + col) =
+          dist_dz_raw(make_uint4(w[0], w[1], w[2], w[3]), m, P.cap, a, b, l2, gv, yc - col);
+      continue;
     }
     const f32x2 top = two(m);
     uint32_t out[4];

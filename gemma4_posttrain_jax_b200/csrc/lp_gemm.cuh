@@ -405,19 +405,57 @@ __device__ __forceinline__ void dist_accumulate(const float (&z)[32], int nvalid
 }
 
 // Logits kept for the backward: 16 bits each, as the distance below the largest of their 32 columns
-// in steps of kKeepRange / 65535 (base 2), at most kKeepRange. A kept logit is off by at most
-// 3.7e-4 * ln2, so a probability by 2.5e-4 of itself, a fifteenth of what the bf16 rounding of dZ
-// that follows may add; what lies further below is kept at 2^-48 of the largest. The largest itself
-// is kept exactly (f32).
+// in 65535 steps of keep_range (48 in base 2, or twice the cap where that is less: all there can be).
+// A kept logit is off by at most 3.7e-4 * ln2, so a probability by 2.5e-4 of itself, a fifteenth of
+// what the bf16 rounding of dZ that follows may add; what lies further below is kept at 2^-48 of the
+// largest. The largest itself is kept exactly (f32).
+// softcap' = 1 - (z / c)^2 takes more where it is near 0: columns of which one reaches |y| > kKeepRawFrom,
+// y = 2 x / c in base 2 (softcap' < 0.061; above it the steps are 5e-4 of softcap' at most), are kept by y
+// instead, in 65535 steps of the range they take. The largest's place then holds a NaN with that range's
+// ends, rounded outward to 1 / 2047 of +-kKeepRawMax (beyond, softcap' is below f32's rounding of z / c).
 constexpr float kKeepRange = 48.f;
-__device__ __forceinline__ void keep_logits(const float (&z)[32], float mx, uint32_t (&pk)[16]) {
+constexpr float kKeepRawFrom = 6.f;
+constexpr float kKeepRawMax = 26.f;
+constexpr float kKeepRawUnit = 2.f * kKeepRawMax / 2047.f;
+__device__ __forceinline__ float keep_range(float c2) { return c2 > 0.f ? fminf(kKeepRange, 2.f * c2) : kKeepRange; }
+__device__ __forceinline__ void keep_logits(const float (&z)[32], float mx, float range, float per_unit,
+                                            uint32_t (&pk)[16]) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     // the low bits of 2^23 + n are n
-    const float lo = fmaf(fminf(mx - z[2 * j], kKeepRange), 65535.f / kKeepRange, 8388608.f);
-    const float hi = fmaf(fminf(mx - z[2 * j + 1], kKeepRange), 65535.f / kKeepRange, 8388608.f);
+    const float lo = fmaf(fminf(mx - z[2 * j], range), per_unit, 8388608.f);
+    const float hi = fmaf(fminf(mx - z[2 * j + 1], range), per_unit, 8388608.f);
     pk[j] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
   }
+}
+// By y; returns what takes the largest's place. Columns of vocabulary padding are 0.
+__device__ __forceinline__ float keep_raw(const uint32_t (&r)[32], float k1, uint32_t (&pk)[16]) {
+  float lo = kKeepRawMax, hi = -kKeepRawMax;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float y = __uint_as_float(r[j]) * k1;
+    lo = fminf(lo, y);
+    hi = fmaxf(hi, y);
+  }
+  const int a = max((int)floorf((lo + kKeepRawMax) * (1.f / kKeepRawUnit)), 0);
+  const int b = min((int)ceilf((hi + kKeepRawMax) * (1.f / kKeepRawUnit)), 2047);
+  const float y0 = fmaf((float)a, kKeepRawUnit, -kKeepRawMax), range = (float)(b - a) * kKeepRawUnit;
+  const float per_unit = range > 0.f ? 65535.f / range : 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float n0 = fminf(fmaxf(fmaf(__uint_as_float(r[2 * j]), k1, -y0), 0.f), range);
+    const float n1 = fminf(fmaxf(fmaf(__uint_as_float(r[2 * j + 1]), k1, -y0), 0.f), range);
+    pk[j] = __byte_perm(__float_as_uint(fmaf(n0, per_unit, 8388608.f)), __float_as_uint(fmaf(n1, per_unit, 8388608.f)),
+                        0x5410);
+  }
+  return __uint_as_float(0x7fc00000u | (uint32_t)a << 11 | (uint32_t)b);
+}
+__device__ __forceinline__ bool kept_raw(float mx) { return (__float_as_uint(mx) & 0x7fc00000u) == 0x7fc00000u; }
+__device__ __forceinline__ void keep_raw_range(float mx, float& y0, float& step) {
+  const uint32_t bits = __float_as_uint(mx);
+  const int a = (int)(bits >> 11 & 2047u), b = (int)(bits & 2047u);
+  y0 = fmaf((float)a, kKeepRawUnit, -kKeepRawMax);
+  step = (float)(b - a) * (kKeepRawUnit / 65535.f);
 }
 
 // The two largest of every G of 32 accumulator columns. The order is that of x (softcap is
@@ -757,6 +795,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const float xlog2e = kDist ? xs * kLog2e : kLog2e;
     const float k1 = HAS_CAP ? 2.0f * xlog2e / cap : 0.f;  // x -> 2x/c in base 2
     const float c2 = HAS_CAP ? cap * kLog2e : 0.f;        // c in base 2
+    const float keep = keep_range(c2), keep_per_unit = 65535.f / keep;  // DIST_KEEP
     bool ok = true;
     const bool dbg_warp = P.dbg != nullptr && warp == 2 && lane == 0;
     unsigned long long dbg_wait = 0, dbg_busy = 0, dbg_t = 0;
@@ -1029,7 +1068,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             if constexpr (EPI == EPI_DIST_KEEP) {
               if (nvalid > 0) {
                 uint32_t pk[16];
-                keep_logits(z, mx, pk);
+                float most = 0.f;  // |x|
+                if constexpr (HAS_CAP) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(__uint_as_float(r[j])));
+                }
+                if (HAS_CAP && most * k1 > kKeepRawFrom) mx = keep_raw(r, k1, pk);
+                else keep_logits(z, mx, keep, keep_per_unit, pk);
                 if (lane == 0) bulk_wait_read<1>();
                 __syncwarp();
                 uint8_t* buf_s = my_staging + sb * SBUF;

@@ -175,7 +175,8 @@ def token_logps_and_entropy(
 
     A differentiable call keeps the logits in 16 bits each for its backward when they take at most
     4 GiB, and recomputes them there otherwise; ``keep_logits`` says so either way. (A kept logit is
-    within 2.6e-4 of its value, which moves the gradients by a fifteenth of their bf16 rounding.)
+    within 2.6e-4 of its value, which moves the gradients by a fifteenth of their bf16 rounding; near
+    the softcap it is kept as it was before it, so that the slope there is as exact.)
 
     ``mesh``, ``token_chunk``, ``dh_reduce_f32`` and ``skip_zero_grad`` are those of
     ``per_token_logps``; over a mesh the shards' statistics are exchanged by one all-gather and the

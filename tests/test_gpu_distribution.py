@@ -81,6 +81,48 @@ def test_gradients(cuda_device, T, V, d, softcap, K, send, keep):
     assert _lib.device_error(0) == 0
 
 
+@pytest.mark.parametrize("softcap", [1.0, 5.0, 30.0, 100.0])
+@pytest.mark.parametrize("K", [1, 2])
+@pytest.mark.parametrize("keep", [True, False])
+def test_gradients_of_saturated_logits(cuda_device, softcap, K, keep):
+    """Logits far beyond the softcap, where its slope is small, one entry of dZ at a time: one position,
+    whose hidden state has one number that is not zero, so that every logit is one exact product and
+    row v of dW is dZ_v times that number."""
+    from gemma4_posttrain_jax_b200 import token_logps_and_entropy
+
+    V, d, lead = 1037, 8, 4.0
+    gen = torch.Generator(device=cuda_device).manual_seed(17)
+    span = torch.rand((V,), generator=gen, device=cuda_device) * 2 - 1
+    span[:256] = span[:256] * 0.4  # slopes that are not small
+    span[256:320] = span[256:320].abs() * 0.3 + 0.7  # every one of 64 neighbours near the cap
+    W = torch.zeros((V, d), device=cuda_device)
+    W[:, 3] = span * 5 * softcap / lead
+    W = W.to(torch.bfloat16).requires_grad_(True)
+    H = torch.zeros((1, d), dtype=torch.bfloat16, device=cuda_device)
+    H[0, 3] = lead
+    z = Reference(W.detach(), H, softcap).z[0]
+    for first in (int(z.argmax()), int(z.argmin()), 300, 7):
+        y = torch.tensor([[first, 260][:K]], device=cuda_device)
+        g = torch.tensor([[1.5, -0.75][:K]], device=cuda_device)
+        ge = torch.tensor([0.25], device=cuda_device)
+        logps, entropy = token_logps_and_entropy(W, H, y, softcap=softcap, keep_logits=keep)
+        (got,) = torch.autograd.grad([logps, entropy], [W], [g, ge])
+        ref = Reference(W.detach(), H, softcap)
+        _, dW, _, _ = ref.grads(y, g, ge)
+        slope = 1 - (ref.z[0] / softcap) ** 2
+        hot = torch.zeros(V, dtype=torch.float64, device=cuda_device).index_add_(0, y[0], g[0].abs().double())
+        raw = hot + ref.p[0] * (g.abs().sum() + ge.abs() * (ref.logp[0].abs() + ref.entropy))
+        # Two roundings to bf16 (dZ and dW). A logit kept by its distance below the largest is off by
+        # 24 ln2 / 65535 = 2.6e-4 at most, and p and log p by that; its slope is above 0.06 and off by
+        # 2 / c of half a step, which is at most 2 * 1.53e-5 / 0.06 of it. Kept by y = 2 x / c in base 2,
+        # in 65535 steps of at most 52.1, it is off by 4e-4 of y: the slope by ln2 * 4e-4, z by
+        # c / 2 * ln2 * 4e-4 of the slope. f32's share is that of z / c, 2^-19 of 1.
+        rel = 2.6e-4 * 2 + 5.1e-4 + 2.8e-4 + 2 * 1.4e-4 * softcap * slope + 2**-18
+        far = 2**-47 * (g.abs().sum() + ge.abs() * (40 + ref.entropy))
+        off = 2.02 * 2**-8 * dW[:, 3].abs() + lead * ((slope * rel + 2**-19) * raw + far) + 1e-30
+        within(got[:, 3], dW[:, 3], off, f"d embedding, token {first}")
+
+
 @pytest.mark.parametrize("frozen", ["embed", "hidden"])
 @pytest.mark.parametrize("K", [1, 3])
 @pytest.mark.parametrize("keep", [True, False])
