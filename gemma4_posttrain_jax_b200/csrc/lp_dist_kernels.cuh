@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
   __shared__ uint32_t lo_s;
   __shared__ int sel_key[kTopSel];
   __shared__ float sel_v[2 * kTopSel];  // of the selected keys: [0, n) the keys, [n, 2 n) the second
-  __shared__ float kth_s;
+  __shared__ float least_s;
   __shared__ long long best_i[kTopMax];
   __shared__ double best_z[kTopMax];
   __shared__ int best_id[kTopMax];
@@ -791,12 +791,14 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
         hi = mid;
       }
     }
-    if (lane == 0) kth_s = key_value(at);
+    // 2^-16 of slack for the accumulation and the bits cut off: of the row's largest value, not of the
+    // k-th alone, since sums near 0 are rounded where their terms are large
+    const float kth = key_value(at), most = key_value(__reduce_max_sync(0xffffffffu, top));
+    if (lane == 0) least_s = kth - 1.52587890625e-05f * fmaxf(fabsf(kth), fabsf(most));
   }
   __syncthreads();
   if (tid < n_sel) {
-    // 2^-16 of slack for the accumulation and the bits cut off; comparisons that a NaN fails keep
-    const float least = kth_s - 1.52587890625e-05f * fabsf(kth_s);
+    const float least = least_s;  // comparisons that a NaN fails keep
     first = sel_key[tid] * G;
     cols = !nonzero || !(group_value<G>(v0) < least) ? 1 : 0;
     if constexpr (GROUPS) {

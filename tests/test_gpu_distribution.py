@@ -533,6 +533,33 @@ def test_near_ties_follow_the_exact_order(cuda_device):
     assert len(set(got.ids[0, :8].tolist()) & set(ids.tolist())) == 8
 
 
+def test_ties_near_zero(cuda_device):
+    """Equal dot products near 0 whose f32 sums differ, with the k-th place among them and larger ones
+    before: the lowest ids come first."""
+    from gemma4_posttrain_jax_b200 import top_token_logps
+
+    V, d, k = 64, 1024, 12
+    gen = torch.Generator().manual_seed(5)
+    W = torch.zeros((V, d))
+    # of sizes from 2^-16 to 2^6, whose sums f32 rounds
+    part = torch.randn((256,), generator=gen) * 2.0 ** torch.randint(-16, 6, (256,), generator=gen)
+    part = part.to(torch.bfloat16).float()
+    W[:, :256] = part
+    # seven rows of the same numbers in other places, which sum to 0 exactly
+    some = [5, 9, 17, 33, 40, 51, 60]
+    for i in some:
+        W[i, :256] = part[torch.randperm(256, generator=gen)]
+    W[:, 256:512] = -part
+    W[:, 512] = -1.0
+    W[some, 512] = 0.0
+    W[torch.tensor([2, 3, 21, 22, 23, 24, 50, 63]), 512] = torch.arange(8) * 4.0 + 16.0
+    H = torch.ones((1, d), dtype=torch.bfloat16, device=cuda_device)
+    W = W.to(torch.bfloat16).to(cuda_device)
+    got = top_token_logps(W, H, None, k)
+    assert torch.equal(got.ids.long(), Reference(W, H, None).order(k))
+    assert got.ids[0, 8:].tolist() == some[:4]
+
+
 def test_rows_with_nan_stay_apart(cuda_device):
     """A row with a NaN answers NaN, with ids of the vocabulary, and leaves the other rows alone."""
     from gemma4_posttrain_jax_b200 import sample_top_k, token_logps_and_entropy, top_token_logps
