@@ -868,7 +868,10 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
     __syncthreads();
   }
   if (tid < P.k) {
-    const double x = ordered_f64(best_i[tid]);
+    double x = ordered_f64(best_i[tid]);
+    // a score that is not finite (two-sums of infinities are NaN) answers NaN: the softcap would bring
+    // it back to +-c
+    if (isinf(x)) x = NAN;
     if constexpr (SAMPLE) best_z[tid] = P.cap > 0.f ? (double)P.cap * tanh(x / (double)P.cap) : x;
     else best_z[tid] = (double)softcap_exact((float)x, P.cap);
   }

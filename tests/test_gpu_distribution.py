@@ -583,6 +583,24 @@ def test_rows_with_nan_stay_apart(cuda_device):
                     assert a[4].isnan().all()
 
 
+def test_infinite_scores_are_not_passed_off_as_finite(cuda_device):
+    """Infinite dot products, which a softcap would bring back to +-c, answer NaN."""
+    from gemma4_posttrain_jax_b200 import sample_top_k, top_token_logps
+
+    for V in (517, 20000):
+        W, H, gen = _inputs(cuda_device, 5, V, 64)
+        clean = H.clone()
+        H[2, 9] = float("inf")
+        u = torch.full((5,), 0.5, device=cuda_device)
+        keep = torch.arange(5, device=cuda_device) != 2
+        for got, ref in (
+            (top_token_logps(W, H, 30.0, 7)[:2], top_token_logps(W, clean, 30.0, 7)[:2]),
+            (sample_top_k(W, H, 30.0, u, temperature=1.0, top_k=7), sample_top_k(W, clean, 30.0, u, temperature=1.0, top_k=7)),
+        ):
+            assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, ref))
+            assert ((got[0][2] >= 0) & (got[0][2] < V)).all() and got[1][2].isnan().all()
+
+
 def test_more_rows_than_one_launch(cuda_device):
     from gemma4_posttrain_jax_b200 import top_token_logps
 
