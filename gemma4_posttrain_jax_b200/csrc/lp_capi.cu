@@ -405,11 +405,11 @@ int launch_gemm_cg(cudaStream_t st, const CUtensorMap& a, const CUtensorMap& b, 
   }
   ProfScope prof(st, tag);
   if constexpr (CG == 1) {
-    kern<<<grid, NUM_THREADS, smem, st>>>(a, b, o, pp);
+    kern<<<grid, num_threads<EPI>(), smem, st>>>(a, b, o, pp);
   } else {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(NUM_THREADS, 1, 1);
+    cfg.blockDim = dim3(num_threads<EPI>(), 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -1341,16 +1341,18 @@ namespace {
 struct DistFwdLayout {
   GemmSched s;
   int cg;
-  size_t part_off, part_a_off, keys_off, total;
+  size_t length_off, part_off, part_a_off, keys_off, total;
 };
 
-// Scratch of one launch over T rows as CTA group cg: its work counter, the (max, S) and A partials,
-// and (top) the rows' selection keys.
+// Scratch of one launch over T rows as CTA group cg: its work counter, (top) the lengths of the
+// embedding's longest rows, the (max, S) and A partials, and (top) the rows' selection keys.
 DistFwdLayout dist_fwd_layout(int cg, int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di, size_t key_row_bytes) {
   DistFwdLayout L{};
   L.cg = cg;
   L.s = plan_fwd(T, Vs, d, di != nullptr ? workers(di, cg) : 148 / cg, 128 * cg);
-  L.part_off = 256;
+  L.length_off = 256;
+  L.part_off = L.length_off +
+               align_up(key_row_bytes > 0 ? (size_t)(di != nullptr ? di->sms : 148) * SCAN_WARPS * sizeof(float) : 0, 256);
   L.part_a_off = L.part_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float2), 256);
   L.keys_off = L.part_a_off + align_up((size_t)2 * L.s.n_groups * T * sizeof(float), 256);
   L.total = L.keys_off + align_up((size_t)T * key_row_bytes, 256);
@@ -1414,11 +1416,24 @@ TopKeys top_keys(int64_t T, int64_t V, int k) {
   return K;
 }
 
+// Single CTAs, since only they can take the lengths of the embedding's rows beside the products; pairs
+// would be 0.94 of the time with many rows.
+DistFwdLayout top_layout(int64_t T, int64_t V, int64_t d, const DeviceInfo* di, size_t key_row_bytes) {
+  return dist_fwd_layout(1, T, V, d, di, key_row_bytes);
+}
+
 size_t top_workspace(int64_t T, int64_t V, int k, const DeviceInfo* di) {
   const TopKeys K = top_keys(T, V, k);
-  size_t need = dist_fwd_bytes(K.rows, V, di, K.row_bytes);
-  if (T % K.rows != 0) need = std::max(need, dist_fwd_bytes(T % K.rows, V, di, K.row_bytes));
+  size_t need = top_layout(K.rows, V, 64, di, K.row_bytes).total;
+  if (T % K.rows != 0) need = std::max(need, top_layout(T % K.rows, V, 64, di, K.row_bytes).total);
   return need;
+}
+
+template <int EPI>
+int launch_top_gemm(bool cap, cudaStream_t st, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o,
+                    const GemmParams& p, const DeviceInfo* di) {
+  return cap ? launch_gemm_cg<1, EPI, false, false, true>(st, a, b, o, p, di, "top_gemm")
+             : launch_gemm_cg<1, EPI, false, false, false>(st, a, b, o, p, di, "top_gemm");
 }
 
 template <bool SAMPLE, int G>
@@ -1461,7 +1476,7 @@ int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
   char* ws = reinterpret_cast<char*>(workspace);
   for (int64_t t0 = 0; t0 < T; t0 += K.rows) {
     const int64_t n = std::min<int64_t>(K.rows, T - t0);
-    const DistFwdLayout L = dist_fwd_layout(n, V, d, di, K.row_bytes);
+    const DistFwdLayout L = top_layout(n, V, d, di, K.row_bytes);
     const __nv_bfloat16* Hc = reinterpret_cast<const __nv_bfloat16*>(H) + t0 * ldh;
     alignas(64) CUtensorMap ta, tb, to;
     if ((rc = map_bf16(&ta, Hc, d, n, ldh, BK, a_box_rows(L, n), "hidden"))) return rc;
@@ -1473,20 +1488,23 @@ int top_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
     p.e.softcap = softcap;
     p.e.part = reinterpret_cast<float2*>(ws + L.part_off);
     p.e.part_a = reinterpret_cast<float*>(ws + L.part_a_off);
+    p.e.length2 = reinterpret_cast<float*>(ws + L.length_off);
     dist_hints(p);
     if (K.group > 1) {
       p.e.top = reinterpret_cast<float*>(ws + L.keys_off);
-      rc = K.group == 32 ? launch_gemm_cap<EPI_DIST_TOP32, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "top_gemm")
-                         : launch_gemm_cap<EPI_DIST_TOP8, false, false>(softcap > 0.f, st, ta, tb, ta, p, di, "top_gemm");
+      rc = K.group == 32 ? launch_top_gemm<EPI_DIST_TOP32>(softcap > 0.f, st, ta, tb, ta, p, di)
+                         : launch_top_gemm<EPI_DIST_TOP8>(softcap > 0.f, st, ta, tb, ta, p, di);
     } else {
       if ((rc = map_store_f32(&to, ws + L.keys_off, V, n, K.ld, "logits store"))) return rc;
-      rc = launch_gemm_cap<EPI_DIST_LOGITS, false, false>(softcap > 0.f, st, ta, tb, to, p, di, "top_gemm");
+      rc = launch_top_gemm<EPI_DIST_LOGITS>(softcap > 0.f, st, ta, tb, to, p, di);
     }
     if (rc) return rc;
     TopParams P = all;
     P.part = p.e.part;
     P.part_a = p.e.part_a;
     P.n_parts = 2 * L.s.n_groups;
+    P.length2 = p.e.length2;
+    P.n_lengths = std::max(1, std::min(L.s.num_units, workers(di, 1))) * SCAN_WARPS;
     P.T = (int)n;
     P.H = Hc;
     P.ldh = ldh;

@@ -18,6 +18,7 @@
 //   warp 1      : TMEM allocator + MMA issuer (one thread; in the pair leader only)
 //   warps 2..9  : epilogue; warp w reads TMEM lanes 32*(w%4).. (its 32 rows of the tile) and
 //                 one half (128 columns) of the tile; two epilogue warps per SM sub-partition
+//   warps 10..13: (selection GEMMs only) lengths of the rows of B, read from the staged tiles
 //
 // The two 256-column f32 accumulators (512 TMEM columns) are double-buffered, so the
 // epilogue of tile i overlaps the MMAs of tile i+1. Operands are K-major or MN-major,
@@ -38,6 +39,8 @@
 //   EPI_DIST_KEEP : EPI_DIST, with the logits kept in 16 bits (keep_logits).
 //   EPI_DIST_TOP32, EPI_DIST_TOP8 : EPI_DIST, with the two largest of every 32 (8) accumulator
 //                 columns, the first's column in its low bits.
+//   The three selection forms also leave the length of the longest row of B, which bounds what an
+//   accumulator may be off by (top_select_kernel). Single CTAs only.
 //   EPI_DIST_DZ : recompute path of log-probabilities and entropy:
 //                 dZ = (g * onehot - p * (a + b * log2 p)) * softcap' with two row constants a, b,
 //                 written as bf16 as EPI_BWD_DZ does.
@@ -45,6 +48,7 @@
 // Synchronisation (all waits bounded, see lp_ptx.cuh):
 //   full[s]   : TMA -> MMA. CG=2: lives in the leader, counts both CTAs' bytes.
 //   empty[s]  : MMA -> TMA, in every CTA; CG=2: one multicast commit arrives on both copies.
+//               Selection GEMMs: the four scan warps arrive, too.
 //   tfull[b]  : MMA -> epilogue, in every CTA (CG=2: one multicast commit).
 //   tempty[b] : epilogue -> MMA, in the leader; every epilogue warp of the pair arrives.
 #pragma once
@@ -84,6 +88,7 @@ constexpr int BN = 256;
 constexpr int BK = 64;
 constexpr int EPI_WARPS = 8;
 constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
+constexpr int SCAN_WARPS = 4;
 constexpr int TMEM_COLS = 2 * BN;
 constexpr int A_STAGE_BYTES = 128 * BK * 2;                // 16 KB: 128 rows of A per CTA
 constexpr float kLog2e = 1.4426950408889634f;
@@ -106,6 +111,16 @@ enum : int {
 template <int EPI>
 __host__ __device__ constexpr int top_group() {
   return EPI == EPI_DIST_TOP32 ? 32 : (EPI == EPI_DIST_TOP8 ? 8 : 0);
+}
+
+// GEMMs that take the lengths of B's rows: the selection's.
+template <int EPI>
+__host__ __device__ constexpr bool scans_lengths() {
+  return top_group<EPI>() > 0 || EPI == EPI_DIST_LOGITS;
+}
+template <int EPI>
+__host__ __device__ constexpr int num_threads() {
+  return NUM_THREADS + (scans_lengths<EPI>() ? 32 * SCAN_WARPS : 0);
 }
 
 // Epilogues that only read the accumulator: no store staging, the deepest operand ring.
@@ -172,6 +187,7 @@ struct EpiParams {
   float* part_a;         // DIST: [n_groups][M] running A (part holds the running max and S)
   float* keep_max;       // DIST_KEEP: [M][8 * tiles_n] largest logit of every 32 columns (base 2)
   float* top;            // DIST_TOP: [2][M][BN / group * tiles_n] largest and second of each group
+  float* length2;        // DIST_TOP, DIST_LOGITS: [CTAs][SCAN_WARPS] largest squared length of B's rows
   const float* row_const;  // DIST_DZ: [3][row_ld] per row: a, b, log2 of the normaliser; or null,
   long long row_ld;        //          then one token per row: its y and g (above), the vocabulary's
   long long vocab;         //          size, and per row the log-normaliser, the entropy and its
@@ -320,10 +336,9 @@ static_assert(gemm_smem_bytes<1, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<1, 
                   gemm_smem_bytes<2, EPI_FWD_LSE>() <= 232448 && gemm_smem_bytes<2, EPI_BWD_DZ>() <= 232448 &&
                   gemm_smem_bytes<2, EPI_STORE>() <= 232448 && gemm_smem_bytes<2, EPI_HEAD>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST_KEEP>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_KEEP>() <= 232448 &&
-                  gemm_smem_bytes<1, EPI_DIST_TOP32>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_TOP32>() <= 232448 &&
-                  gemm_smem_bytes<1, EPI_DIST_TOP8>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_TOP8>() <= 232448 &&
+                  gemm_smem_bytes<1, EPI_DIST_TOP32>() <= 232448 && gemm_smem_bytes<1, EPI_DIST_TOP8>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST>() <= 232448 && gemm_smem_bytes<2, EPI_DIST>() <= 232448 &&
-                  gemm_smem_bytes<1, EPI_DIST_LOGITS>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_LOGITS>() <= 232448 &&
+                  gemm_smem_bytes<1, EPI_DIST_LOGITS>() <= 232448 &&
                   gemm_smem_bytes<1, EPI_DIST_DZ>() <= 232448 && gemm_smem_bytes<2, EPI_DIST_DZ>() <= 232448,
               "GEMM shared memory above 227 KB");
 
@@ -480,7 +495,7 @@ __device__ __forceinline__ void top_keys_of(const uint32_t (&r)[32], int nvalid,
 
 // ----------------------------------------------------------------------------- kernel
 template <int CG, int EPI, bool A_MN, bool B_MN, bool HAS_CAP>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(num_threads<EPI>(), 1)
     tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmO, const GemmParams P) {
   using C = Cfg<CG>;
@@ -512,12 +527,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const bool leader = rank == 0;
   // consumers of a ring entry: the MMA thread and the epilogue warps (+ the peer's
   // producer and epilogue warps for a pair)
-  constexpr int kRingConsumers = CG == 1 ? 1 + EPI_WARPS : 2 * (1 + EPI_WARPS);
+  constexpr int kScanners = scans_lengths<EPI>() ? SCAN_WARPS : 0;
+  static_assert(kScanners == 0 || (CG == 1 && !B_MN), "lengths are taken by single CTAs, of rows");
+  constexpr int kRingConsumers = CG == 1 ? 1 + EPI_WARPS + kScanners : 2 * (1 + EPI_WARPS);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full_bar[s], 1);
-      mbar_init(&empty_bar[s], 1);
+      mbar_init(&empty_bar[s], 1 + kScanners);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull_bar[b], 1);
@@ -775,6 +792,61 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
     }
     __syncwarp();
+  } else if (scans_lengths<EPI>() && warp >= 2 + EPI_WARPS) {
+    // ------------------------------------------------------------------ lengths of B's rows
+    // Each thread sums the squares of two rows of the tile, stage by stage beside the MMA (in the first
+    // M tile's units; the others bring the same rows again): a stage's 64 columns in bf16 pairs, 32 steps
+    // of 2^-8 each (top_accumulator_error allows for them), then in f32. One row of the 262144 x 2048
+    // head: 182 us, without lengths 179; where products, not HBM, bound a tile, reading its 32 KB
+    // stages a second time from shared memory doubles its time (2048 rows: 1.76 ms, without 1.68).
+    const int r = (int)threadIdx.x - 32 * (2 + EPI_WARPS);  // rows r and r + 128
+    uint32_t it = 0, most = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      const int slot = i % SR;
+      const bool got = mbar_wait_bounded(&sfull_bar[slot], (i / SR) & 1, abort_flag, DEV_TIMEOUT_EPILOGUE);
+      if (!__all_sync(0xffffffffu, got)) break;
+      const int u = sched_u[slot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sempty_bar[slot]);
+      if (u < 0) break;
+      const Unit un = get_unit(S, u);
+      for (int nt = 0; ok && nt < un.n_count; ++nt) {
+        float sum0 = 0.f, sum1 = 0.f;
+        for (int kb = 0; kb < un.kb_count; ++kb, ++it) {
+          const int s = it % NS;
+          const bool full = mbar_wait_bounded(&full_bar[s], (it / NS) & 1, abort_flag, DEV_TIMEOUT_EPILOGUE);
+          ok = __all_sync(0xffffffffu, full);
+          if (!ok) break;
+          if (un.m_tile == 0) {
+            const uint8_t* b = stages + s * C::STAGE_BYTES + A_STAGE_BYTES + r * 128;
+            uint32_t p0 = 0, p1 = 0;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const int at = (c ^ (r & 7)) << 4;  // 128-byte swizzle
+              const uint4 x = *reinterpret_cast<const uint4*>(b + at);
+              const uint4 y = *reinterpret_cast<const uint4*>(b + 128 * 128 + at);
+              p0 = fma_bf16x2(x.x, x.x, p0);
+              p1 = fma_bf16x2(y.x, y.x, p1);
+              p0 = fma_bf16x2(x.y, x.y, p0);
+              p1 = fma_bf16x2(y.y, y.y, p1);
+              p0 = fma_bf16x2(x.z, x.z, p0);
+              p1 = fma_bf16x2(y.z, y.z, p1);
+              p0 = fma_bf16x2(x.w, x.w, p0);
+              p1 = fma_bf16x2(y.w, y.w, p1);
+            }
+            sum0 += __uint_as_float(p0 << 16) + __uint_as_float(p0 & 0xffff0000u);
+            sum1 += __uint_as_float(p1 << 16) + __uint_as_float(p1 & 0xffff0000u);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty_bar[s]);
+        }
+        // as integers they have the same order, with a NaN last
+        most = max(most, max(__float_as_uint(sum0), __float_as_uint(sum1)));
+      }
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) P.e.length2[blockIdx.x * SCAN_WARPS + (warp - 2 - EPI_WARPS)] = __uint_as_float(most);
   } else {
     // ------------------------------------------------------------------ epilogue warps
     // Two warps per TMEM lane quarter: warp 2+e (e = 0..7) reads lanes 32*(warp%4).. and

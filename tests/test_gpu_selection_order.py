@@ -1,0 +1,75 @@
+"""The order that ``top_token_logps`` and ``sample_top_k`` promise -- exact dot products, the lowest id first
+among equals -- where f32 sums cannot tell the tokens apart: cancelling terms, thousands of neighbours within
+a rounding, rows of the embedding of very different lengths."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.dist_reference import Reference, within
+
+pytestmark = pytest.mark.gpu
+
+def _cancelling(V, d=1024, seed=5):
+    """Seven rows whose dot product with a row of ones is exactly 0, the sum of terms from 2^-16 to 2^6 that
+    f32 rounds differently in each; -1 for every other row."""
+    gen = torch.Generator().manual_seed(seed)
+    W = torch.zeros((V, d))
+    part = torch.randn((256,), generator=gen) * 2.0 ** torch.randint(-16, 6, (256,), generator=gen)
+    part = part.to(torch.bfloat16).float()
+    W[:, :256] = part
+    some = [5, 9, 17, 33, 40, 51, 60]
+    for i in some:
+        W[i, :256] = part[torch.randperm(256, generator=gen)]
+    W[:, 256:512] = -part
+    W[:, 512] = -1.0
+    W[some, 512] = 0.0
+    return W.to(torch.bfloat16), torch.ones((1, d), dtype=torch.bfloat16), some
+
+
+@pytest.mark.parametrize("V", [64, 4099, 60000])
+@pytest.mark.parametrize("k", [1, 4, 7])
+def test_equal_sums_of_cancelling_terms(cuda_device, V, k):
+    from gemma4_posttrain_jax_b200 import sample_top_k, top_token_logps
+
+    W, H, some = _cancelling(V)
+    W, H = W.to(cuda_device), H.to(cuda_device)
+    got = top_token_logps(W, H, None, k)
+    assert got.ids[0].tolist() == some[:k]
+    # k equal weights: the numbers (j + 1/2) / k draw token j
+    u = (torch.arange(k, device=cuda_device) + 0.5) / k
+    token, _ = sample_top_k(W, H.expand(k, -1), None, u, temperature=1.0, top_k=k)
+    assert token.tolist() == some[:k]
+
+
+@pytest.mark.parametrize("d", [16, 136, 2048, 8192])
+def test_what_an_accumulator_may_be_off_by(cuda_device, d):
+    """The bound that the selection counts on, (17/4 + 1) 2^-23 of |h| |w| for every 16 terms, against sums
+    that lose the most: one large term with many that lie just below its last bits, on either side of it."""
+    from gemma4_posttrain_jax_b200 import _lib, ops
+
+    lib = _lib.load()
+    gen = torch.Generator(device=cuda_device).manual_seed(d)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=gen, device=cuda_device)
+
+    small = 2.0 ** -torch.arange(10, 42, device=cuda_device).float()[:, None]
+    rows = []
+    for sign in (1.0, -1.0):
+        for size in (1.0, 1.9921875):
+            for every in (d, 64, 16):
+                w = (size * sign * small).expand(-1, d).clone()
+                w[:, ::every] = 1.0
+                rows.append(w)
+    rows += [normal(64, d), normal(64, d).abs(), normal(64, d) * 2.0 ** torch.randint(-12, 12, (64, d), generator=gen, device=cuda_device)]
+    W = torch.cat(rows).to(torch.bfloat16)
+    H = torch.cat([torch.ones((1, d), device=cuda_device), normal(63, d), normal(64, d).abs()]).to(torch.bfloat16)
+    D = torch.empty((H.shape[0], W.shape[0]), device=cuda_device)
+    rc = lib.lp_gemm_bf16(ops._stream(cuda_device), ops._ptr(H), H.shape[0], d, d, 0, ops._ptr(W), W.shape[0], d, 0,
+                          ops._ptr(D), W.shape[0])
+    _lib.check(rc, "lp_gemm_bf16")
+    off = (D.double() - H.double() @ W.double().T).abs()
+    lengths = H.double().norm(dim=1)[:, None] * W.double().norm(dim=1)
+    within(off, torch.zeros_like(off), -(-d // 16) * 5.25 * 2**-23 * lengths, "accumulators")
