@@ -1395,7 +1395,7 @@ int check_dist(const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, 
 }
 
 // Selection keys of a row: two values per group of 32 or 8 columns, or the f32 logits. Larger groups
-// are fewer bytes to write and to search, but two of the n = k + kTopSpare selected tokens fall into
+// are fewer bytes to write and to search, but two of the about n = k + kTopSpare selected tokens fall into
 // one group n^2 / (2 V / group) times, and then its other columns are scored again. A group size is
 // taken where that adds at most half as many scores again: V >= 992 n for 32, 56 n for 8.
 struct TopKeys {
@@ -1440,7 +1440,7 @@ template <bool SAMPLE, int G>
 int launch_top_select(cudaStream_t st, TopParams& P, int64_t rows) {
   const size_t key_bytes = align_up((size_t)P.n_keys * sizeof(uint32_t), 16);
   P.keys_in_smem = key_bytes <= (size_t)kTopKeyBytes;
-  const size_t smem = std::max<size_t>(P.keys_in_smem ? key_bytes : 0, kTopCandBytes);
+  const size_t smem = P.keys_in_smem ? key_bytes : 0;
   auto kern = top_select_kernel<SAMPLE, G>;
   static bool configured[kMaxDevices] = {};
   int dev = 0;

@@ -466,12 +466,13 @@ __global__ void dist_dz_targets_kernel(const int32_t* __restrict__ y, const floa
 // ----------------------------------------------------------------------------- selection
 // The k most likely tokens of a row, in the order of the exact dot products h . W_v (softcap is
 // monotone), the lowest id first among equals. The GEMM only nominates: a key is one accumulator
-// (f32) or the largest of G neighbours with the second largest beside it. The k + kTopSpare largest
-// keys are selected. The k-th largest of the values seen there (keys and second largest) is a lower
+// (f32) or the largest of G neighbours with the second largest beside it. The largest keys, a few more
+// than k, are selected. The k-th largest of the values seen there (keys and second largest) is a lower
 // bound of the k-th logit: a key below it, beyond what either may be off by, is dropped, and a group
 // whose second largest reaches it has all its columns scored. Candidates are scored again to 2^-48 and
-// ranked by that, so the nomination's rounding can exchange neighbours only if more than kTopSpare
-// values lie within it of the k-th.
+// ranked by that. Where a key that was not selected could still hold one of the k (it reaches the exact
+// k-th score, but for what it may be off by), all such keys follow, as many at a time as there are slots:
+// equal or nearly equal tokens by the thousand, which a row in earnest does not have.
 //
 // What an accumulator may be off by (top_accumulator_error): one step of the tensor core adds 16
 // products, aligned to the largest of them and the sum so far, without what lies below 2^-25 of that,
@@ -485,12 +486,11 @@ __global__ void dist_dz_targets_kernel(const int32_t* __restrict__ y, const floa
 // (about n^2 / (2 kTopThreads), the keys that share a thread). Only when more than kTopSel do, a
 // bisection over all keys follows.
 constexpr int kTopMax = 128;
-constexpr int kTopSpare = 8;
+constexpr int kTopSpare = 8;  // keys selected beyond k, with k / 16 more: they lie the closer, the larger k
 constexpr int kTopThreads = 512;
 constexpr int kTopSel = kTopMax + 8 * kTopSpare;  // most selected keys
 constexpr int kTopBatch = 384;                    // candidates scored and ranked at a time,
 constexpr int kTopCand = kTopBatch + kTopMax;     // beside the best of those before them
-constexpr int kTopCandBytes = kTopCand * (int)(sizeof(long long) + sizeof(int));
 constexpr int kTopKeyBytes = 184 * 1024;  // most key bytes kept in shared memory, beside the static part
 
 // Order-preserving map of f32 to u32; NaN comes last.
@@ -572,17 +572,15 @@ __device__ __forceinline__ double ordered_f64(long long b) {
 template <bool SAMPLE, int G>
 __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopParams P) {
   constexpr bool GROUPS = G > 1;
-  // keys while selecting, then the candidates' scores and ids
-  extern __shared__ __align__(16) uint8_t dyn_s[];
-  uint32_t* keys_s = reinterpret_cast<uint32_t*>(dyn_s);
-  long long* cand_z = reinterpret_cast<long long*>(dyn_s);
-  int* cand_id = reinterpret_cast<int*>(dyn_s + kTopCand * sizeof(long long));
+  extern __shared__ __align__(16) uint32_t keys_s[];  // where they fit
+  __shared__ long long cand_z[kTopCand];
+  __shared__ int cand_id[kTopCand];
   constexpr int kWarps = kTopThreads / 32;
   __shared__ __align__(16) uint32_t max_s[kTopThreads];
   __shared__ float red_s[4][kWarps];
   __shared__ uint32_t length_s[kWarps];
   __shared__ int warp_s[kWarps];
-  __shared__ int n_sel_s;
+  __shared__ int n_sel_s, next_s;
   __shared__ uint32_t lo_s;
   __shared__ int sel_key[kTopSel];
   __shared__ float sel_v[2 * kTopSel];  // of the selected keys: [0, n) the keys, [n, 2 n) the second
@@ -695,9 +693,9 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
     for (int o = 16; o > 0; o >>= 1) h2 += __shfl_xor_sync(0xffffffffu, h2, o);
     if (lane == 0) error_s = top_accumulator_error(h2, __uint_as_float(w2), P.d);
   }
-  uint32_t lo = 0u;
+  uint32_t lo = 0u, reached = 0u;  // the keys from lo on are selected; k keys at least reach the other
   if (nonzero) {
-    const int n = min(n_keys, P.k + kTopSpare);
+    const int n = min(n_keys, P.k + kTopSpare + P.k / 16);
     // ---- a threshold that at least n keys reach, by bisection on the threads' maxima
     if (n < n_keys && warp == 0) {
       uint32_t v[kTopThreads / 32];
@@ -736,7 +734,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
       lo_s = 0u;
     }
     __syncthreads();
-    lo = lo_s;
+    lo = reached = lo_s;
     for (int i = tid; i < n_keys; i += kTopThreads) {
       if (key(i) >= lo) {
         const int at = atomicAdd(&n_sel_s, 1);
@@ -760,37 +758,13 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
           hi = mid;
         }
       }
-      const bool ties = c_lo > kTopSel;  // then hi = lo + 1: more equal keys than slots
+      reached = lo;
+      if (c_lo > kTopSel) ++lo;  // more equal keys than slots: at first those above them, fewer than n
       if (tid == 0) n_sel_s = 0;
       __syncthreads();
-      for (int i = tid; i < n_keys; i += kTopThreads) {
-        const uint32_t x = key(i);
-        if (ties ? x > lo : x >= lo) sel_key[atomicAdd(&n_sel_s, 1)] = i;
-      }
+      for (int i = tid; i < n_keys; i += kTopThreads)
+        if (key(i) >= lo) sel_key[atomicAdd(&n_sel_s, 1)] = i;
       __syncthreads();
-      if (ties) {
-        // fewer than n keys lie above the tie; fill up to n with the lowest of the tie
-        int have = n_sel_s;
-        __syncthreads();
-        for (int base = 0; base < n_keys && have < n; base += kTopThreads) {
-          const int i = base + tid;
-          const bool hit = i < n_keys && key(i) == lo;
-          const unsigned ballot = __ballot_sync(0xffffffffu, hit);
-          if (lane == 0) warp_s[warp] = __popc(ballot);
-          __syncthreads();
-          int before = 0, total = 0;
-          for (int w = 0; w < kWarps; ++w) {
-            before += w < warp ? warp_s[w] : 0;
-            total += warp_s[w];
-          }
-          const int slot = have + before + __popc(ballot & ((1u << lane) - 1u));
-          if (hit && slot < n) sel_key[slot] = i;
-          have = min(n, have + total);
-          __syncthreads();
-        }
-        if (tid == 0) n_sel_s = n;
-        __syncthreads();
-      }
     }
   } else {
     // every logit is exactly 0: the first k tokens, or every column of the groups that hold them
@@ -798,120 +772,165 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
     if (tid == 0) n_sel_s = (P.k + G - 1) / G;
     __syncthreads();
   }
-  // ---- candidates of the selected keys: where each key's first one is
-  const int n_sel = n_sel_s;  // the keys in shared memory are not read below
-  int first = 0, cols = 0;    // this thread's key
-  float v0 = -INFINITY, v1 = -INFINITY;
-  if (tid < n_sel) {
-    v0 = values[sel_key[tid]];
-    if constexpr (GROUPS) v1 = group_value<G>(values[(size_t)P.T * P.ld_keys + sel_key[tid]]);
-    sel_v[tid] = group_value<G>(v0);
-    sel_v[n_sel + tid] = v1;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    // a value that at least k of those seen reach, and nearly no more
-    constexpr int kSeen = (GROUPS ? 2 : 1) * kTopSel / 32;
-    uint32_t v[kSeen];
-    uint32_t top = 0u;
-#pragma unroll
-    for (int j = 0; j < kSeen; ++j) {
-      const int i = j * 32 + lane;
-      v[j] = i < (GROUPS ? 2 : 1) * n_sel ? ordered_key(sel_v[i]) : 0u;
-      top = max(top, v[j]);
+  // ---- rounds: the selected keys, then those that may still hold one of the k
+  int n_sel = n_sel_s, n_best = 0;
+  float least = 0.f;  // what lies below is not one of the k
+  for (int pos = -1;;) {  // after the first round: where the keys that follow start
+    int first = 0, cols = 0;  // candidates of this thread's key
+    float v0 = -INFINITY, v1 = -INFINITY;
+    if (tid < n_sel) {
+      v0 = values[sel_key[tid]];
+      if constexpr (GROUPS) v1 = group_value<G>(values[(size_t)P.T * P.ld_keys + sel_key[tid]]);
     }
-    uint32_t at = min(lo, __reduce_max_sync(0xffffffffu, top));
-    unsigned long long hi = (unsigned long long)__reduce_max_sync(0xffffffffu, top) + 1;
-    int c_at = 2 * kTopSel;
-    while (c_at > P.k && hi - at > 1) {
-      const uint32_t mid = (uint32_t)(at + (hi - at) / 2);
-      int c = 0;
+    if (pos < 0) {
+      if (tid < n_sel) {
+        sel_v[tid] = group_value<G>(v0);
+        sel_v[n_sel + tid] = v1;
+      }
+      __syncthreads();
+      if (warp == 0) {
+        // a value that at least k of those seen reach, and nearly no more
+        constexpr int kSeen = (GROUPS ? 2 : 1) * kTopSel / 32;
+        uint32_t v[kSeen];
+        uint32_t top = reached;
 #pragma unroll
-      for (int j = 0; j < kSeen; ++j) c += v[j] >= mid ? 1 : 0;
-      c = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
-      if (c >= P.k) {
-        at = mid;
-        c_at = c;
-      } else {
-        hi = mid;
+        for (int j = 0; j < kSeen; ++j) {
+          const int i = j * 32 + lane;
+          v[j] = i < (GROUPS ? 2 : 1) * n_sel ? ordered_key(sel_v[i]) : 0u;
+          top = max(top, v[j]);
+        }
+        uint32_t at = reached;
+        unsigned long long hi = (unsigned long long)__reduce_max_sync(0xffffffffu, top) + 1;
+        int c_at = 2 * kTopSel;
+        while (c_at > P.k && hi - at > 1) {
+          const uint32_t mid = (uint32_t)(at + (hi - at) / 2);
+          int c = 0;
+#pragma unroll
+          for (int j = 0; j < kSeen; ++j) c += v[j] >= mid ? 1 : 0;
+          c = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
+          if (c >= P.k) {
+            at = mid;
+            c_at = c;
+          } else {
+            hi = mid;
+          }
+        }
+        // A value that is dropped is off by as much as the k-th; the bits cut off from either are at most
+        // G 2^-23 of the k-th (of a larger value above it, which stays anyway), with as much again for
+        // these sums.
+        const float kth = key_value(at);
+        if (lane == 0) least_s = kth - 2.f * error_s - 2.f * (G * 2.384185791015625e-07f) * fabsf(kth);
+      }
+      __syncthreads();
+      least = least_s;
+    }
+    if (tid < n_sel) {
+      first = sel_key[tid] * G;
+      cols = !nonzero || !(group_value<G>(v0) < least) ? 1 : 0;  // comparisons that a NaN fails keep
+      if constexpr (GROUPS) {
+        if (!nonzero || !(v1 < least)) cols = (int)min((long long)G, P.V - first);
+        else first += (int)(__float_as_uint(v0) & (uint32_t)(G - 1));
       }
     }
-    // A value that is dropped is off by as much as the k-th; the bits cut off from either are at most G 2^-23
-    // of the k-th (of a larger value above it, which stays anyway), with as much again for these sums.
-    const float kth = key_value(at);
-    if (lane == 0) least_s = kth - 2.f * error_s - 2.f * (G * 2.384185791015625e-07f) * fabsf(kth);
-  }
-  __syncthreads();
-  if (tid < n_sel) {
-    const float least = least_s;  // comparisons that a NaN fails keep
-    first = sel_key[tid] * G;
-    cols = !nonzero || !(group_value<G>(v0) < least) ? 1 : 0;
-    if constexpr (GROUPS) {
-      if (!nonzero || !(v1 < least)) cols = (int)min((long long)G, P.V - first);
-      else first += (int)(__float_as_uint(v0) & (uint32_t)(G - 1));
+    // where this key's candidates are: exclusive scan over the threads
+    int my_at = cols;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, my_at, o);
+      if (lane >= o) my_at += y;
     }
-  }
-  // exclusive scan over the threads
-  int my_at = cols;
+    if (lane == 31) warp_s[warp] = my_at;
+    __syncthreads();
+    my_at -= cols;
+    int n_cand = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, my_at, o);
-    if (lane >= o) my_at += y;
-  }
-  if (lane == 31) warp_s[warp] = my_at;
-  __syncthreads();
-  my_at -= cols;
-  int n_cand = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      my_at += w < warp ? warp_s[w] : 0;
+      n_cand += warp_s[w];
+    }
+    // batches of candidates; the best so far take part in the next batch's ranking
+    for (int b0 = 0; b0 < n_cand; b0 += kTopBatch) {
+      const int have = n_best;
+      const int count = have + min(kTopBatch, n_cand - b0);
+      if (tid < have) {
+        cand_z[tid] = best_i[tid];
+        cand_id[tid] = best_id[tid];
+      }
+      for (int c = max(0, b0 - my_at); c < min(cols, b0 + kTopBatch - my_at); ++c)
+        cand_id[have + my_at + c - b0] = first + c;
+      __syncthreads();
+#pragma unroll 1
+      for (int i = have + warp; i < count; i += kWarps) {
+        const double z = warp_dot_exact(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);
+        if (lane == 0) cand_z[i] = ordered_i64(z);
+      }
+      __syncthreads();
+      // rank by (score descending, id ascending), four threads per candidate
+      for (int i0 = 0; i0 < count; i0 += kTopThreads / 4) {
+        const int i = i0 + tid / 4;
+        const long long z = i < count ? cand_z[i] : 0;
+        const int id = i < count ? cand_id[i] : 0;
+        int rank = 0;
+#pragma unroll 4
+        for (int j = tid % 4; j < count; j += 4) {
+          const long long o = cand_z[j];
+          rank += (o > z || (o == z && cand_id[j] < id)) ? 1 : 0;
+        }
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        if (tid % 4 == 0 && i < count && rank < P.k) {
+          best_i[rank] = z;
+          best_id[rank] = id;
+        }
+      }
+      __syncthreads();
+      n_best = min(P.k, count);
+    }
+    if (!nonzero || lo == 0u) break;  // all keys were selected
+    if (n_best == P.k) {
+      float sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    my_at += w < warp ? warp_s[w] : 0;
-    n_cand += warp_s[w];
+      for (int w = 0; w < kWarps; ++w) sum += red_s[1][w];
+      if (sum != sum) break;  // a logit is NaN, or +inf without a softcap: so is all that this row answers
+      const float kth = (float)ordered_f64(best_i[P.k - 1]);
+      least = fmaxf(least, kth - error_s - (G * 2.384185791015625e-07f) * fabsf(kth));
+    }
+    if (pos < 0) {
+      if (key_value(lo - 1u) < least) break;  // no key below lo can hold one of the k
+      pos = 0;
+    }
+    // the next of them, in order
+    n_sel = 0;
+    while (pos < n_keys && n_sel < kTopSel) {
+      const int i = pos + tid;
+      const uint32_t x = i < n_keys ? key(i) : 0xffffffffu;
+      const bool hit = x < lo && !(key_value(x) < least);
+      const unsigned ballot = __ballot_sync(0xffffffffu, hit);
+      __syncthreads();  // warp_s and next_s have been read
+      if (lane == 0) warp_s[warp] = __popc(ballot);
+      __syncthreads();
+      int slot = n_sel + __popc(ballot & ((1u << lane) - 1u)), total = 0;
+      for (int w = 0; w < kWarps; ++w) {
+        slot += w < warp ? warp_s[w] : 0;
+        total += warp_s[w];
+      }
+      if (hit && slot < kTopSel) sel_key[slot] = i;
+      if (hit && slot == kTopSel) next_s = i;
+      __syncthreads();
+      pos = n_sel + total > kTopSel ? next_s : pos + kTopThreads;
+      n_sel = min(n_sel + total, kTopSel);
+    }
+    if (n_sel == 0) break;
   }
   s = a = 0.f;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
+    m = fmaxf(m, red_s[0][w]);
     s += red_s[1][w];
     a += red_s[2][w];
   }
   const DistAcc acc{m, s, a};
   const float lse = dist_lse(acc);
-
-  // ---- batches of candidates; the best k so far take part in the next batch's ranking
-  for (int b0 = 0; b0 < n_cand; b0 += kTopBatch) {
-    const int have = b0 == 0 ? 0 : P.k;  // a batch before this one was full, so it had k
-    const int count = have + min(kTopBatch, n_cand - b0);
-    if (tid < have) {
-      cand_z[tid] = best_i[tid];
-      cand_id[tid] = best_id[tid];
-    }
-    for (int c = max(0, b0 - my_at); c < min(cols, b0 + kTopBatch - my_at); ++c) cand_id[have + my_at + c - b0] = first + c;
-    __syncthreads();
-#pragma unroll 1
-    for (int i = have + warp; i < count; i += kWarps) {
-      const double z = warp_dot_exact(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);
-      if (lane == 0) cand_z[i] = ordered_i64(z);
-    }
-    __syncthreads();
-    // rank by (score descending, id ascending), four threads per candidate
-    for (int i0 = 0; i0 < count; i0 += kTopThreads / 4) {
-      const int i = i0 + tid / 4;
-      const long long z = i < count ? cand_z[i] : 0;
-      const int id = i < count ? cand_id[i] : 0;
-      int rank = 0;
-#pragma unroll 4
-      for (int j = tid % 4; j < count; j += 4) {
-        const long long o = cand_z[j];
-        rank += (o > z || (o == z && cand_id[j] < id)) ? 1 : 0;
-      }
-      rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-      rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-      if (tid % 4 == 0 && i < count && rank < P.k) {
-        best_i[rank] = z;
-        best_id[rank] = id;
-      }
-    }
-    __syncthreads();
-  }
   if (tid < P.k) {
     double x = ordered_f64(best_i[tid]);
     // a score that is not finite (two-sums of infinities are NaN) answers NaN: the softcap would bring
