@@ -861,7 +861,10 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
       __syncthreads();
 #pragma unroll 1
       for (int i = have + warp; i < count; i += kWarps) {
-        const double z = warp_dot_exact(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);
+        const __nv_bfloat16* w = P.W + (size_t)cand_id[i] * P.d;
+        double z = warp_dot_exact(h, w, P.d, lane);
+        // two-sums of infinities are NaN; their place is that of the infinity
+        if (__any_sync(0xffffffffu, lane == 0 && z != z)) z = warp_dot(h, w, P.d, lane);
         if (lane == 0) cand_z[i] = ordered_i64(z);
       }
       __syncthreads();
@@ -933,8 +936,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
   const float lse = dist_lse(acc);
   if (tid < P.k) {
     double x = ordered_f64(best_i[tid]);
-    // a score that is not finite (two-sums of infinities are NaN) answers NaN: the softcap would bring
-    // it back to +-c
+    // a score that is not finite answers NaN: the softcap would bring it back to +-c
     if (isinf(x)) x = NAN;
     if constexpr (SAMPLE) best_z[tid] = P.cap > 0.f ? (double)P.cap * tanh(x / (double)P.cap) : x;
     else best_z[tid] = (double)softcap_exact((float)x, P.cap);

@@ -150,3 +150,23 @@ def test_long_rows_that_cancel(cuda_device, V):
     W, H = W.to(torch.bfloat16), H.to(torch.bfloat16)
     got = top_token_logps(W, H, None, k)
     assert torch.equal(got.ids.long(), Reference(W, H, None).order(k))
+
+
+@pytest.mark.parametrize("V", VOCABS)
+def test_an_infinite_logit_is_not_left_out(cuda_device, V):
+    """Under a softcap the row's other log-probabilities stay finite; the infinite score answers NaN."""
+    from gemma4_posttrain_jax_b200 import top_token_logps
+
+    k, at = 5, 1037
+    gen = torch.Generator(device=cuda_device).manual_seed(V + 4)
+    W = torch.randn((V, 64), generator=gen, device=cuda_device).to(torch.bfloat16)
+    H = torch.randn((3, 64), generator=gen, device=cuda_device).to(torch.bfloat16)
+    H[:, 9] = 1.0
+    want = Reference(W, H, 30.0).order(k)
+    W[at, 9] = float("inf")
+    got = top_token_logps(W, H, 30.0, k)
+    assert (got.ids[:, 0] == at).all() and got.logps[:, 0].isnan().all()
+    for t in range(3):
+        rest = [i for i in want[t].tolist() if i != at][: k - 1]
+        assert got.ids[t, 1:].tolist() == rest
+    assert got.logps[:, 1:].isfinite().all()
