@@ -1021,6 +1021,7 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
         z.row_ld = T;
       } else {
         z.y = y + t0;
+        z.zt = dist->zt + t0;
         z.g = dist->g != nullptr ? dist->g + t0 : nullptr;
         z.ge = dist->ge != nullptr ? dist->ge + t0 : nullptr;
         z.lse = dist->lse + t0;
@@ -1048,6 +1049,7 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
         if (row_const != nullptr) zr.row_const = z.row_const + r;
         else {
           zr.y = z.y + r;
+          zr.zt = z.zt + r;
           zr.g = z.g != nullptr ? z.g + r : nullptr;
           zr.ge = z.ge != nullptr ? z.ge + r : nullptr;
           zr.lse = z.lse + r;

@@ -313,7 +313,8 @@ __global__ void dist_gather_kernel(const int32_t* __restrict__ idx, const int* _
 
 // dZ of a chunk from kept logits (EPI_DIST_KEEP) instead of a recomputed product: reads 2 bytes and
 // writes 2 per entry, where the recompute costs 2 d flops. The same formula as EPI_DIST_DZ's; with one
-// token per row its entry is in it, too. A block takes a run of one row's columns, eight (16 bytes) per
+// token per row its entry is in it, too, from its f32 logit: where p is near 1, g - p G keeps nothing of
+// a logit in 16 bits. A block takes a run of one row's columns, eight (16 bytes) per
 // thread and step, the next step's load ahead of the arithmetic. Bound by HBM: 4 T Vs bytes. It takes
 // many warps to keep HBM busy: 3686 rows of 262144 in 727 us (5.3 TB/s; a copy of the same bytes takes
 // 575) with 2048 threads an SM, 911 with 1024 threads and four steps in flight each.
@@ -325,7 +326,7 @@ struct DistDzParams {
   const float* row_const;  // [3][row_ld], or null: one token per row and the pointers below
   long long row_ld;
   const int32_t* y;
-  const float *g, *ge, *lse, *entropy;
+  const float *zt, *g, *ge, *lse, *entropy;
   long long vocab, v_off, Vs;
   float cap;
   __nv_bfloat16* dz;
@@ -334,11 +335,9 @@ struct DistDzParams {
 };
 constexpr int kDzStep = 2048;  // columns of a block's step
 
-// Eight entries whose columns are kept by y = 2 x / c in base 2 (keep_raw), the one of place `at`
-// with gv. With e = 2^y, r = 1 / (1 + e): z = c (1 - 2 r) and softcap' = 4 e r^2, near 0 too. Out of
+// Eight entries whose columns are kept by y = 2 x / c in base 2 (keep_raw). With e = 2^y, r = 1 / (1 + e): z = c (1 - 2 r) and softcap' = 4 e r^2, near 0 too. Out of
 // line: rare, and the common path has no registers to spare.
-__device__ __noinline__ uint4 dist_dz_raw(uint4 kept, float slot, float cap, float a, float b, float l2, float gv,
-                                          int at) {
+__device__ __noinline__ uint4 dist_dz_raw(uint4 kept, float slot, float cap, float a, float b, float l2) {
   const uint32_t w[4] = {kept.x, kept.y, kept.z, kept.w};
   float y0, step;
   keep_raw_range(slot, y0, step);
@@ -350,9 +349,17 @@ __device__ __noinline__ uint4 dist_dz_raw(uint4 kept, float slot, float cap, flo
     const float e = fast_ex2(fmaf((float)n, step, y0));
     const float r = fast_rcp(1.f + e);
     const float lp = fmaf(-2.f * c2, r, c2 - l2);
-    v[j] = 4.f * e * r * r * ((j == at ? gv : 0.f) - fast_ex2(lp) * fmaf(b, lp, a));
+    v[j] = -4.f * e * r * r * (fast_ex2(lp) * fmaf(b, lp, a));
   }
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// The entry of a token whose slots' gradients sum to `sum`, from its f32 logit, rounded once:
+// softcap'(z) * (sum - p * (a + b log2 p)), softcap'(z) = 1 - (z / c)^2.
+__device__ __forceinline__ __nv_bfloat16 dist_dz_given(float z, float cap, float a, float b, float l2, float sum) {
+  const float lp = fmaf(z, kLog2e, -l2);
+  const float u = cap > 0.f ? z / cap : 0.f;
+  return __float2bfloat16_rn(fmaf(-u, u, 1.f) * (sum - exp2f(lp) * fmaf(b, lp, a)));
 }
 
 __global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
@@ -400,44 +407,40 @@ __global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
       q = __ldcs(reinterpret_cast<const uint4*>(kept + col + kDzStep));
       mx = __ldg(kept_max + (col + kDzStep) / 32);
     }
-    if (kept_raw(m)) {
-      *reinterpret_cast<uint4*>(dz + col) =
-          dist_dz_raw(make_uint4(w[0], w[1], w[2], w[3]), m, P.cap, a, b, l2, gv, yc - col);
-      continue;
-    }
-    const f32x2 top = two(m);
     uint32_t out[4];
+    if (kept_raw(m)) {
+      const uint4 v = dist_dz_raw(make_uint4(w[0], w[1], w[2], w[3]), m, P.cap, a, b, l2);
+      out[0] = v.x;
+      out[1] = v.y;
+      out[2] = v.z;
+      out[3] = v.w;
+    } else {
+      const f32x2 top = two(m);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      // 2^23 + n, whose low bits are n, less 2^23
-      const f32x2 n = add_f32x2(pack_f32x2(__uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7610)),
-                                           __uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7632))),
-                                m23);
-      const f32x2 z = fma_f32x2(n, mstep2, top);
-      const f32x2 lp = add_f32x2(z, ml2);
-      const f32x2 u = mul_f32x2(z, ucap2);
-      float l0, l1, v0, v1;
-      unpack_f32x2(lp, l0, l1);
-      // p (a + b log2 p) (u^2 - 1)
-      const f32x2 v = mul_f32x2(mul_f32x2(pack_f32x2(fast_ex2(l0), fast_ex2(l1)), fma_f32x2(b2, lp, a2)),
-                                fma_f32x2(u, u, mone));
-      unpack_f32x2(v, v0, v1);
-      out[j] = pack_bf16x2(v0, v1);
+      for (int j = 0; j < 4; ++j) {
+        // 2^23 + n, whose low bits are n, less 2^23
+        const f32x2 n = add_f32x2(pack_f32x2(__uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7610)),
+                                             __uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7632))),
+                                  m23);
+        const f32x2 z = fma_f32x2(n, mstep2, top);
+        const f32x2 lp = add_f32x2(z, ml2);
+        const f32x2 u = mul_f32x2(z, ucap2);
+        float l0, l1, v0, v1;
+        unpack_f32x2(lp, l0, l1);
+        // p (a + b log2 p) (u^2 - 1)
+        const f32x2 v = mul_f32x2(mul_f32x2(pack_f32x2(fast_ex2(l0), fast_ex2(l1)), fma_f32x2(b2, lp, a2)),
+                                  fma_f32x2(u, u, mone));
+        unpack_f32x2(v, v0, v1);
+        out[j] = pack_bf16x2(v0, v1);
+      }
     }
     // rows of dZ are padded to 16 bytes
     *reinterpret_cast<uint4*>(dz + col) = make_uint4(out[0], out[1], out[2], out[3]);
-    if ((unsigned)(yc - col) < 8u) {
-      // the row's token: its entry again, with its gradient
-      const float z = fmaf((float)kept[yc], -step, m);
-      const float lp = z - l2, u = z * ucap;
-      dz[yc] = __float2bfloat16_rn((fmaf(b, lp, a) * fast_ex2(lp) - gv) * fmaf(u, u, -1.f));
-    }
+    if ((unsigned)(yc - col) < 8u) dz[yc] = dist_dz_given(P.zt[t], P.cap, a, b, l2, gv);
   }
 }
 
-// The given tokens' entries of a chunk's dZ, computed from their f32 logits and rounded once:
-//   dZ[t, y] = softcap'(z) * (sum of g over the row's slots that hold y - p * (a + b log2 p))
-// softcap'(z) = 1 - (z / c)^2. The first slot of a token writes the entry, so a token that a row
+// The given tokens' entries of a chunk's dZ, `sum` over the row's slots that hold the token. The first slot of a token writes the entry, so a token that a row
 // names twice is written once, with both gradients.
 __global__ void dist_dz_targets_kernel(const int32_t* __restrict__ y, const float* __restrict__ zt,
                                        const float* __restrict__ g, const float* __restrict__ row_const,
@@ -456,11 +459,8 @@ __global__ void dist_dz_targets_kernel(const int32_t* __restrict__ y, const floa
   if (g != nullptr)
     for (int j = k; j < K; ++j)
       if (yt[j] == id) sum += g[(size_t)t * K + j];
-  const float z = zt[i];
-  const float lp = fmaf(z, kLog2e, -row_const[2 * row_ld + t]);
-  const float u = cap > 0.f ? z / cap : 0.f;
-  const float w = fmaf(row_const[row_ld + t], lp, row_const[t]);
-  dz[(size_t)t * ldz + v] = __float2bfloat16_rn(fmaf(-u, u, 1.f) * (sum - exp2f(lp) * w));
+  dz[(size_t)t * ldz + v] =
+      dist_dz_given(zt[i], cap, row_const[t], row_const[row_ld + t], row_const[2 * row_ld + t], sum);
 }
 
 // ----------------------------------------------------------------------------- selection
