@@ -335,21 +335,30 @@ struct DistDzParams {
 };
 constexpr int kDzStep = 2048;  // columns of a block's step
 
-// Eight entries whose columns are kept by y = 2 x / c in base 2 (keep_raw). With e = 2^y, r = 1 / (1 + e): z = c (1 - 2 r) and softcap' = 4 e r^2, near 0 too. Out of
-// line: rare, and the common path has no registers to spare.
-__device__ __noinline__ uint4 dist_dz_raw(uint4 kept, float slot, float cap, float a, float b, float l2) {
+// Eight entries of columns of which one is far (keep_far). By y, with e = 2^y and r = 1 / (1 + e):
+// z = c (1 - 2 r) and softcap' = 4 e r^2, near 0 too.
+__device__ __forceinline__ uint4 dist_dz_far(uint4 kept, float slot, float cap, float a, float b, float l2) {
   const uint32_t w[4] = {kept.x, kept.y, kept.z, kept.w};
-  float y0, step;
-  keep_raw_range(slot, y0, step);
   const float c2 = cap * kLog2e;
+  const float top = kept_far_top(slot, c2), step = keep_range(c2) / 32767.f;
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const uint32_t n = (j & 1) ? w[j / 2] >> 16 : w[j / 2] & 0xffffu;
-    const float e = fast_ex2(fmaf((float)n, step, y0));
-    const float r = fast_rcp(1.f + e);
-    const float lp = fmaf(-2.f * c2, r, c2 - l2);
-    v[j] = -4.f * e * r * r * (fast_ex2(lp) * fmaf(b, lp, a));
+    float lp, slope;
+    if (n & 0x8000u) {
+      const float y = fmaf((float)(n & 0x3fffu), kKeepFarUnit, kKeepFarFrom);
+      const float e = fast_ex2(n & 0x4000u ? -y : y);
+      const float r = fast_rcp(1.f + e);
+      lp = fmaf(-2.f * c2, r, c2 - l2);
+      slope = 4.f * e * r * r;
+    } else {
+      const float z = fmaf((float)n, -step, top);
+      const float u = z / c2;
+      lp = z - l2;
+      slope = fmaf(-u, u, 1.f);
+    }
+    v[j] = -slope * (fast_ex2(lp) * fmaf(b, lp, a));
   }
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
@@ -398,7 +407,7 @@ __global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
   auto two = [](float x) { return pack_f32x2(x, x); };
   const f32x2 a2 = two(a), b2 = two(b), ml2 = two(-l2), ucap2 = two(ucap), mstep2 = two(-step), m23 = two(-8388608.f),
               mone = two(-1.f);
-  const int yc = yl >= 0 && yl < P.Vs ? (int)yl : -8;  // the row's token among this shard's columns
+  bool far = false;
 #pragma unroll 1
   for (int col = c0; col < end; col += kDzStep) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -407,37 +416,42 @@ __global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
       q = __ldcs(reinterpret_cast<const uint4*>(kept + col + kDzStep));
       mx = __ldg(kept_max + (col + kDzStep) / 32);
     }
+    far |= kept_far(m);
+    const f32x2 top = two(m);
     uint32_t out[4];
-    if (kept_raw(m)) {
-      const uint4 v = dist_dz_raw(make_uint4(w[0], w[1], w[2], w[3]), m, P.cap, a, b, l2);
-      out[0] = v.x;
-      out[1] = v.y;
-      out[2] = v.z;
-      out[3] = v.w;
-    } else {
-      const f32x2 top = two(m);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // 2^23 + n, whose low bits are n, less 2^23
-        const f32x2 n = add_f32x2(pack_f32x2(__uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7610)),
-                                             __uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7632))),
-                                  m23);
-        const f32x2 z = fma_f32x2(n, mstep2, top);
-        const f32x2 lp = add_f32x2(z, ml2);
-        const f32x2 u = mul_f32x2(z, ucap2);
-        float l0, l1, v0, v1;
-        unpack_f32x2(lp, l0, l1);
-        // p (a + b log2 p) (u^2 - 1)
-        const f32x2 v = mul_f32x2(mul_f32x2(pack_f32x2(fast_ex2(l0), fast_ex2(l1)), fma_f32x2(b2, lp, a2)),
-                                  fma_f32x2(u, u, mone));
-        unpack_f32x2(v, v0, v1);
-        out[j] = pack_bf16x2(v0, v1);
-      }
+    for (int j = 0; j < 4; ++j) {
+      // 2^23 + n, whose low bits are n, less 2^23
+      const f32x2 n = add_f32x2(pack_f32x2(__uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7610)),
+                                           __uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7632))),
+                                m23);
+      const f32x2 z = fma_f32x2(n, mstep2, top);
+      const f32x2 lp = add_f32x2(z, ml2);
+      const f32x2 u = mul_f32x2(z, ucap2);
+      float l0, l1, v0, v1;
+      unpack_f32x2(lp, l0, l1);
+      // p (a + b log2 p) (u^2 - 1)
+      const f32x2 v = mul_f32x2(mul_f32x2(pack_f32x2(fast_ex2(l0), fast_ex2(l1)), fma_f32x2(b2, lp, a2)),
+                                fma_f32x2(u, u, mone));
+      unpack_f32x2(v, v0, v1);
+      out[j] = pack_bf16x2(v0, v1);
     }
     // rows of dZ are padded to 16 bytes
     *reinterpret_cast<uint4*>(dz + col) = make_uint4(out[0], out[1], out[2], out[3]);
-    if ((unsigned)(yc - col) < 8u) dz[yc] = dist_dz_given(P.zt[t], P.cap, a, b, l2, gv);
   }
+  // Rare: this thread's far columns, once more. Here, not above, where they would take registers that
+  // the loop's loads in flight need (809 instead of 727 us).
+  if (far) {
+#pragma unroll 1
+    for (int col = c0; col < end; col += kDzStep) {
+      const float m = kept_max[col / 32];
+      if (kept_far(m))
+        *reinterpret_cast<uint4*>(dz + col) =
+            dist_dz_far(*reinterpret_cast<const uint4*>(kept + col), m, P.cap, a, b, l2);
+    }
+  }
+  // the row's token, where this thread has written its entry
+  if (yl >= c0 && yl < end && (yl - c0) % kDzStep < 8) dz[yl] = dist_dz_given(P.zt[t], P.cap, a, b, l2, gv);
 }
 
 // The given tokens' entries of a chunk's dZ, `sum` over the row's slots that hold the token. The first slot of a token writes the entry, so a token that a row

@@ -424,14 +424,17 @@ __device__ __forceinline__ void dist_accumulate(const float (&z)[32], int nvalid
 // A kept logit is off by at most 3.7e-4 * ln2, so a probability by 2.5e-4 of itself, a fifteenth of
 // what the bf16 rounding of dZ that follows may add; what lies further below is kept at 2^-48 of the
 // largest. The largest itself is kept exactly (f32).
-// softcap' = 1 - (z / c)^2 takes more where it is near 0: columns of which one reaches |y| > kKeepRawFrom,
-// y = 2 x / c in base 2 (softcap' < 0.061; above it the steps are 5e-4 of softcap' at most), are kept by y
-// instead, in 65535 steps of the range they take. The largest's place then holds a NaN with that range's
-// ends, rounded outward to 1 / 2047 of +-kKeepRawMax (beyond, softcap' is below f32's rounding of z / c).
+// softcap' = 1 - (z / c)^2 takes more where it is near 0. With y = 2 x / c in base 2, columns of which one
+// has |y| > kKeepFarFrom (softcap' < 0.061) are kept in 15 bits and a mark: those with such a y by its sign
+// and 14 bits of its size up to kKeepFarMax (beyond, softcap' is below f32's rounding of z / c), which is
+// 4.2e-4 of softcap' at most and 1.3e-5 c of the logit; the others by the distance as above, in 32767
+// steps, below the largest of theirs (5.1e-4 of the logit and of a probability, 2 / c of that of softcap').
+// The largest's place then holds a NaN with that one, rounded up to 22 bits.
 constexpr float kKeepRange = 48.f;
-constexpr float kKeepRawFrom = 6.f;
-constexpr float kKeepRawMax = 26.f;
-constexpr float kKeepRawUnit = 2.f * kKeepRawMax / 2047.f;
+constexpr float kKeepFarFrom = 6.f;
+constexpr float kKeepFarMax = 26.f;
+constexpr float kKeepFarUnit = (kKeepFarMax - kKeepFarFrom) / 16383.f;
+constexpr float kKeepTopUnits = 4194303.f;
 __device__ __forceinline__ float keep_range(float c2) { return c2 > 0.f ? fminf(kKeepRange, 2.f * c2) : kKeepRange; }
 __device__ __forceinline__ void keep_logits(const float (&z)[32], float mx, float range, float per_unit,
                                             uint32_t (&pk)[16]) {
@@ -443,34 +446,34 @@ __device__ __forceinline__ void keep_logits(const float (&z)[32], float mx, floa
     pk[j] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
   }
 }
-// By y; returns what takes the largest's place. Columns of vocabulary padding are 0.
-__device__ __forceinline__ float keep_raw(const uint32_t (&r)[32], float k1, uint32_t (&pk)[16]) {
-  float lo = kKeepRawMax, hi = -kKeepRawMax;
+// With the far columns by y; returns what takes the largest's place. Only the first nvalid columns count.
+__device__ __forceinline__ float keep_far(const uint32_t (&r)[32], const float (&z)[32], int nvalid, float k1, float c2,
+                                          float range, uint32_t (&pk)[16]) {
+  float top = -c2;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j < nvalid && fabsf(__uint_as_float(r[j]) * k1) <= kKeepFarFrom) top = fmaxf(top, z[j]);
+  const float units = fminf(ceilf((top + c2) * (kKeepTopUnits / (2.f * c2))), kKeepTopUnits);
+  top = fmaf(units, 2.f * c2 / kKeepTopUnits, -c2);
+  const float per_unit = 32767.f / range;
+  uint32_t n[32];
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
     const float y = __uint_as_float(r[j]) * k1;
-    lo = fminf(lo, y);
-    hi = fmaxf(hi, y);
+    const bool far = !(fabsf(y) <= kKeepFarFrom);
+    const float steps = far ? (fminf(fabsf(y), kKeepFarMax) - kKeepFarFrom) * (1.f / kKeepFarUnit)
+                            : fminf(fmaxf(top - z[j], 0.f), range) * per_unit;
+    // the low bits of 2^23 + n are n
+    n[j] = __float_as_uint(steps + 8388608.f) | (far ? (y < 0.f ? 0xc000u : 0x8000u) : 0u);
   }
-  const int a = max((int)floorf((lo + kKeepRawMax) * (1.f / kKeepRawUnit)), 0);
-  const int b = min((int)ceilf((hi + kKeepRawMax) * (1.f / kKeepRawUnit)), 2047);
-  const float y0 = fmaf((float)a, kKeepRawUnit, -kKeepRawMax), range = (float)(b - a) * kKeepRawUnit;
-  const float per_unit = range > 0.f ? 65535.f / range : 0.f;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const float n0 = fminf(fmaxf(fmaf(__uint_as_float(r[2 * j]), k1, -y0), 0.f), range);
-    const float n1 = fminf(fmaxf(fmaf(__uint_as_float(r[2 * j + 1]), k1, -y0), 0.f), range);
-    pk[j] = __byte_perm(__float_as_uint(fmaf(n0, per_unit, 8388608.f)), __float_as_uint(fmaf(n1, per_unit, 8388608.f)),
-                        0x5410);
-  }
-  return __uint_as_float(0x7fc00000u | (uint32_t)a << 11 | (uint32_t)b);
+  for (int j = 0; j < 16; ++j) pk[j] = __byte_perm(n[2 * j], n[2 * j + 1], 0x5410);
+  return __uint_as_float(0x7fc00000u | (uint32_t)units);
 }
-__device__ __forceinline__ bool kept_raw(float mx) { return (__float_as_uint(mx) & 0x7fc00000u) == 0x7fc00000u; }
-__device__ __forceinline__ void keep_raw_range(float mx, float& y0, float& step) {
-  const uint32_t bits = __float_as_uint(mx);
-  const int a = (int)(bits >> 11 & 2047u), b = (int)(bits & 2047u);
-  y0 = fmaf((float)a, kKeepRawUnit, -kKeepRawMax);
-  step = (float)(b - a) * (kKeepRawUnit / 65535.f);
+__device__ __forceinline__ bool kept_far(float mx) { return (__float_as_uint(mx) & 0x7fc00000u) == 0x7fc00000u; }
+// The largest of the columns kept by their distance.
+__device__ __forceinline__ float kept_far_top(float mx, float c2) {
+  return fmaf((float)(__float_as_uint(mx) & 0x3fffffu), 2.f * c2 / kKeepTopUnits, -c2);
 }
 
 // The two largest of every G of 32 accumulator columns. The order is that of x (softcap is
@@ -1145,7 +1148,7 @@ __global__ void __launch_bounds__(num_threads<EPI>(), 1)
 #pragma unroll
                   for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(__uint_as_float(r[j])));
                 }
-                if (HAS_CAP && most * k1 > kKeepRawFrom) mx = keep_raw(r, k1, pk);
+                if (HAS_CAP && most * k1 > kKeepFarFrom) mx = keep_far(r, z, nvalid, k1, c2, keep, pk);
                 else keep_logits(z, mx, keep, keep_per_unit, pk);
                 if (lane == 0) bulk_wait_read<1>();
                 __syncwarp();

@@ -58,3 +58,35 @@ def test_given_token_that_is_nearly_certain(cuda_device, softcap, far, K, keep):
     # 1 - p by that times p; the slope, 1 - (z / c)^2 in f32, is off by 2^-21
     off = 2.02 * 2**-8 * want + slope * p * 2**-21 * (z.abs() + softcap + 1) + 2**-21 * (1 - p)
     within(got.reshape(1), want.reshape(1), off.reshape(1), "d logit of the target")
+
+
+@pytest.mark.parametrize("softcap", [5.0, 30.0, 300.0])
+@pytest.mark.parametrize("far", [-9.0, -2.5, 2.5])
+@pytest.mark.parametrize("K", [1, 2])
+@pytest.mark.parametrize("keep", [True, False])
+def test_ordinary_logits_beside_a_saturated_one(cuda_device, softcap, far, K, keep):
+    """One of every 32 neighbours is far beyond the softcap; the other 31 keep their accuracy."""
+    V = 640
+    gen = torch.Generator(device=cuda_device).manual_seed(int(softcap) + 11)
+    logits = torch.randn((V,), generator=gen, device=cuda_device) * min(3.0, softcap / 4)
+    logits[::32] = far * softcap
+    ordinary = torch.arange(V, device=cuda_device) % 32 != 0
+    W, H = _one_position(cuda_device, logits)
+    y = torch.tensor([[70, -1][:K]], device=cuda_device)
+    g, ge = torch.tensor([[1.5, 1.0][:K]], device=cuda_device), torch.tensor([0.5], device=cuda_device)
+    got = _dz_of(W, H, y, g, ge, softcap, keep)
+    ref = Reference(W, H, softcap)
+    slope = 1 - (ref.z[0] / softcap) ** 2
+    E, lp, p = ref.entropy[0], ref.logp[0], ref.p[0]
+    hot = torch.zeros_like(p)
+    hot[70] = 1.5
+    want = slope * (hot - p * (1.5 + 0.5 * (lp + E)))
+    # Two roundings to bf16. A logit kept in 15 bits over a range of 48 ln2 at most is off by half a step, 5.1e-4:
+    # p by that of itself, log p by that, the slope, 1 - (z / c)^2, by 2 |z| / c^2 times that. f32's share: 2^-18.
+    # What lies further below the group's largest than the range is at 2^-48 of it.
+    half = 5.1e-4
+    raw = hot + p * (1.5 + 0.5 * (lp.abs() + E))
+    off = 2.02 * 2**-8 * want.abs() + slope * p * half * (1.5 + 0.5 * (lp.abs() + E) + 0.5)
+    off = off + 2 * ref.z[0].abs() / softcap**2 * half * p * (1.5 + 0.5 * (lp.abs() + E)) + 2**-18 * raw
+    off = off + 2**-47 * (1.5 + 0.5 * (40 + E)) + 1e-30
+    within(got[ordinary], want[ordinary], off[ordinary], "d logits")
