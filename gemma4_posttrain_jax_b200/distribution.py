@@ -202,6 +202,8 @@ def token_logps_and_entropy(
         raise ValueError(f"at most {_lib.LP_DIST_MAX_TOKENS} tokens per position, got {K}")
     if mesh is not None and mesh.size > 1 and mesh.axis_names != ("d",):
         raise ValueError(f"vocab-parallel mesh needs axis 'd': {mesh.axis_names}")
+    if not torch.is_grad_enabled():
+        keep_logits = False  # autograd.Function cannot see it: its forward is always outside grad mode
     leaves = [x for x in (embed_tokens, hidden) if x.requires_grad and x.is_leaf] if torch.is_grad_enabled() else []
     capturing = bool(leaves) and hidden.is_cuda and torch.cuda.is_current_stream_capturing()
     if capturing and any(ref() is x for node in _eager_graphs for ref in node.leaves for x in leaves):

@@ -11,6 +11,7 @@ from gemma4_posttrain_jax_b200 import (
     _lib,
     build,
     completion_logps_and_entropy,
+    distribution,
     sample_top_k,
     token_logps_and_entropy,
     top_token_logps,
@@ -163,3 +164,22 @@ def test_c_entries_refuse_before_the_device(lib):
     refused(draw(top_p=0.0), "top_p")
     refused(draw(top_p=1.5), "top_p")
     refused(draw(uniform=None), "null uniform")
+
+
+def test_no_logits_are_kept_where_no_gradient_can_follow(lib, monkeypatch):
+    """Scoring under no_grad, with parameters that otherwise train, leaves nothing for a backward."""
+    kept_calls = []
+
+    def forward(embed, hidden, tokens, softcap, logp, entropy, saved, kept=None):
+        kept_calls.append(kept is not None)
+        logp.zero_(), entropy.zero_()
+
+    monkeypatch.setattr(distribution.ops, "dist_forward", forward)
+    for embed, hidden in ((W.clone().requires_grad_(), H), (W, H.clone().requires_grad_())):
+        for keep in (None, True):
+            logps, entropy = token_logps_and_entropy(embed, hidden, Y, softcap=30.0, keep_logits=keep)
+            assert logps.requires_grad and entropy.requires_grad
+            with torch.no_grad():
+                token_logps_and_entropy(embed, hidden, Y, softcap=30.0, keep_logits=keep)
+            token_logps_and_entropy(embed.detach(), hidden.detach(), Y, softcap=30.0, keep_logits=keep)
+    assert kept_calls == [True, False, False] * 4
