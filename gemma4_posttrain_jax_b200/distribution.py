@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import math
 import operator
+import threading
 import weakref
 from typing import NamedTuple
 
@@ -139,8 +140,26 @@ def _dist_gradients(ctx, g, ge):
 _once = once_differentiable(_dist_gradients)
 
 
-# Autograd nodes of this operator's eager calls that are still alive, each with its leaves.
-_eager_graphs: weakref.WeakSet = weakref.WeakSet()
+class _EagerGraphs:
+    """Autograd nodes of this operator's eager calls that are still alive, each with its leaves. Calls of
+    several threads may add to it while others look."""
+
+    def __init__(self):
+        self._nodes: weakref.WeakSet = weakref.WeakSet()
+        self._lock = threading.RLock()
+
+    def add(self, node, leaves: list[torch.Tensor]) -> None:
+        node.leaves = [weakref.ref(x) for x in leaves]
+        with self._lock:
+            self._nodes.add(node)
+
+    def holds(self, leaves: list[torch.Tensor]) -> bool:
+        with self._lock:
+            nodes = list(self._nodes)
+        return any(ref() is x for node in nodes for ref in node.leaves for x in leaves)
+
+
+_eager_graphs = _EagerGraphs()
 
 # Logits are kept for the backward up to this many bytes (8064 rows of a vocabulary of 262144), the
 # size of the backward's own dZ scratch.
@@ -206,7 +225,7 @@ def token_logps_and_entropy(
         keep_logits = False  # autograd.Function cannot see it: its forward is always outside grad mode
     leaves = [x for x in (embed_tokens, hidden) if x.requires_grad and x.is_leaf] if torch.is_grad_enabled() else []
     capturing = bool(leaves) and hidden.is_cuda and torch.cuda.is_current_stream_capturing()
-    if capturing and any(ref() is x for node in _eager_graphs for ref in node.leaves for x in leaves):
+    if capturing and _eager_graphs.holds(leaves):
         raise RuntimeError(
             "token_logps_and_entropy: an eager graph of the same leaves is alive; free it (or use detached leaves) "
             "before capturing this call"
@@ -216,8 +235,7 @@ def token_logps_and_entropy(
         dh_reduce_f32, skip_zero_grad, keep_logits,
     )
     if leaves and not capturing:
-        logps.grad_fn.leaves = [weakref.ref(x) for x in leaves]
-        _eager_graphs.add(logps.grad_fn)
+        _eager_graphs.add(logps.grad_fn, leaves)
     return logps, entropy
 
 

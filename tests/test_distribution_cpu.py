@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -183,3 +184,34 @@ def test_no_logits_are_kept_where_no_gradient_can_follow(lib, monkeypatch):
                 token_logps_and_entropy(embed, hidden, Y, softcap=30.0, keep_logits=keep)
             token_logps_and_entropy(embed.detach(), hidden.detach(), Y, softcap=30.0, keep_logits=keep)
     assert kept_calls == [True, False, False] * 4
+
+
+def test_captures_look_at_the_eager_graphs_while_other_threads_add_to_them():
+    """A thread's eager call may finish while another thread's captured one looks for graphs of its leaves."""
+
+    class Node:
+        def __init__(self, *leaves):
+            self.leaves = leaves
+
+    leaf, other = W.clone(), W.clone()
+    threads, nodes = [], [Node(), Node(), Node()]
+
+    def added_meanwhile():  # stands for a weak reference
+        nodes.append(Node())
+        threads.append(threading.Thread(target=distribution._eager_graphs.add, args=(nodes[-1], [other])))
+        threads[-1].start()
+        threads[-1].join(0.2)
+
+    try:
+        for node in nodes[:3]:
+            distribution._eager_graphs.add(node, [other])
+            node.leaves = (added_meanwhile,)
+        assert not distribution._eager_graphs.holds([leaf])
+        for thread in threads:
+            thread.join(10)
+            assert not thread.is_alive()
+        assert len(threads) == 3 and distribution._eager_graphs.holds([other])
+    finally:
+        nodes.clear()
+        threads.clear()
+    assert not distribution._eager_graphs.holds([other])
