@@ -275,7 +275,9 @@ def completion_logps_and_entropy(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``completion_logps`` with the entropy: (logps [B, N], entropy [B, N]) of the completion tokens of
     hidden [B, P + N, d], differentiable, computed at the valid slots only and 0 elsewhere. The host
-    waits once for the number of valid slots. ``options`` are those of ``token_logps_and_entropy``.
+    waits once for the number of valid slots, so the call cannot be captured into a CUDA graph and is
+    refused there (``token_logps_and_entropy``, with -1 for the tokens of the other slots, can be).
+    ``options`` are those of ``token_logps_and_entropy``.
     """
     if hidden.ndim != 3 or completion_ids.ndim != 2 or completion_mask.shape != completion_ids.shape:
         raise ValueError("hidden must be [B, S, d] and completion ids / mask [B, N]")
@@ -285,6 +287,11 @@ def completion_logps_and_entropy(
         raise ValueError("prompt_width and completion width do not fit the hidden sequence")
     _check_embed(embed_tokens, hidden)
     _validate_softcap(softcap)
+    if hidden.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(
+            "completion_logps_and_entropy waits for the number of valid slots and cannot be captured; capture "
+            "token_logps_and_entropy with -1 for the tokens of the other slots"
+        )
     rows = hidden
     if hidden.stride(-1) != 1 or hidden.stride(0) % 8 or hidden.stride(1) % 8 or hidden.data_ptr() % 16:
         rows = hidden.contiguous()

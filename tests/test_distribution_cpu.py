@@ -215,3 +215,16 @@ def test_captures_look_at_the_eager_graphs_while_other_threads_add_to_them():
         nodes.clear()
         threads.clear()
     assert not distribution._eager_graphs.holds([other])
+
+
+def test_completions_refuse_a_capture(monkeypatch):
+    """They wait for the number of valid slots, which a stream that is captured must not."""
+
+    class OnGpu(torch.Tensor):
+        is_cuda = property(lambda self: True)
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        completion_logps_and_entropy(
+            W, H.as_subclass(OnGpu), torch.zeros((2, 2), dtype=torch.int64), torch.ones((2, 2), dtype=torch.bool), prompt_width=2, softcap=30.0
+        )
