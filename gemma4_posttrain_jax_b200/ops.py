@@ -622,12 +622,15 @@ def compact(
                 raise ValueError("ids must match the mask shape")
             ids = ids.to(torch.int32).contiguous()
             yc = torch.empty((B * N,), dtype=torch.int32, device=dev)
-    ws, wsp, wsn = _workspace(lib.lp_compact_workspace_bytes(B, N), dev)
-    rc = lib.lp_compact(
-        _stream(dev), _ptr(m), B, N, _ptr(hidden), hb, hr, int(row_offset), d, _ptr(ids), _ptr(Hc), _ptr(yc), _ptr(idx),
-        _ptr(pos), _ptr(count), wsp, wsn,
-    )
-    _lib.check(rc, "lp_compact")
+
+    def call(stream):
+        ws, wsp, wsn = _workspace(lib.lp_compact_workspace_bytes(B, N), dev)
+        return lib.lp_compact(
+            stream, _ptr(m), B, N, _ptr(hidden), hb, hr, int(row_offset), d, _ptr(ids), _ptr(Hc), _ptr(yc), _ptr(idx),
+            _ptr(pos), _ptr(count), wsp, wsn,
+        )
+
+    _on_device(dev, "lp_compact", call)
     return Hc, yc, idx, pos, count
 
 
@@ -666,11 +669,10 @@ def scatter_rows(src: torch.Tensor, pos: torch.Tensor, out: torch.Tensor) -> tor
     # an empty src is never read (every pos is -1); any valid pointer stands in for it
     src_ptr = _ptr(s2) if s2.shape[0] > 0 else _ptr(out)
     src_ld = int(s2.stride(0)) if s2.shape[0] > 0 else width
-    rc = lib.lp_scatter_rows(
-        _stream(dev), src_ptr, src_ld, _ptr(p), slots, width, src.element_size(), _ptr(out), row_stride,
-        rows_per_group, group_stride, out.element_size(),
-    )
-    _lib.check(rc, "lp_scatter_rows")
+    _on_device(dev, "lp_scatter_rows", lambda stream: lib.lp_scatter_rows(
+        stream, src_ptr, src_ld, _ptr(p), slots, width, src.element_size(), _ptr(out), row_stride, rows_per_group,
+        group_stride, out.element_size(),
+    ))
     return out
 
 

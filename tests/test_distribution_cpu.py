@@ -228,3 +228,50 @@ def test_completions_refuse_a_capture(monkeypatch):
         completion_logps_and_entropy(
             W, H.as_subclass(OnGpu), torch.zeros((2, 2), dtype=torch.int64), torch.ones((2, 2), dtype=torch.bool), prompt_width=2, softcap=30.0
         )
+
+
+def test_compaction_and_scatter_run_on_the_device_of_their_tensors(monkeypatch):
+    """The rows of completions on another device than the current one: their kernels are launched with that
+    device current, on its stream, as the distribution kernels are."""
+    ops = distribution.ops
+    calls = []
+
+    class Lib:
+        lp_compact_workspace_bytes = staticmethod(lambda B, N: 256)
+        lp_compact = staticmethod(lambda stream, *args: calls.append(("lp_compact", stream)) or _lib.LP_OK)
+        lp_scatter_rows = staticmethod(lambda stream, *args: calls.append(("lp_scatter_rows", stream)) or _lib.LP_OK)
+
+    def on_device(dev, what, call):
+        calls.append((what, dev))
+        assert call("its stream") == _lib.LP_OK
+
+    cpu = torch.device("cpu")
+    monkeypatch.setattr(ops._lib, "load", Lib)
+    monkeypatch.setattr(ops, "_require_cuda", lambda *tensors: cpu)
+    monkeypatch.setattr(ops, "_on_device", on_device)
+    ops.compact(torch.ones((2, 2), dtype=torch.bool), H, torch.zeros((2, 2), dtype=torch.int64), row_offset=1)
+    ops.scatter_rows(H[0], torch.zeros(4, dtype=torch.int32), torch.zeros((4, 16), dtype=torch.bfloat16))
+    assert calls == [("lp_compact", cpu), ("lp_compact", "its stream"), ("lp_scatter_rows", cpu), ("lp_scatter_rows", "its stream")]
+
+
+def test_kernels_run_with_the_device_of_their_tensors_current(monkeypatch):
+    ops = distribution.ops
+    current = [0]
+
+    class Current:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            current.append(self.dev.index)
+
+        def __exit__(self, *exc):
+            current.pop()
+
+    monkeypatch.setattr(ops, "_current_device", lambda: current[-1])
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: f"stream of {index}")
+    monkeypatch.setattr(torch.cuda, "device", Current)
+    seen = []
+    for index in (0, 1):
+        ops._on_device(torch.device("cuda", index), "a kernel", lambda stream: seen.append((stream, current[-1])) or _lib.LP_OK)
+    assert seen == [("stream of 0", 0), ("stream of 1", 1)] and current == [0]
