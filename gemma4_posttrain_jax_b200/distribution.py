@@ -5,7 +5,10 @@ log-probability: any number of given tokens per position (a distillation or KL t
 teacher's alternatives) and the entropy of the policy (an entropy bonus), with the gradients of
 both; ``completion_logps_and_entropy`` is its caller for completions, as ``completion_logps`` is
 ``per_token_logps``'. ``top_token_logps`` gives such alternatives: the k most likely tokens of each position.
-Neither writes a ``[..., vocab]`` array of probabilities. The reference has no counterpart.
+Neither writes ``[..., vocab]`` probabilities. What is written of that shape: the logits in 16 bits that a
+differentiable call keeps for its backward, where they take at most 4 GiB; that backward's dZ, a chunk of
+rows at a time; and the f32 logits of a vocabulary of a few thousand that ``top_token_logps`` searches.
+The reference has no counterpart.
 """
 
 from __future__ import annotations
@@ -161,8 +164,8 @@ class _EagerGraphs:
 
 _eager_graphs = _EagerGraphs()
 
-# Logits are kept for the backward up to this many bytes (8064 rows of a vocabulary of 262144), the
-# size of the backward's own dZ scratch.
+# Logits are kept for the backward up to this many bytes (7710 rows of a vocabulary of 262144, 16 bits
+# each and an f32 for every 32), the size of the backward's own dZ scratch.
 _KEPT_MAX_BYTES = 4 << 30
 
 # Rows without a gradient add nothing, and a backward of at least this much work (about 3 ms)
@@ -193,15 +196,18 @@ def token_logps_and_entropy(
     named twice in a row counts twice.
 
     A differentiable call keeps the logits in 16 bits each for its backward when they take at most
-    4 GiB, and recomputes them there otherwise; ``keep_logits`` says so either way. (A kept logit is
-    within 2.6e-4 of its value, which moves the gradients by a fifteenth of their bf16 rounding. Among
-    32 neighbours of which one is within 3 % of the softcap it is within 5.1e-4, or within 1.3e-5 of the
-    softcap where it is so near itself; the softcap's slope there is within 4.2e-4 of itself. The given
-    tokens' own entries come from their f32 logits.)
+    4 GiB, and recomputes them there otherwise; ``keep_logits`` says so either way. They live as long as
+    the call's graph does, so several forwards before their backwards hold as many of them:
+    ``keep_logits=False`` trades that memory for the recompute. (A kept logit is within 2.6e-4 of its
+    value, which moves the gradients by a fifteenth of their bf16 rounding. Among 32 neighbours of which
+    one is within 3 % of the softcap it is within 5.1e-4, or within 1.3e-5 of the softcap where it is so
+    near itself; the softcap's slope there is within 4.2e-4 of itself. The given tokens' own entries come
+    from their f32 logits.)
 
     ``mesh``, ``token_chunk``, ``dh_reduce_f32`` and ``skip_zero_grad`` are those of
-    ``per_token_logps``; over a mesh the shards' statistics are exchanged by one all-gather and the
-    dH partials summed by one all-reduce. The call and its backward can be captured into a CUDA graph;
+    ``per_token_logps``, but rows without a gradient are left out only of a backward of 5e12 flops or
+    more (counted as 6 T V d), where that saves more than it costs; over a mesh the shards' statistics are
+    exchanged by one all-gather and the dH partials summed by one all-reduce. The call and its backward can be captured into a CUDA graph;
     rows without a gradient are then computed like the others, since leaving them out takes a read
     on the host. A captured backward must not meet an eager graph of the same leaves: autograd would
     tie the capture to the stream of the eager one. While such a graph of this operator lives, a
