@@ -71,7 +71,7 @@ LP_API long long lp_launch_count(void);
  * faster for it (CTA pairs on two SMs, 256x256 tiles, for the forward, the dZ recompute, dH
  * and dW; single CTAs, 128x256 tiles, for the sampler head and for the dW GEMM of a token
  * chunk of at most 1024 rows); 1 or 2 forces one group for every GEMM (also
- * LP_B200_CTA_GROUP=1|2). Results agree to f32 rounding; lp_get_cta_group() returns the
+ * LP_B200_CTA_GROUP=1|2) but those of lp_top and lp_sample_top_k, which are single CTAs. Results agree to f32 rounding; lp_get_cta_group() returns the
  * forced group or 0. */
 LP_API int lp_set_cta_group(int cg);
 LP_API int lp_get_cta_group(void);
@@ -345,7 +345,7 @@ LP_API size_t lp_top_workspace_bytes(int64_t T, int64_t V, int k);
 /*
  * The k most likely tokens of each row, 1 <= k <= min(LP_TOP_MAX, V), over the whole vocabulary.
  * They are ranked by their dot products H[t] . W[v] (to 2^-48 of sum |H W|), the lowest id first
- * among equals.
+ * among equals. One that is not finite has the log-probability NaN.
  *   tokens       int32 [T] or NULL: one given token per row
  *   ids          int32 [T, k]; logps f32 [T, k]: their log-probabilities, most likely first
  *   entropy      f32 [T]
