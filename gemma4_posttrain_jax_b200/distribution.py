@@ -302,6 +302,8 @@ def completion_logps_and_entropy(
     if hidden.stride(-1) != 1 or hidden.stride(0) % 8 or hidden.stride(1) % 8 or hidden.data_ptr() % 16:
         rows = hidden.contiguous()
     rows, tokens, idx = _ValidSlots.apply(rows, _as_int32(completion_ids), completion_mask, prompt_width - 1)
+    if rows.grad_fn is not None and hidden.is_leaf:
+        _eager_graphs.add(rows.grad_fn, [hidden])
     logps, entropy = token_logps_and_entropy(embed_tokens, rows, tokens, softcap=softcap, **options)
     slots = idx.long()
 

@@ -158,3 +158,21 @@ def test_gradients_that_are_views_or_absent(cuda_device):
     assert torch.equal(a, b) and torch.equal(a, c) and torch.equal(a, e)
     (f,) = torch.autograd.grad([entropy.sum()], [H])
     assert f.isfinite().all() and (f != 0).any()
+
+
+def test_captures_refuse_the_leaves_of_living_completions(cuda_device):
+    """A graph of completions holds its hidden states as well as the embedding."""
+    from gemma4_posttrain_jax_b200 import completion_logps_and_entropy, distribution, token_logps_and_entropy
+
+    W, H, y, _ = _inputs(cuda_device)
+    H = H.reshape(10, 15, -1)
+    W.requires_grad_(True), H.requires_grad_(True)
+    ids, mask = y[:90, 0].reshape(10, 9), torch.ones((10, 9), dtype=torch.bool, device=cuda_device)
+    alive = completion_logps_and_entropy(W, H, ids, mask, prompt_width=4, softcap=30.0)
+    assert distribution._eager_graphs.holds([W]) and distribution._eager_graphs.holds([H])
+    fixed = W.detach()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            token_logps_and_entropy(fixed, H, y.reshape(10, 15, 3), softcap=30.0)
+    del alive
+    assert not distribution._eager_graphs.holds([W]) and not distribution._eager_graphs.holds([H])
