@@ -892,10 +892,11 @@ struct DistBwdPlan {
   int cg_dz, cg_dh;
   bool split_dh;  // whether the dH GEMM may split K
   BwdLayout L;
-  size_t row_off, base;
+  size_t row_off, dh_off, base;
 };
 DistBwdPlan dist_bwd_plan(int64_t T, int64_t d, int64_t Vs, int64_t token_chunk, int flags, const DeviceInfo* di) {
   DistBwdPlan P;
+  const bool want_dh = !(flags & LP_BWD_NO_DH);
   const int64_t tc = token_chunk > 0 ? std::min<int64_t>(token_chunk, T) : default_token_chunk(T, Vs, d);
   P.cg_dz = cta_group_dist(tc, Vs, d, di, CG_DZ);
   // rows of one M tile waste half of a pair whatever the split of K; and a reduce launch takes
@@ -905,7 +906,9 @@ DistBwdPlan dist_bwd_plan(int64_t T, int64_t d, int64_t Vs, int64_t token_chunk,
   if (!P.split_dh) flags |= LP_BWD_NO_DH;  // no room for partials
   P.L = bwd_layout(T, d, Vs, token_chunk, flags, di != nullptr ? workers(di, P.cg_dh) : 148 / P.cg_dh, 128 * P.cg_dh);
   P.row_off = align_up((size_t)std::max<int64_t>(P.L.chunks, 1) * 3 * sizeof(unsigned), 1024);
-  P.base = P.row_off + align_up((size_t)T * 3 * sizeof(float), 1024);
+  P.dh_off = P.row_off + align_up((size_t)T * 3 * sizeof(float), 1024);
+  // dH of a chunk in f32, where it is not split
+  P.base = P.dh_off + (want_dh && P.L.max_splits <= 1 ? align_up((size_t)P.L.mpad * d * sizeof(float), 1024) : 0);
   return P;
 }
 
@@ -1060,6 +1063,24 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
         LP_LAUNCH_CHECK("dist_dz_kernel");
       }
     }
+    DistEntries entries{};
+    if (dist != nullptr) {
+      const int64_t at = t0 * dist->K;
+      entries.y = y + at;
+      entries.K = dist->K;
+      entries.zt = dist->zt + at;
+      entries.g = dist->g != nullptr ? dist->g + at : nullptr;
+      entries.row_const = row_const != nullptr ? row_const + t0 : nullptr;
+      entries.row_ld = T;
+      entries.ge = dist->ge != nullptr ? dist->ge + t0 : nullptr;
+      entries.lse = dist->lse + t0;
+      entries.entropy = dist->entropy + t0;
+      entries.v_off = v_off;
+      entries.Vs = Vs;
+      entries.cap = softcap;
+      entries.dz = dz;
+      entries.ldz = L.ldz;
+    }
     if (dist != nullptr && row_const != nullptr && dist->K > 0) {
       // the given tokens' entries
       ProfScope prof(st, "dist_dz_targets");
@@ -1080,6 +1101,11 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
       const int wk = workers(di, cg_dh);
       p.s = plan_gemm(tcur, d, Vs, wk, split_dh, 1, 128 * cg_dh);
       char* dh_c = reinterpret_cast<char*>(dH) + (size_t)t0 * ld_dh * (dh_f32 ? 4 : 2);
+      // with given tokens the product stays in f32 until what rounding left of their entries has joined it
+      const bool finish = dist != nullptr && dist->K > 0;
+      float* dh_part = part;
+      if (finish && p.s.k_splits == 1 && L.max_splits <= 1)
+        dh_part = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + DP.dh_off);
       if (ms != nullptr) {
         // partial tiles stored (bf16) into this rank's copy, summed across ranks by the
         // reduce items of the same launch
@@ -1097,7 +1123,7 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
         p.e.sum_rank = ms->rank;
         p.e.sum_world = ms->world;
         p.e.peer_limit_ns = ms->limit_ns;
-      } else if (p.s.k_splits == 1) {
+      } else if (p.s.k_splits == 1 && !finish) {
         if (dh_f32) {
           if ((rc = map_store_f32(&to, dh_c, d, tcur, ld_dh, "dH store", store_box_bytes(cg_dh)))) return rc;
           p.e.store_mode = STORE_F32;
@@ -1107,7 +1133,7 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
         }
         p.e.split_rows = 0;
       } else {
-        if ((rc = map_store_f32(&to, part, d, (uint64_t)p.s.k_splits * L.mpad, d, "dH partials",
+        if ((rc = map_store_f32(&to, dh_part, d, (uint64_t)p.s.k_splits * L.mpad, d, "dH partials",
                                 store_box_bytes(cg_dh))))
           return rc;
         p.e.store_mode = STORE_F32;
@@ -1116,7 +1142,12 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
       set_hints(p, G_DH);
       if (counters != nullptr) p.sched = counters++;
       if ((rc = launch_gemm<EPI_STORE, false, true, false>(st, ta, tb, to, p, di, "bwd_dh_gemm"))) return rc;
-      if (p.s.k_splits > 1) {
+      if (finish) {
+        ProfScope prof(st, "dist_dh_finish");
+        dist_dh_finish_kernel<<<(unsigned)tcur, kDistRowThreads, 0, st>>>(
+            dh_part, p.s.k_splits, L.mpad, entries, reinterpret_cast<const __nv_bfloat16*>(W), d, dh_c, ld_dh, !dh_f32);
+        LP_LAUNCH_CHECK("dist_dh_finish_kernel");
+      } else if (p.s.k_splits > 1) {
         const int64_t total = tcur * (d / 4);
         const unsigned grid = (unsigned)std::min<int64_t>(cdiv(total, 256), (int64_t)di->sms * 8);
         ProfScope prof(st, "splitk_reduce");
@@ -1149,6 +1180,11 @@ int bwd_impl(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, con
       set_hints(p, G_DW);
       if (counters != nullptr) p.sched = counters++;
       if ((rc = launch_gemm<EPI_STORE, true, true, false>(st, ta, tb, to, p, di, "bwd_dw_gemm"))) return rc;
+      if (dist != nullptr && dist->K > 0 && L.chunks == 1 && T <= kDistRowThreads && T * T * dist->K <= kDistDwRows) {
+        ProfScope prof(st, "dist_dw_rows");
+        dist_dw_rows_kernel<<<(unsigned)(T * dist->K), kDistRowThreads, 0, st>>>(entries, (int)T, Hb, ldh, d, dW, dw_bf16);
+        LP_LAUNCH_CHECK("dist_dw_rows_kernel");
+      }
     }
   }
   if (want_dw && dw_bf16 && L.chunks > 1) {
@@ -1546,6 +1582,7 @@ int check_top(const void* H, int64_t T, int64_t d, int64_t ldh, const void* W, i
 }  // namespace
 
 static_assert(kTopMax == LP_TOP_MAX, "LP_TOP_MAX");
+static_assert(LP_DIST_MAX_TOKENS <= kDistRowThreads, "a thread for each of a row's tokens");
 
 extern "C" {
 
@@ -1653,6 +1690,8 @@ int lp_dist_bwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, 
   static const int32_t none = 0;
   if (kept != nullptr && ((reinterpret_cast<uintptr_t>(kept) & 15) != 0 || kept_rows < (row_of != nullptr ? 1 : T)))
     return fail(LP_EINVAL, "kept logits must be 16-byte aligned and have a row for each row");
+  if (((reinterpret_cast<uintptr_t>(dH) | reinterpret_cast<uintptr_t>(dW)) & 15) != 0)
+    return fail(LP_EINVAL, "dH and dW must be 16-byte aligned");
   const DistGrad dg{(int)K, V, zt, lse, entropy, K > 0 ? g_logp : nullptr, g_entropy, kept, kept_rows, row_of};
   return bwd_impl(stream, H, T, d, ldh, W, Vs, v_off, K > 0 ? y : &none, softcap, nullptr, nullptr, dH, ld_dh, dW, flags,
                   token_chunk, workspace, workspace_bytes, nullptr, &dg);

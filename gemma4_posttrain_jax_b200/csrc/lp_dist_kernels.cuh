@@ -363,12 +363,12 @@ __device__ __forceinline__ uint4 dist_dz_far(uint4 kept, float slot, float cap, 
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-// The entry of a token whose slots' gradients sum to `sum`, from its f32 logit, rounded once:
+// The entry of a token whose slots' gradients sum to `sum`, from its f32 logit:
 // softcap'(z) * (sum - p * (a + b log2 p)), softcap'(z) = 1 - (z / c)^2.
-__device__ __forceinline__ __nv_bfloat16 dist_dz_given(float z, float cap, float a, float b, float l2, float sum) {
+__device__ __forceinline__ float dist_dz_given(float z, float cap, float a, float b, float l2, float sum) {
   const float lp = fmaf(z, kLog2e, -l2);
   const float u = cap > 0.f ? z / cap : 0.f;
-  return __float2bfloat16_rn(fmaf(-u, u, 1.f) * (sum - exp2f(lp) * fmaf(b, lp, a)));
+  return fmaf(-u, u, 1.f) * (sum - exp2f(lp) * fmaf(b, lp, a));
 }
 
 __global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
@@ -451,7 +451,8 @@ __global__ void __launch_bounds__(256, 8) dist_dz_kernel(const DistDzParams P) {
     }
   }
   // the row's token, where this thread has written its entry
-  if (yl >= c0 && yl < end && (yl - c0) % kDzStep < 8) dz[yl] = dist_dz_given(P.zt[t], P.cap, a, b, l2, gv);
+  if (yl >= c0 && yl < end && (yl - c0) % kDzStep < 8) 
+    dz[yl] = __float2bfloat16_rn(dist_dz_given(P.zt[t], P.cap, a, b, l2, gv));
 }
 
 // The given tokens' entries of a chunk's dZ, `sum` over the row's slots that hold the token. The first slot of a token writes the entry, so a token that a row
@@ -473,8 +474,137 @@ __global__ void dist_dz_targets_kernel(const int32_t* __restrict__ y, const floa
   if (g != nullptr)
     for (int j = k; j < K; ++j)
       if (yt[j] == id) sum += g[(size_t)t * K + j];
-  dz[(size_t)t * ldz + v] =
-      dist_dz_given(zt[i], cap, row_const[t], row_const[row_ld + t], row_const[2 * row_ld + t], sum);
+  dz[(size_t)t * ldz + v] = __float2bfloat16_rn(
+      dist_dz_given(zt[i], cap, row_const[t], row_const[row_ld + t], row_const[2 * row_ld + t], sum));
+}
+
+// The given tokens' entries are most of a row's gradient, and what rounding them to bf16 leaves (of each up
+// to 2^-8) is most of the gradients' error where few rows enter a sum. So they do not keep that rounding:
+// dH takes the rest beside the product, and the rows of dW that few rows make are summed again in f32.
+// (Error of the gradients against 64 bits, over that of rounding the exact ones to bf16, of 150 random calls,
+// most of fewer than a hundred rows: up to 2.1 with the entries as they are in dZ, at most 1.3 without their
+// rounding.)
+struct DistEntries {
+  const int32_t* y;  // [T, K]
+  int K;
+  const float *zt, *g;     // [T, K] (g or null)
+  const float* row_const;  // [3][row_ld], or null: one token per row and the pointers below
+  long long row_ld;
+  const float *ge, *lse, *entropy;
+  long long v_off, Vs;
+  float cap;
+  const __nv_bfloat16* dz;
+  long long ldz;
+};
+
+// Row t's entry in f32 if `id` is one of its tokens, else as it is in dZ; id is one of this shard's.
+__device__ __forceinline__ float dist_entry(const DistEntries& P, int t, int32_t id, bool& given) {
+  const int32_t* y = P.y + (size_t)t * P.K;
+  float sum = 0.f, z = 0.f;
+  given = false;
+  for (int k = 0; k < P.K; ++k) {
+    if (y[k] != id) continue;
+    given = true;
+    z = P.zt[(size_t)t * P.K + k];
+    if (P.g != nullptr) sum += P.g[(size_t)t * P.K + k];
+  }
+  if (!given) return __bfloat162float(P.dz[(size_t)t * P.ldz + (id - P.v_off)]);
+  float a, b, l2;
+  if (P.row_const != nullptr) {
+    a = P.row_const[t];
+    b = P.row_const[P.row_ld + t];
+    l2 = P.row_const[2 * P.row_ld + t];
+  } else {
+    const float e = P.ge != nullptr ? P.ge[t] : 0.f;
+    a = e != 0.f ? fmaf(e, P.entropy[t], sum) : sum;
+    b = e * kLn2;
+    l2 = P.lse[t] * kLog2e;
+  }
+  return dist_dz_given(z, P.cap, a, b, l2, sum);
+}
+
+// Adds f times four bf16 numbers.
+__device__ __forceinline__ void add_scaled(float4& acc, float f, const __nv_bfloat16* __restrict__ x) {
+  const uint2 v = __ldg(reinterpret_cast<const uint2*>(x));
+  acc.x = fmaf(f, __uint_as_float(v.x << 16), acc.x);
+  acc.y = fmaf(f, __uint_as_float(v.x & 0xffff0000u), acc.y);
+  acc.z = fmaf(f, __uint_as_float(v.y << 16), acc.z);
+  acc.w = fmaf(f, __uint_as_float(v.y & 0xffff0000u), acc.w);
+}
+__device__ __forceinline__ void store_row4(void* out, long long at, bool bf16, const float4& v) {
+  if (bf16)
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(out) + at) =
+        make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+  else
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at) = v;
+}
+
+// dH of row t: the product's f32 partials part [S][mpad][d] and, for each of the row's tokens once, what
+// rounding left of its entry times its row of W. One block per row; K at most the block's threads.
+constexpr int kDistRowThreads = 256;
+__global__ void __launch_bounds__(kDistRowThreads)
+    dist_dh_finish_kernel(const float* __restrict__ part, int S, long long mpad, const DistEntries P,
+                          const __nv_bfloat16* __restrict__ W, long long d, void* __restrict__ out, long long ld_out,
+                          bool out_bf16) {
+  __shared__ float left_s[kDistRowThreads];
+  __shared__ int row_s[kDistRowThreads];
+  const int t = blockIdx.x, tid = threadIdx.x;
+  if (tid < P.K) {
+    const int32_t* y = P.y + (size_t)t * P.K;
+    const long long v = (long long)y[tid] - P.v_off;
+    float left = 0.f;
+    if (v >= 0 && v < P.Vs) {
+      bool first = true, given;
+      for (int j = 0; j < tid; ++j) first &= y[j] != y[tid];
+      if (first) left = dist_entry(P, t, y[tid], given) - __bfloat162float(P.dz[(size_t)t * P.ldz + v]);
+    }
+    left_s[tid] = left;
+    row_s[tid] = left != 0.f ? (int)v : -1;
+  }
+  __syncthreads();
+  for (long long c = tid * 4; c < d; c += kDistRowThreads * 4) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < S; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(part + ((size_t)s * mpad + t) * d + c);
+      acc.x += x.x;
+      acc.y += x.y;
+      acc.z += x.z;
+      acc.w += x.w;
+    }
+#pragma unroll 4
+    for (int k = 0; k < P.K; ++k)
+      if (row_s[k] >= 0) add_scaled(acc, left_s[k], W + (size_t)row_s[k] * d + c);
+    store_row4(out, t * ld_out + c, out_bf16, acc);
+  }
+}
+
+// The given tokens' rows of dW over T rows, T at most the block's threads: dW[v] = sum over t of dZ[t, v] h[t],
+// its given entries in f32. One block per (row, slot); the first that names a token has it. It reads T rows of
+// H, so it is taken for T T K <= kDistDwRows (268 MB from L2 at d = 2048, some 30 us): with more rows the
+// roundings of their entries average out.
+constexpr int kDistDwRows = 65536;
+__global__ void __launch_bounds__(kDistRowThreads)
+    dist_dw_rows_kernel(const DistEntries P, int T, const __nv_bfloat16* __restrict__ H, long long ldh, long long d,
+                        void* __restrict__ dW, bool out_bf16) {
+  __shared__ float entry_s[kDistRowThreads];
+  const int i = blockIdx.x, tid = threadIdx.x;
+  const int32_t id = P.y[i];
+  const long long v = (long long)id - P.v_off;
+  if (v < 0 || v >= P.Vs) return;  // the whole block
+  bool earlier = false;
+  for (int j = tid; j < i; j += kDistRowThreads) earlier |= P.y[j] == id;
+  if (tid < T) {
+    bool given;
+    entry_s[tid] = dist_entry(P, tid, id, given);
+  }
+  if (__syncthreads_or(earlier)) return;
+  for (long long c = tid * 4; c < d; c += kDistRowThreads * 4) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int t = 0; t < T; ++t) add_scaled(acc, entry_s[t], H + (size_t)t * ldh + c);
+    store_row4(dW, v * d + c, out_bf16, acc);
+  }
 }
 
 // ----------------------------------------------------------------------------- selection

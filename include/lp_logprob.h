@@ -311,7 +311,8 @@ LP_API size_t lp_dist_bwd_workspace_bytes(int64_t T, int64_t d, int64_t Vs, int6
  *   dZ[t, v] = softcap'(z) * (sum_k g_logp[t, k] [y[t, k] = v]
  *                             - p * (sum_k g_logp[t, k] + g_entropy[t] * (log p + entropy[t])))
  *   dH = dZ . W (partial over this shard), dW = dZ^T . H
- * (the first sum inside the brackets runs over the ids of [0, V) only; dZ is rounded to bf16).
+ * (the sums inside the brackets run over the ids of [0, V) only). dZ is rounded to bf16, but dH, and the
+ * rows of dW that T T K <= 65536 rows and tokens make, take the given tokens' entries in f32.
  *   zt, lse, entropy   the forward's (merged over the shards)
  *   g_logp   f32 [T, K] or NULL (no gradient)      g_entropy  f32 [T] or NULL
  *   kept     the forward's kept logits of kept_rows rows, or NULL: they are recomputed. Row t's are
