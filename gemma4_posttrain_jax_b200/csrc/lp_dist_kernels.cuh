@@ -26,7 +26,15 @@ __device__ __forceinline__ float dist_logp(float z, float lse) {
   return lp > 0.f ? 0.f : lp;
 }
 
+__device__ __forceinline__ float dist_logp(double z, double lse) {
+  const float lp = (float)(z - lse);
+  return lp > 0.f ? 0.f : lp;
+}
+
 __device__ __forceinline__ float softcap_exact(float x, float cap) { return cap > 0.f ? cap * tanhf(x / cap) : x; }
+__device__ __forceinline__ double softcap_f64(double x, float cap) {
+  return cap > 0.f ? (double)cap * tanh(x / (double)cap) : x;
+}
 
 // Raw dot product h . w over one warp (every lane returns it): 16-byte loads, products of two
 // bf16 numbers are exact in f32.
@@ -119,6 +127,14 @@ __device__ __forceinline__ double warp_dot_exact(const __nv_bfloat16* __restrict
     a.add(x);
   }
   return (double)a.s + (double)a.e;
+}
+
+// The same; two-sums of infinities are NaN, for which the f32 sum stands in (an infinity, or NaN).
+__device__ __forceinline__ double warp_score(const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ w,
+                                             long long d, int lane) {
+  double z = warp_dot_exact(h, w, d, lane);
+  if (__any_sync(0xffffffffu, lane == 0 && z != z)) z = warp_dot(h, w, d, lane);
+  return z;
 }
 
 // Merges the GEMM's partials of R consecutive rows per block and computes the given tokens'
@@ -1005,10 +1021,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
       __syncthreads();
 #pragma unroll 1
       for (int i = have + warp; i < count; i += kWarps) {
-        const __nv_bfloat16* w = P.W + (size_t)cand_id[i] * P.d;
-        double z = warp_dot_exact(h, w, P.d, lane);
-        // two-sums of infinities are NaN; their place is that of the infinity
-        if (__any_sync(0xffffffffu, lane == 0 && z != z)) z = warp_dot(h, w, P.d, lane);
+        const double z = warp_score(h, P.W + (size_t)cand_id[i] * P.d, P.d, lane);
         if (lane == 0) cand_z[i] = ordered_i64(z);
       }
       __syncthreads();
@@ -1076,27 +1089,35 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
     s += red_s[1][w];
     a += red_s[2][w];
   }
-  const DistAcc acc{m, s, a};
-  const float lse = dist_lse(acc);
   if (tid < P.k) {
     double x = ordered_f64(best_i[tid]);
     // a score that is not finite answers NaN: the softcap would bring it back to +-c
     if (isinf(x)) x = NAN;
-    if constexpr (SAMPLE) best_z[tid] = P.cap > 0.f ? (double)P.cap * tanh(x / (double)P.cap) : x;
-    else best_z[tid] = (double)softcap_exact((float)x, P.cap);
+    best_z[tid] = softcap_f64(x, P.cap);
   }
   __syncthreads();
+  // The sums, with the best token's terms (1 of S, 0 of A) taken from its exact logit: the GEMM's is off by the
+  // accumulation and the softcap's fast functions (1e-5 at c = 50), which would be all that is left of the
+  // log-probability of a token that has nearly all of the mass.
+  const double z_gemm = (double)m * 0.6931471805599453;
+  double off = best_z[0] - z_gemm;
+  if (!isfinite(off)) off = 0.;
+  const double more = expm1(off), sum = (double)s + more, log_sum = log(sum);
+  const double lse = z_gemm + log_sum;
 
   if constexpr (!SAMPLE) {
     for (int j = tid; j < P.k; j += kTopThreads) {
       P.ids[(size_t)t * P.k + j] = best_id[j];
-      P.logps[(size_t)t * P.k + j] = dist_logp((float)best_z[j], lse);
+      P.logps[(size_t)t * P.k + j] = dist_logp(best_z[j], lse);
     }
-    if (tid == 0) P.entropy[t] = dist_entropy(acc);
+    if (tid == 0) {
+      const float entropy = (float)(log_sum - ((double)a * 0.6931471805599453 + (1. + more) * off) / sum);
+      P.entropy[t] = entropy < 0.f ? 0.f : entropy;  // (a NaN stays a NaN)
+    }
     if (P.tokens != nullptr && warp == kTopThreads / 32 - 1) {
       const long long v = token;
       float lp = 0.f;
-      if (v >= 0 && v < P.V) lp = dist_logp(softcap_exact(warp_dot(h, P.W + (size_t)v * P.d, P.d, lane), P.cap), lse);
+      if (v >= 0 && v < P.V) lp = dist_logp(softcap_f64(warp_score(h, P.W + (size_t)v * P.d, P.d, lane), P.cap), lse);
       if (lane == 0) P.token_logps[t] = lp;
     }
   } else {
@@ -1147,7 +1168,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_select_kernel(const TopPar
     place = min((int)__reduce_add_sync(0xffffffffu, place), n_kept - 1);
     if (lane == 0) {
       P.sampled[t] = best_id[place];
-      P.logps[t] = dist_logp((float)best_z[place], lse);
+      P.logps[t] = dist_logp(best_z[place], lse);
     }
   }
 }
