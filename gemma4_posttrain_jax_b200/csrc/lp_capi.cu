@@ -1396,13 +1396,12 @@ DistFwdLayout dist_fwd_layout(int cg, int64_t T, int64_t Vs, int64_t d, const De
   L.total = L.keys_off + align_up((size_t)T * key_row_bytes, 256);
   return L;
 }
-DistFwdLayout dist_fwd_layout(int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di, size_t key_row_bytes) {
-  return dist_fwd_layout(cta_group_dist(T, Vs, d, di, CG_FWD), T, Vs, d, di, key_row_bytes);
+DistFwdLayout dist_fwd_layout(int64_t T, int64_t Vs, int64_t d, const DeviceInfo* di) {
+  return dist_fwd_layout(cta_group_dist(T, Vs, d, di, CG_FWD), T, Vs, d, di, 0);
 }
 // Enough for any hidden size, whichever CTA group that leads to.
-size_t dist_fwd_bytes(int64_t T, int64_t Vs, const DeviceInfo* di, size_t key_row_bytes) {
-  return std::max(dist_fwd_layout(1, T, Vs, 64, di, key_row_bytes).total,
-                  dist_fwd_layout(2, T, Vs, 64, di, key_row_bytes).total);
+size_t dist_fwd_bytes(int64_t T, int64_t Vs, const DeviceInfo* di) {
+  return std::max(dist_fwd_layout(1, T, Vs, 64, di, 0).total, dist_fwd_layout(2, T, Vs, 64, di, 0).total);
 }
 
 // Rows of the hidden operand's box: of a single M tile only the rows there are (in eights, the
@@ -1590,7 +1589,7 @@ size_t lp_dist_fwd_workspace_bytes(int64_t T, int64_t Vs) {
   DeviceInfo* di = nullptr;
   const bool have = current_device_info(&di) == LP_OK;
   if (T <= 0 || Vs <= 0) return 256;
-  return dist_fwd_bytes(T, Vs, have ? di : nullptr, 0);
+  return dist_fwd_bytes(T, Vs, have ? di : nullptr);
 }
 
 size_t lp_dist_kept_bytes(int64_t T, int64_t Vs) {
@@ -1605,7 +1604,7 @@ int lp_dist_fwd(void* stream, const void* H, int64_t T, int64_t d, int64_t ldh, 
   if (T == 0) return LP_OK;
   DeviceInfo* di = nullptr;
   if ((rc = current_device_info(&di))) return rc;
-  const DistFwdLayout L = dist_fwd_layout(T, Vs, d, di, 0);
+  const DistFwdLayout L = dist_fwd_layout(T, Vs, d, di);
   if (workspace == nullptr || workspace_bytes < L.total)
     return fail(LP_EWORKSPACE, "lp_dist_fwd needs %zu workspace bytes, got %zu", L.total, workspace_bytes);
   if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return fail(LP_EINVAL, "workspace must be 256-byte aligned");
